@@ -8,7 +8,7 @@ import os
 
 from . import build as _build
 
-_i32, _i64, _vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p
+_i32, _i64, _vp, _f32 = ctypes.c_int32, ctypes.c_int64, ctypes.c_void_p, ctypes.c_float
 
 FG_OK = 0
 ERROR_NAMES = {1: "invalid argument", 2: "CUDA error", 3: "out of device memory", 4: "bad index"}
@@ -47,6 +47,23 @@ SIGNATURES = {
     "fg_gather_rows_f32": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i32, _vp, _i64, _vp]),
     "fg_csr_validate": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, _vp]),
     "fg_coo_validate": (ctypes.c_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp]),
+    "fg_rms_norm": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _f32, _i32, _i32, _i32, _vp]),
+    "fg_quantize_rows": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i32, _i32, _vp]),
+    "fg_rms_norm_backward_blocks": (_i64, [_i64, _i32]),
+    "fg_rms_norm_backward": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i32, _f32, _i32, _i32,
+                                            _vp]),
+    "fg_route": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "fg_route_backward": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "fg_group_rows_workspace": (_i64, [_i64, _i32]),
+    "fg_group_rows": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "fg_grouped_matmul_workspace": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    "fg_grouped_matmul": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i64, _vp, _i64, _i32, _i32, _i32,
+                                         _i32, _i32, _vp, _i64, _vp]),
+    "fg_grouped_matmul_wgrad_workspace": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    "fg_grouped_matmul_wgrad": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64,
+                                               _vp]),
+    "fg_combine_rows": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp]),
+    "fg_combine_rows_backward": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _i32, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _vp]),
 }
 
 _lib = None

@@ -1,0 +1,414 @@
+// Root-mean-square norm of rows with the residual's addition, its 8-bit form, and its gradient.
+//
+//   h = round(x + residual)      y = h * r * w,   r = 1 / sqrt(mean(h^2) + eps)
+//   8 bits: s = max|h r w| / 448 (1 for a row of zeros),  q = e4m3(h r w / s)
+//   dx = dresidual = dh + r g - h r^3 / d * sum(g h),  g = dy w;      dw = sum over rows of dy h r
+//
+// Bound: device memory - each array is touched once.  TPR threads own a row and hold its E values each in
+// registers between the reductions and the output, so a row is read once whatever is computed from it (its sum of
+// squares, its largest value, its products with the incoming gradient); a row wider than TPR * E goes to the next
+// larger TPR.  The statistics are recomputed from h in the backward pass: h has to be read there in any case, and a
+// saved r would be one more array.  All sums are 32-bit; h is rounded to its type before it is normalised, because
+// the rounded value is what the following layers add to and what the backward pass reads.
+//
+// dw: each block adds the rows it walks into registers (a fixed row sequence per block) and writes one partial row;
+// a second kernel adds the partial rows in order.  No atomics: the same bits on every run.
+#include <climits>
+
+#include "rows.cuh"
+
+namespace {
+
+using fg::from_f32;
+using fg::load_pack;
+using fg::Pack;
+using fg::store_pack;
+using fg::to_f32;
+
+constexpr int kE4M3Max = 448;
+
+// Sum / maximum over the TPR threads of a row; `slot` picks a buffer so that two reductions in a row need no
+// barrier between them.
+template <int TPR, bool MAX>
+__device__ __forceinline__ float row_reduce(float v, float* buffer) {
+    v = MAX ? fg::warp_max(v) : fg::warp_sum(v);
+    if (TPR == 32) return v;
+    constexpr int kWarps = TPR / 32;
+    const int warp = threadIdx.x >> 5, first = (threadIdx.x / TPR) * kWarps;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) buffer[warp] = v;
+    __syncthreads();
+    v = buffer[first];
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) {
+        const float w = buffer[first + i];
+        if (MAX) v = (w > v || w != w) ? w : v;
+        else v = __fadd_rn(v, w);
+    }
+    return v;
+}
+
+__device__ __forceinline__ float weight_at(const void* w, bool f32, int i, float) {
+    return w == nullptr ? 1.0f : static_cast<const float*>(w)[i];
+}
+template <typename T>
+__device__ __forceinline__ float weight_at(const void* w, bool f32, int i, T) {
+    if (w == nullptr) return 1.0f;
+    return f32 ? static_cast<const float*>(w)[i] : to_f32<T>(static_cast<const T*>(w)[i]);
+}
+
+struct NormArgs {
+    const void *x, *residual, *weight;
+    void *h, *y;
+    float* scales;
+    int64_t ldx, ldr, n;
+    int32_t d;
+    float eps;
+    bool weight_f32, normalize, e4m3;
+};
+
+template <typename T, int VEC, int TPR, int E>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_kernel(const NormArgs a) {
+    constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR, NV = E / VEC;
+    __shared__ float buffer[kThreads / 32];
+    const int t = threadIdx.x % TPR;
+    const int64_t row = (int64_t)blockIdx.x * kRows + threadIdx.x / TPR;
+    const bool live = row < a.n;  // a dead row still takes part in the barriers
+    const T* x = static_cast<const T*>(a.x) + (live ? row : 0) * a.ldx;
+    float v[E];
+    Pack<T, VEC> px[NV];
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        const int i = (c * TPR + t) * VEC;
+        if (live && i < a.d) px[c] = load_pack<T, VEC>(x + i);
+    }
+    if (a.residual != nullptr) {
+        const T* res = static_cast<const T*>(a.residual) + (live ? row : 0) * a.ldr;
+        T* h = static_cast<T*>(a.h) + row * a.d;
+        Pack<T, VEC> pr[NV];
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int i = (c * TPR + t) * VEC;
+            if (live && i < a.d) pr[c] = load_pack<T, VEC>(res + i);
+        }
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int i = (c * TPR + t) * VEC;
+            if (live && i < a.d) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    px[c].v[j] = from_f32<T>(__fadd_rn(to_f32<T>(px[c].v[j]), to_f32<T>(pr[c].v[j])));
+                store_pack<T, VEC>(h + i, px[c]);
+            }
+        }
+    }
+    float ss = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        const int i = (c * TPR + t) * VEC;
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const float u = (live && i < a.d) ? to_f32<T>(px[c].v[j]) : 0.0f;
+            v[c * VEC + j] = u;
+            ss = __fmaf_rn(u, u, ss);
+        }
+    }
+    if (a.normalize) {
+        ss = row_reduce<TPR, false>(ss, buffer);
+        const float r = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.d), a.eps));
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int i = (c * TPR + t) * VEC;
+            if (i < a.d) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j)
+                    v[c * VEC + j] = __fmul_rn(__fmul_rn(v[c * VEC + j], r), weight_at(a.weight, a.weight_f32, i + j, T()));
+            }
+        }
+    }
+    if (!a.e4m3) {
+        T* y = static_cast<T*>(a.y) + row * a.d;
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int i = (c * TPR + t) * VEC;
+            if (live && i < a.d) {
+                Pack<T, VEC> o;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) o.v[j] = from_f32<T>(v[c * VEC + j]);
+                store_pack<T, VEC>(y + i, o);
+            }
+        }
+        return;
+    }
+    float most = 0.0f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const float u = fabsf(v[e]);
+        most = (u > most || u != u) ? u : most;
+    }
+    most = row_reduce<TPR, true>(most, buffer);
+    const float scale = most == 0.0f ? 1.0f : __fdiv_rn(most, (float)kE4M3Max);
+    uint8_t* q = static_cast<uint8_t*>(a.y) + row * a.d;
+    if (live && t == 0) a.scales[row] = scale;
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        const int i = (c * TPR + t) * VEC;
+        if (live && i < a.d) {
+            Pack<uint8_t, VEC> o;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j)
+                o.v[j] = __nv_cvt_float_to_fp8(__fdiv_rn(v[c * VEC + j], scale), __NV_SATFINITE, __NV_E4M3);
+            store_pack<uint8_t, VEC>(q + i, o);
+        }
+    }
+}
+
+struct NormGradArgs {
+    const void *h, *weight, *dy, *dh;
+    void* dx;
+    float* partial;  // [gridDim.x, d], or NULL where the weight's gradient is not wanted
+    int64_t ldh, lddy, lddh, n;
+    int32_t d;
+    float eps;
+    bool weight_f32;
+};
+
+template <typename T, int VEC, int TPR, int E>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(const NormGradArgs a) {
+    constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR, NV = E / VEC;
+    __shared__ float buffer[2][kThreads / 32];
+    __shared__ float across[kRows > 1 ? kRows * TPR * E : 1];
+    const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    float acc[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
+    for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.n; base += (int64_t)gridDim.x * kRows) {
+        const int64_t row = base + sub;
+        const bool live = row < a.n;
+        const T* h = static_cast<const T*>(a.h) + (live ? row : 0) * a.ldh;
+        const T* dy = static_cast<const T*>(a.dy) + (live ? row : 0) * a.lddy;
+        Pack<T, VEC> ph[NV], pg[NV], pd[NV];
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int i = (c * TPR + t) * VEC;
+            if (live && i < a.d) {
+                ph[c] = load_pack<T, VEC>(h + i);
+                pg[c] = load_pack<T, VEC>(dy + i);
+            }
+        }
+        if (a.dh != nullptr) {
+            const T* dh = static_cast<const T*>(a.dh) + (live ? row : 0) * a.lddh;
+#pragma unroll
+            for (int c = 0; c < NV; ++c) {
+                const int i = (c * TPR + t) * VEC;
+                if (live && i < a.d) pd[c] = load_pack<T, VEC>(dh + i);
+            }
+        }
+        float ss = 0.0f, sg = 0.0f;
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int i = (c * TPR + t) * VEC;
+            if (live && i < a.d) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float u = to_f32<T>(ph[c].v[j]);
+                    const float g = __fmul_rn(to_f32<T>(pg[c].v[j]), weight_at(a.weight, a.weight_f32, i + j, T()));
+                    ss = __fmaf_rn(u, u, ss);
+                    sg = __fmaf_rn(u, g, sg);
+                }
+            }
+        }
+        ss = row_reduce<TPR, false>(ss, buffer[0]);
+        sg = row_reduce<TPR, false>(sg, buffer[1]);
+        const float r = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.d), a.eps));
+        const float along = __fmul_rn(__fmul_rn(r, r), __fmul_rn(r, __fdiv_rn(sg, (float)a.d)));
+        T* dx = static_cast<T*>(a.dx) + row * a.d;
+#pragma unroll
+        for (int c = 0; c < NV; ++c) {
+            const int i = (c * TPR + t) * VEC;
+            if (live && i < a.d) {
+                Pack<T, VEC> o;
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) {
+                    const float u = to_f32<T>(ph[c].v[j]), dyj = to_f32<T>(pg[c].v[j]);
+                    const float g = __fmul_rn(dyj, weight_at(a.weight, a.weight_f32, i + j, T()));
+                    float v = __fmaf_rn(-u, along, __fmul_rn(r, g));
+                    if (a.dh != nullptr) v = __fadd_rn(v, to_f32<T>(pd[c].v[j]));
+                    o.v[j] = from_f32<T>(v);
+                    acc[c * VEC + j] = __fmaf_rn(dyj, __fmul_rn(u, r), acc[c * VEC + j]);
+                }
+                store_pack<T, VEC>(dx + i, o);
+            }
+        }
+    }
+    if (a.partial == nullptr) return;
+    float* out = a.partial + (int64_t)blockIdx.x * a.d;
+    if (kRows > 1) {  // the block's row groups hold the same columns: add them in order
+        for (int e = 0; e < E; ++e) across[(sub * E + e) * TPR + t] = acc[e];
+        __syncthreads();
+        if (sub != 0) return;
+        for (int s = 1; s < kRows; ++s)
+            for (int e = 0; e < E; ++e) acc[e] = __fadd_rn(acc[e], across[(s * E + e) * TPR + t]);
+    }
+#pragma unroll
+    for (int c = 0; c < NV; ++c) {
+        const int i = (c * TPR + t) * VEC;
+        for (int j = 0; j < VEC; ++j)
+            if (i + j < a.d) out[i + j] = acc[c * VEC + j];
+    }
+}
+
+// dw[c] = sum of partial[0 .. rows)[c]: 32 columns a block, 8 row sequences each, joined in order.
+template <typename W>
+__global__ void __launch_bounds__(256) weight_grad_kernel(const float* __restrict__ partial, int rows, int d, W* __restrict__ dw) {
+    __shared__ float part[8][33];
+    const int lane = threadIdx.x & 31, seq = threadIdx.x >> 5;
+    const int c = blockIdx.x * 32 + lane;
+    float s = 0.0f;
+    if (c < d)
+        for (int r = seq; r < rows; r += 8) s = __fadd_rn(s, partial[(int64_t)r * d + c]);
+    part[seq][lane] = s;
+    __syncthreads();
+    if (seq == 0 && c < d) {
+        for (int q = 1; q < 8; ++q) s = __fadd_rn(s, part[q][lane]);
+        dw[c] = from_f32<W>(s);
+    }
+}
+
+constexpr int kMaxWidth = 16384;
+
+// Calls f.template operator()<T, VEC, TPR, E>() with the smallest TPR * E that covers d.
+template <typename T, int VEC, typename F>
+void by_width(int d, F&& f) {
+    if (d <= 256) f.template operator()<T, VEC, 32, 8>();
+    else if (d <= 512) f.template operator()<T, VEC, 32, 16>();
+    else if (d <= 1024) f.template operator()<T, VEC, 64, 16>();
+    else if (d <= 2048) f.template operator()<T, VEC, 128, 16>();
+    else if (d <= 4096) f.template operator()<T, VEC, 256, 16>();
+    else if (d <= 8192) f.template operator()<T, VEC, 512, 16>();
+    else f.template operator()<T, VEC, 1024, 16>();
+}
+template <typename F>
+void by_type(int32_t type, bool vec, int d, F&& f) {
+    if (type == FG_F32) vec ? by_width<float, 4>(d, f) : by_width<float, 1>(d, f);
+    else if (type == FG_F16) vec ? by_width<__half, 8>(d, f) : by_width<__half, 1>(d, f);
+    else vec ? by_width<__nv_bfloat16, 8>(d, f) : by_width<__nv_bfloat16, 1>(d, f);
+}
+
+int rows_per_block(int d) { return d <= 512 ? 8 : d <= 1024 ? 4 : d <= 2048 ? 2 : 1; }
+
+// 128-bit accesses need every row to start on a 16-byte boundary.
+bool vector_rows(const void* p, int64_t ld, int32_t type) {
+    return p == nullptr || (fg::aligned16(p) && (ld * fg::type_size(type)) % 16 == 0);
+}
+
+struct LaunchNorm {
+    const NormArgs& a;
+    cudaStream_t s;
+    template <typename T, int VEC, int TPR, int E>
+    void operator()() const {
+        constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR;
+        norm_kernel<T, VEC, TPR, E><<<(unsigned)((a.n + kRows - 1) / kRows), kThreads, 0, s>>>(a);
+    }
+};
+struct LaunchNormGrad {
+    const NormGradArgs& a;
+    unsigned blocks;
+    cudaStream_t s;
+    template <typename T, int VEC, int TPR, int E>
+    void operator()() const {
+        norm_grad_kernel<T, VEC, TPR, E><<<blocks, TPR < 256 ? 256 : TPR, 0, s>>>(a);
+    }
+};
+
+int launch_norm(NormArgs& a, int32_t type, void* stream) {
+    const bool vec = a.d % (16 / fg::type_size(type)) == 0 && vector_rows(a.x, a.ldx, type) &&
+                     vector_rows(a.residual, a.ldr, type) && vector_rows(a.h, a.d, type) && fg::aligned16(a.y);
+    by_type(type, vec, a.d, LaunchNorm{a, static_cast<cudaStream_t>(stream)});
+    FG_CUDA_TRY(cudaGetLastError());
+    fg::count_launches(1);
+    return FG_OK;
+}
+
+int check_rows(int64_t n, int32_t d, int32_t type) {
+    if (n < 0 || n > INT_MAX || d < 1 || d > kMaxWidth)
+        return fg::fail(FG_ERR_INVALID_ARGUMENT, "bad sizes n=%lld d=%d (1 <= d <= %d)", (long long)n, d, kMaxWidth);
+    if (!fg::float_type(type)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "unknown value type %d", type);
+    return FG_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int fg_rms_norm(const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, const void* d_weight, void* d_h, void* d_y,
+                float* d_scales, int64_t n, int32_t d, float eps, int32_t type, int32_t weight_type, int32_t out_type,
+                void* stream) {
+    if (int rc = check_rows(n, d, type)) return rc;
+    if (d_weight && weight_type != type && weight_type != FG_F32)
+        return fg::fail(FG_ERR_INVALID_ARGUMENT, "the weight is of the rows' type or fp32");
+    if (out_type != type && out_type != FG_E4M3) return fg::fail(FG_ERR_INVALID_ARGUMENT, "the output is of the rows' type or e4m3");
+    if (!(eps >= 0.0f)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "eps must be >= 0");
+    if (ldx == 0) ldx = d;
+    if (ldr == 0) ldr = d;
+    if (ldx < d || ldr < d) return fg::fail(FG_ERR_INVALID_ARGUMENT, "row strides must be 0 or >= d=%d", d);
+    if (n == 0) return FG_OK;
+    if (!d_x || !d_y || (d_residual && !d_h) || (out_type == FG_E4M3 && !d_scales))
+        return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
+    NormArgs a{d_x, d_residual, d_weight, d_h, d_y, d_scales, ldx, ldr, n, d, eps, weight_type == FG_F32, true, out_type == FG_E4M3};
+    return launch_norm(a, type, stream);
+}
+
+int fg_quantize_rows(const void* d_x, int64_t ldx, void* d_y, float* d_scales, int64_t n, int32_t d, int32_t type, void* stream) {
+    if (int rc = check_rows(n, d, type)) return rc;
+    if (ldx == 0) ldx = d;
+    if (ldx < d) return fg::fail(FG_ERR_INVALID_ARGUMENT, "row strides must be 0 or >= d=%d", d);
+    if (n == 0) return FG_OK;
+    if (!d_x || !d_y || !d_scales) return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
+    NormArgs a{d_x, nullptr, nullptr, nullptr, d_y, d_scales, ldx, 0, n, d, 0.0f, true, false, true};
+    return launch_norm(a, type, stream);
+}
+
+int64_t fg_rms_norm_backward_blocks(int64_t n, int32_t d) {
+    if (n < 1 || d < 1) return 0;
+    const int rows = rows_per_block(d);
+    const int64_t want = (n + rows - 1) / rows, most = (int64_t)fg::device_props().sm_count * (d <= 4096 ? 4 : d <= 8192 ? 2 : 1);
+    return want < most ? want : most;
+}
+
+int fg_rms_norm_backward(const void* d_h, int64_t ldh, const void* d_weight, const void* d_dy, int64_t lddy, const void* d_dh,
+                         int64_t lddh, void* d_dx, void* d_dweight, float* d_partial, int64_t blocks, int64_t n, int32_t d,
+                         float eps, int32_t type, int32_t weight_type, void* stream) {
+    if (int rc = check_rows(n, d, type)) return rc;
+    if (d_weight && weight_type != type && weight_type != FG_F32)
+        return fg::fail(FG_ERR_INVALID_ARGUMENT, "the weight is of the rows' type or fp32");
+    if (ldh == 0) ldh = d;
+    if (lddy == 0) lddy = d;
+    if (lddh == 0) lddh = d;
+    if (ldh < d || lddy < d || lddh < d) return fg::fail(FG_ERR_INVALID_ARGUMENT, "row strides must be 0 or >= d=%d", d);
+    if (n == 0) {
+        if (d_dweight)
+            FG_CUDA_TRY(cudaMemsetAsync(d_dweight, 0, (size_t)d * fg::type_size(weight_type), static_cast<cudaStream_t>(stream)));
+        return FG_OK;
+    }
+    if (!d_h || !d_dy || !d_dx || (d_dweight && !d_partial)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
+    if (blocks < 1 || blocks > INT_MAX) return fg::fail(FG_ERR_INVALID_ARGUMENT, "blocks must come from fg_rms_norm_backward_blocks");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    NormGradArgs a{d_h, d_weight, d_dy, d_dh, d_dx, d_dweight ? d_partial : nullptr, ldh, lddy, lddh, n, d, eps, weight_type == FG_F32};
+    const bool vec = d % (16 / fg::type_size(type)) == 0 && vector_rows(d_h, ldh, type) && vector_rows(d_dy, lddy, type) &&
+                     vector_rows(d_dh, lddh, type) && fg::aligned16(d_dx);
+    by_type(type, vec, d, LaunchNormGrad{a, (unsigned)blocks, s});
+    FG_CUDA_TRY(cudaGetLastError());
+    fg::count_launches(1);
+    if (d_dweight) {
+        const unsigned grid = (unsigned)((d + 31) / 32);
+        if (weight_type == FG_F32) weight_grad_kernel<float><<<grid, 256, 0, s>>>(d_partial, (int)blocks, d, static_cast<float*>(d_dweight));
+        else if (weight_type == FG_F16) weight_grad_kernel<__half><<<grid, 256, 0, s>>>(d_partial, (int)blocks, d, static_cast<__half*>(d_dweight));
+        else weight_grad_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(d_partial, (int)blocks, d, static_cast<__nv_bfloat16*>(d_dweight));
+        FG_CUDA_TRY(cudaGetLastError());
+        fg::count_launches(1);
+    }
+    return FG_OK;
+}
+
+}  // extern "C"

@@ -8,3 +8,7 @@ VanillaSDDMM = VanillaSDDMMcuda
 # SpMM followed by SDDMM on its output, in one pass (no counterpart class in the reference: it runs the two
 # modules above back to back)
 from .fused import AggregateThenScore
+
+# what a layer with several experts, node types or relations computes densely around them (module/rows.py)
+from .rows import (QuantizedRows, Routing, RowGroups, combine_rows, group_rows, grouped_matmul, quantize_rows,
+                   rms_norm, route)

@@ -1,0 +1,462 @@
+"""Row operators that stand around the sparse ones in a layer with several experts, node types or relations.
+
+The reference covers the sparse half of a graph layer (aggregation and edge scores); these cover what such a layer
+computes densely before and after it, with their gradients:
+
+    y, h = rms_norm(x, weight, residual=res)            # pre-norm on a residual stream
+    r    = route(logits, k)                             # k of G experts a row, and the rows' lists by expert
+    z    = grouped_matmul(y, W, r.groups, gather=True)  # one weight [out, in] an expert
+    out  = combine_rows(z, r.groups, r.weights)         # weighted sum back, row order
+
+A relation- or type-specific transform is the same with ``groups = group_rows(types, num_types)`` in the place of the
+router.  ``rms_norm(..., quantize=True)`` gives 8-bit rows with a scale each (``QuantizedRows``), which
+``grouped_matmul`` takes together with 8-bit weights.
+
+All functions run on the current stream, allocate their outputs and workspaces there, never synchronise, and may be
+captured into a CUDA graph (``featgraph_b200.graph_capture``).  A captured backward pass goes through
+``torch.autograd.grad`` and returns detached outputs: torch ties a leaf's gradient accumulation to the stream of its
+first live graph, so no graph of an eager step on the same leaves may be alive while a step is captured.
+
+Types: float32, float16, bfloat16; sums are 32-bit and each output is rounded once.  No atomics on values: the same bits on
+every run.
+"""
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _device as dev
+
+_TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4m3fn: 3}
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
+_SCORING = {"softmax": 0, "sigmoid": 1}
+MAX_WIDTH, MAX_GROUPS, MAX_CHOICES = 16384, 1024, 32
+
+
+class QuantizedRows(NamedTuple):
+    """8-bit rows: ``values`` (float8_e4m3fn) [..., d] times ``scales`` (float32) [...]."""
+    values: torch.Tensor
+    scales: torch.Tensor
+
+
+class RowGroups:
+    """The lists of ``group_rows``: slots ``offsets[g] .. offsets[g + 1]`` belong to group g, ``order[slot]`` is the
+    entry (row * k + choice) that a slot holds, ``position`` [n, k] the slot of each entry.  Entries in no group have
+    position -1; the slots from ``offsets[-1]`` on hold -1.  All int32, on one device.  The lists are trusted to
+    be such a pair of permutations; values out of range are treated as -1."""
+    __slots__ = ("offsets", "order", "position")
+
+    def __init__(self, offsets, order, position):
+        for name, t in (("offsets", offsets), ("order", order), ("position", position)):
+            if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or not t.is_contiguous() or t.device != offsets.device:
+                raise ValueError("%s must be a contiguous int32 tensor, on one device with the others" % name)
+        if offsets.dim() != 1 or not 2 <= offsets.numel() <= MAX_GROUPS + 1:
+            raise ValueError("offsets must have 2 to %d values" % (MAX_GROUPS + 1))
+        if position.dim() != 2 or order.dim() != 1 or order.numel() != position.numel() or not 1 <= position.shape[1] <= MAX_CHOICES:
+            raise ValueError("order [n k] and position [n, k], 1 <= k <= %d, must list the same entries" % MAX_CHOICES)
+        self.offsets, self.order, self.position = offsets, order, position
+
+    @property
+    def num_groups(self):
+        return self.offsets.numel() - 1
+
+    @property
+    def num_entries(self):
+        return self.order.numel()
+
+    @property
+    def num_rows(self):
+        return self.position.shape[0]
+
+    @property
+    def choices(self):
+        return self.position.shape[1]
+
+
+class Routing(NamedTuple):
+    """``weights`` [n, k] (float32, differentiable), ``experts`` [n, k] (int32, -1 where a row ran out of open
+    experts) and the ``RowGroups`` of the experts."""
+    weights: torch.Tensor
+    experts: torch.Tensor
+    groups: RowGroups
+
+
+def _call(name, device, *args):
+    fn = getattr(dev.lib(), name)
+    if torch.cuda.current_device() == device.index:
+        dev.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+    else:
+        with torch.cuda.device(device):
+            dev.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _tensor(t, what, dtypes, dims=None):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s: expected a torch.Tensor, got %r" % (what, type(t)))
+    if t.dtype not in dtypes:
+        raise TypeError("%s must be %s, got %s" % (what, " or ".join(str(d).replace("torch.", "") for d in dtypes), t.dtype))
+    if dims is not None and t.dim() != dims:
+        raise ValueError("%s must have %d dimensions, has shape %s" % (what, dims, tuple(t.shape)))
+    return t
+
+
+def _on(device, **tensors):
+    dev.resolve_device(device)
+    for what, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError("%s lives on %s, the rows on %s" % (what, t.device, device))
+
+
+def _as_rows(t):
+    """t as a 2-D tensor whose rows are dense (a row stride of its own is kept), and that stride."""
+    if t.dim() != 2:
+        t = t.reshape(-1, t.shape[-1]) if t.dim() else t
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def _wants_grad(*tensors):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+# ---- norm ----
+
+def _norm_forward(x, weight, residual, eps, quantize):
+    shape, d = x.shape, x.shape[-1]
+    xr, ldx = _as_rows(x)
+    n = xr.shape[0]
+    rr, ldr = (None, 0) if residual is None else _as_rows(residual)
+    h = None if residual is None else torch.empty((n, d), dtype=x.dtype, device=x.device)
+    y = torch.empty((n, d), dtype=torch.float8_e4m3fn if quantize else x.dtype, device=x.device)
+    scales = torch.empty((n,), dtype=torch.float32, device=x.device) if quantize else None
+    kind = _TYPES[x.dtype]
+    _call("fg_rms_norm", x.device, xr.data_ptr(), ldx, _ptr(rr), ldr, _ptr(weight), _ptr(h), y.data_ptr(), _ptr(scales), n, d, eps, kind,
+          kind if weight is None else _TYPES[weight.dtype], 3 if quantize else kind)
+    return y.view(shape), None if h is None else h.view(shape), None if scales is None else scales.view(shape[:-1])
+
+
+class _Norm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        y, h, _ = _norm_forward(x, weight, residual, eps, False)
+        ctx.eps = eps
+        ctx.save_for_backward(x if h is None else h, weight)
+        ctx.set_materialize_grads(False)
+        return (y, h) if h is not None else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dh=None):
+        h, weight = ctx.saved_tensors
+        if dy is None:  # only the sum was used
+            return (dh if ctx.needs_input_grad[0] else None, None if weight is None else torch.zeros_like(weight),
+                    dh if ctx.needs_input_grad[2] else None, None)
+        d = h.shape[-1]
+        hr, ldh = _as_rows(h)
+        gr, ldg = _as_rows(dy)
+        sr, lds = (None, 0) if dh is None else _as_rows(dh)
+        n = hr.shape[0]
+        dx = torch.empty((n, d), dtype=h.dtype, device=h.device)
+        dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
+        partial = None
+        blocks = dev.lib().fg_rms_norm_backward_blocks(n, d)
+        if dw is not None:
+            partial = torch.empty((blocks, d), dtype=torch.float32, device=h.device)
+        kind = _TYPES[h.dtype]
+        _call("fg_rms_norm_backward", h.device, hr.data_ptr(), ldh, _ptr(weight), gr.data_ptr(), ldg, _ptr(sr), lds, dx.data_ptr(), _ptr(dw),
+              _ptr(partial), blocks, n, d, ctx.eps, kind, kind if weight is None else _TYPES[weight.dtype])
+        dx = dx.view(h.shape)
+        return dx if ctx.needs_input_grad[0] else None, dw, dx if ctx.needs_input_grad[2] else None, None
+
+
+def rms_norm(x, weight=None, residual=None, eps=1e-6, quantize=False):
+    """Root-mean-square norm of the rows of ``x`` [..., d], d <= 16384, with the residual's addition:
+
+        h = x + residual (in x's type; h = x without one)      y = h / sqrt(mean(h^2) + eps) * weight
+
+    Returns ``y``, or ``(y, h)`` with a residual: h is the stream that the next layer adds to.  ``weight`` [d] is of
+    x's type or float32 (None: ones).  ``quantize``: y as ``QuantizedRows`` (scale = max|y| / 448 a row, 1 for a
+    row of zeros; a row with an infinity or NaN has a scale that says so) - the form for serving, which has no gradient
+    and refuses inputs that want one."""
+    _tensor(x, "x", _FLOATS)
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
+        raise ValueError("x must have rows of 1 to %d values, has shape %s" % (MAX_WIDTH, tuple(x.shape)))
+    if weight is not None:
+        _tensor(weight, "weight", (x.dtype, torch.float32), 1)
+        if weight.shape[0] != x.shape[-1]:
+            raise ValueError("weight has %d values, the rows %d" % (weight.shape[0], x.shape[-1]))
+    if residual is not None:
+        _tensor(residual, "residual", (x.dtype,))
+        if residual.shape != x.shape:
+            raise ValueError("residual has shape %s, x %s" % (tuple(residual.shape), tuple(x.shape)))
+    eps = float(eps)
+    if not eps >= 0.0:
+        raise ValueError("eps must be >= 0, got %r" % eps)
+    _on(x.device, weight=weight, residual=residual)
+    if weight is not None:
+        weight = weight.contiguous()
+    if _wants_grad(x, weight, residual):
+        if quantize:
+            raise ValueError("the 8-bit output has no gradient: call it under torch.no_grad() or on detached tensors")
+        return _Norm.apply(x, weight, residual, eps)
+    y, h, scales = _norm_forward(x, weight, residual, eps, bool(quantize))
+    if quantize:
+        y = QuantizedRows(y, scales)
+    return y if h is None else (y, h)
+
+
+def quantize_rows(x):
+    """``x`` [..., d] as ``QuantizedRows``, the values that ``rms_norm(quantize=True)`` would give for y = x.  For a weight
+    [groups, out, in] that is a scale for each output of each group.  No gradient."""
+    _tensor(x, "x", _FLOATS)
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
+        raise ValueError("x must have rows of 1 to %d values, has shape %s" % (MAX_WIDTH, tuple(x.shape)))
+    _on(x.device)
+    if _wants_grad(x):
+        raise ValueError("the 8-bit output has no gradient: call it under torch.no_grad() or on detached tensors")
+    xr, ldx = _as_rows(x)
+    n, d = xr.shape
+    y = torch.empty((n, d), dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty((n,), dtype=torch.float32, device=x.device)
+    _call("fg_quantize_rows", x.device, xr.data_ptr(), ldx, y.data_ptr(), scales.data_ptr(), n, d, _TYPES[x.dtype])
+    return QuantizedRows(y.view(x.shape), scales.view(x.shape[:-1]))
+
+
+# ---- routing ----
+
+def group_rows(keys, num_groups):
+    """``RowGroups`` of entries with ``keys`` [n] or [n, k] (int32 or int64): entry row * k + j belongs to group
+    keys[row, j]; any value outside [0, num_groups) means no group.  Slots of a group hold its entries in ascending
+    order.  num_groups <= 1024, k <= 32, n k < 2^31."""
+    _tensor(keys, "keys", (torch.int32, torch.int64))
+    if keys.dim() == 1:
+        keys = keys.unsqueeze(1)
+    if keys.dim() != 2 or not 1 <= keys.shape[1] <= MAX_CHOICES:
+        raise ValueError("keys must be [n] or [n, k] with 1 <= k <= %d, have shape %s" % (MAX_CHOICES, tuple(keys.shape)))
+    num_groups = int(num_groups)
+    if not 1 <= num_groups <= MAX_GROUPS:
+        raise ValueError("num_groups must be 1 to %d, got %d" % (MAX_GROUPS, num_groups))
+    if keys.numel() >= 2 ** 31:
+        raise ValueError("%d entries: fewer than 2^31 are wanted" % keys.numel())
+    _on(keys.device)
+    if keys.dtype == torch.int64:
+        keys = keys.clamp(-1, num_groups).int()
+    return _group(keys.contiguous(), num_groups)
+
+
+def _group(keys, num_groups):
+    m, device = keys.numel(), keys.device
+    offsets = torch.empty((num_groups + 1,), dtype=torch.int32, device=device)
+    order = torch.empty((m,), dtype=torch.int32, device=device)
+    position = torch.empty_like(keys)
+    size = dev.lib().fg_group_rows_workspace(m, num_groups)
+    work = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
+    _call("fg_group_rows", device, keys.data_ptr(), m, num_groups, offsets.data_ptr(), order.data_ptr(), position.data_ptr(), _ptr(work), size)
+    return RowGroups(offsets, order, position)
+
+
+def _choose(logits, k, scoring, normalize):
+    x, ld = _as_rows(logits)
+    n, experts = x.shape
+    weights = torch.empty((n, k), dtype=torch.float32, device=x.device)
+    chosen = torch.empty((n, k), dtype=torch.int32, device=x.device)
+    _call("fg_route", x.device, x.data_ptr(), ld, weights.data_ptr(), chosen.data_ptr(), n, experts, k, _TYPES[x.dtype], scoring, normalize)
+    return weights, chosen
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, k, scoring, normalize):
+        weights, chosen = _choose(logits, k, scoring, normalize)
+        ctx.mark_non_differentiable(chosen)
+        ctx.save_for_backward(logits, weights, chosen)
+        ctx.args = (k, scoring, normalize)
+        return weights, chosen
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dweights, _):
+        logits, weights, chosen = ctx.saved_tensors
+        x, ld = _as_rows(logits)
+        dweights = dweights.contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        k, scoring, normalize = ctx.args
+        _call("fg_route_backward", x.device, x.data_ptr(), ld, weights.data_ptr(), chosen.data_ptr(), dweights.data_ptr(), dx.data_ptr(),
+              x.shape[0], x.shape[1], k, _TYPES[x.dtype], scoring, normalize)
+        return dx, None, None, None
+
+
+def route(logits, k, scoring="softmax", normalize=True):
+    """The k largest logits of each row of ``logits`` [n, experts] in descending order, ties to the lowest index, as a
+    ``Routing``.  Weights: softmax over the row, or sigmoid; ``normalize``: divided by their sum over the choice.
+    A logit of -inf or NaN is closed: never chosen and without weight; where fewer than k are open, the remaining
+    choices are -1 with weight 0.  experts <= 1024, k <= 32.  The weights are differentiable."""
+    _tensor(logits, "logits", _FLOATS, 2)
+    n, experts = logits.shape
+    k = int(k)
+    if scoring not in _SCORING:
+        raise ValueError("scoring must be 'softmax' or 'sigmoid', got %r" % (scoring,))
+    if not 1 <= experts <= MAX_GROUPS:
+        raise ValueError("1 to %d experts are possible, got %d" % (MAX_GROUPS, experts))
+    if not 1 <= k <= min(experts, MAX_CHOICES):
+        raise ValueError("k must be 1 to %d, got %d" % (min(experts, MAX_CHOICES), k))
+    if n * k >= 2 ** 31:
+        raise ValueError("%d entries: fewer than 2^31 are wanted" % (n * k))
+    _on(logits.device)
+    args = (k, _SCORING[scoring], 1 if normalize else 0)
+    weights, chosen = _Route.apply(logits, *args) if _wants_grad(logits) else _choose(logits, *args)
+    return Routing(weights, chosen, _group(chosen, experts))
+
+
+# ---- products ----
+
+def _product(x, ldx, x_scales, w, strides, w_scales, groups, gather, x_rows, inner, outer, out_dtype):
+    device, kind = x.device, _TYPES[x.dtype]
+    y = torch.empty((groups.num_entries, outer), dtype=out_dtype, device=device)
+    size = dev.lib().fg_grouped_matmul_workspace(groups.num_entries, x_rows, groups.num_groups, inner, outer, kind)
+    work = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
+    _call("fg_grouped_matmul", device, x.data_ptr(), ldx, _ptr(x_scales), w.data_ptr(), *strides, _ptr(w_scales), groups.offsets.data_ptr(),
+          groups.order.data_ptr() if gather else None, groups.choices, x_rows, y.data_ptr(), groups.num_entries, groups.num_groups, inner,
+          outer, kind, _TYPES[out_dtype], _ptr(work), size)
+    return y
+
+
+class _Product(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, groups, gather):
+        xr, ldx = _as_rows(x)
+        ctx.groups, ctx.gather = groups, gather
+        ctx.save_for_backward(x, w)
+        return _product(xr, ldx, None, w, w.stride(), None, groups, gather, x.shape[0], w.shape[2], w.shape[1], x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, w = ctx.saved_tensors
+        groups, gather = ctx.groups, ctx.gather
+        outer, inner = w.shape[1], w.shape[2]
+        dyr, ldy = _as_rows(dy)
+        dx = dw = None
+        if ctx.needs_input_grad[0]:
+            # per slot first, in x's type; with k slots a row their sum is then taken in 32 bits
+            dx = _product(dyr, ldy, None, w, (w.stride(0), w.stride(2), w.stride(1)), None, groups, False, dyr.shape[0], outer, inner, x.dtype)
+            if gather:
+                dx = _combine(dx, groups, None)
+        if ctx.needs_input_grad[1]:
+            xr, ldx = _as_rows(x)
+            kind = _TYPES[x.dtype]
+            dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
+            size = dev.lib().fg_grouped_matmul_wgrad_workspace(groups.num_entries, x.shape[0], groups.num_groups, inner, outer, kind)
+            work = torch.empty((size,), dtype=torch.uint8, device=w.device) if size else None
+            _call("fg_grouped_matmul_wgrad", x.device, xr.data_ptr(), ldx, dyr.data_ptr(), ldy, groups.offsets.data_ptr(),
+                  groups.order.data_ptr() if gather else None, groups.choices, x.shape[0], dw.data_ptr(), groups.num_entries,
+                  groups.num_groups, inner, outer, kind, _ptr(work), size)
+        return dx, dw, None, None
+
+
+def grouped_matmul(x, weight, groups, gather=False, out_dtype=None):
+    """One product for each group: ``y[p] = weight[g] @ row`` for the slots p of group g; y is [entries, out], slots in
+    no group are 0.  ``weight`` [groups, out, in] (any strides).  ``x`` [entries, in] holds a row for each slot, or, with
+    ``gather``, [n, in] the rows in their own order, of which slot p reads row order[p] // k.  The groups' sizes stay on
+    the device.  Differentiable in x and weight.
+
+    ``x`` and ``weight`` may both be ``QuantizedRows`` (scales [rows] and [groups, out]): products of the 8-bit values
+    in 32-bit sums, scaled at the end, in ``out_dtype`` (bfloat16 unless stated); no gradient."""
+    if not isinstance(groups, RowGroups):
+        raise TypeError("groups: expected RowGroups (group_rows, route), got %r" % (type(groups),))
+    eight = isinstance(x, QuantizedRows)
+    if eight != isinstance(weight, QuantizedRows):
+        raise TypeError("x and weight must both be QuantizedRows, or neither")
+    x_scales = w_scales = None
+    if eight:
+        (x, x_scales), (weight, w_scales) = x, weight
+        _tensor(x, "x.values", (torch.float8_e4m3fn,), 2)
+        _tensor(weight, "weight.values", (torch.float8_e4m3fn,), 3)
+        _tensor(x_scales, "x.scales", (torch.float32,), 1)
+        _tensor(w_scales, "weight.scales", (torch.float32,), 2)
+        if x_scales.shape != x.shape[:1] or w_scales.shape != weight.shape[:2]:
+            raise ValueError("a scale for each row of x and for each output of weight is wanted")
+        out_dtype = torch.bfloat16 if out_dtype is None else out_dtype
+        if out_dtype not in _FLOATS:
+            raise TypeError("out_dtype must be float32, float16 or bfloat16, got %s" % (out_dtype,))
+    else:
+        _tensor(x, "x", _FLOATS, 2)
+        _tensor(weight, "weight", (x.dtype,), 3)
+        if out_dtype not in (None, x.dtype):
+            raise TypeError("out_dtype is x's type (%s) unless the inputs are 8-bit" % (x.dtype,))
+        out_dtype = x.dtype
+    if weight.shape[0] != groups.num_groups:
+        raise ValueError("weight has %d groups, the rows %d" % (weight.shape[0], groups.num_groups))
+    if weight.shape[2] != x.shape[1]:
+        raise ValueError("weight takes %d values, the rows have %d" % (weight.shape[2], x.shape[1]))
+    if weight.shape[1] < 1 or weight.shape[2] < 1:
+        raise ValueError("weight has shape %s" % (tuple(weight.shape),))
+    want = groups.num_rows if gather else groups.num_entries
+    if x.shape[0] != want:
+        raise ValueError("x has %d rows, the groups %d%s" % (x.shape[0], want, "" if gather else " slots"))
+    _on(x.device, weight=weight, groups=groups.offsets, scales=x_scales, weight_scales=w_scales)
+    gather = bool(gather)
+    if not eight and _wants_grad(x, weight):
+        return _Product.apply(x, weight, groups, gather)
+    xr, ldx = _as_rows(x)
+    if eight:
+        x_scales, w_scales = x_scales.contiguous(), w_scales.contiguous()
+    return _product(xr, ldx, x_scales, weight, weight.stride(), w_scales, groups, gather, x.shape[0], weight.shape[2], weight.shape[1], out_dtype)
+
+
+# ---- weighted sum back ----
+
+def _combine(y, groups, weights):
+    yr, ldy = _as_rows(y)
+    n, k, d = groups.num_rows, groups.choices, y.shape[1]
+    out = torch.empty((n, d), dtype=y.dtype, device=y.device)
+    _call("fg_combine_rows", y.device, yr.data_ptr(), ldy, _ptr(weights), groups.position.data_ptr(), out.data_ptr(), n, k, d, _TYPES[y.dtype])
+    return out
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, groups, weights):
+        ctx.groups = groups
+        ctx.save_for_backward(y, weights)
+        return _combine(y, groups, weights)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        y, weights = ctx.saved_tensors
+        groups = ctx.groups
+        yr, ldy = _as_rows(y)
+        gr, ldd = _as_rows(dout)
+        n, k, d = groups.num_rows, groups.choices, y.shape[1]
+        dy = torch.empty((n * k, d), dtype=y.dtype, device=y.device) if ctx.needs_input_grad[0] else None
+        dw = torch.empty((n, k), dtype=torch.float32, device=y.device) if weights is not None and ctx.needs_input_grad[2] else None
+        _call("fg_combine_rows_backward", y.device, yr.data_ptr(), ldy, _ptr(weights), groups.position.data_ptr(), groups.offsets.data_ptr(),
+              groups.num_groups, gr.data_ptr(), ldd, _ptr(dy), _ptr(dw), n, k, d, _TYPES[y.dtype])
+        return dy, None, dw
+
+
+def combine_rows(y, groups, weights=None):
+    """``out[t] = sum over j of weights[t, j] * y[position[t, j]]`` for ``y`` [entries, d] in slot order: the rows of
+    ``grouped_matmul`` summed back into row order, [n, d].  Entries in no group add nothing.  ``weights`` [n, k] float32
+    (None: ones).  Differentiable in y and weights."""
+    if not isinstance(groups, RowGroups):
+        raise TypeError("groups: expected RowGroups (group_rows, route), got %r" % (type(groups),))
+    _tensor(y, "y", _FLOATS, 2)
+    if y.shape[0] != groups.num_entries or y.shape[1] < 1:
+        raise ValueError("y must have a row for each of %d slots, has shape %s" % (groups.num_entries, tuple(y.shape)))
+    if weights is not None:
+        _tensor(weights, "weights", (torch.float32,), 2)
+        if weights.shape != groups.position.shape:
+            raise ValueError("weights have shape %s, the choices %s" % (tuple(weights.shape), tuple(groups.position.shape)))
+    _on(y.device, groups=groups.offsets, weights=weights)
+    if weights is not None:
+        weights = weights.contiguous()
+    if _wants_grad(y, weights):
+        return _Combine.apply(y, groups, weights)
+    return _combine(y, groups, weights)

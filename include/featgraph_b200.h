@@ -333,6 +333,75 @@ int fg_csr_validate(const int32_t* d_indptr, const int32_t* d_indices, int64_t n
 int fg_coo_validate(const int32_t* d_row, const int32_t* d_col, int64_t n_rows, int64_t n_cols,
                     int64_t nnz, int32_t* rows_sorted, void* stream);
 
+/* --------------------------------------------------------------------------------------
+ * Row operators around the sparse ones (no counterpart in the reference): what a layer with several experts, node
+ * types or relations computes densely before and after it aggregates.  Value types are FG_F32, FG_F16, FG_BF16 and,
+ * for rows held in 8 bits with a scale each, FG_E4M3.  Sums, statistics and accumulators are fp32; each output is
+ * rounded once to its type unless stated.  No atomics on values: the same bits on every run.  Strides in values
+ * (0 = dense).  Lists are bounds-checked in the kernels: a wrong entry gives wrong rows, not a wrong address.
+ * -------------------------------------------------------------------------------------- */
+#define FG_F32 0
+#define FG_F16 1
+#define FG_BF16 2
+#define FG_E4M3 3
+
+/* Root-mean-square norm: h = x + residual (rounded to `type`; h = x and d_h unused where d_residual is NULL),
+ * y = h * r * weight with r = 1 / sqrt(mean(h^2) + eps).  d_weight may be NULL (ones), else of `type` or fp32.
+ * out_type FG_E4M3: d_scales[row] = max|y| / 448 (1 for a row of zeros) and the 8-bit values y / scale.
+ * 1 <= d <= 16384; h, y dense.  fg_quantize_rows: the 8-bit form of x itself. */
+int fg_rms_norm(const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, const void* d_weight, void* d_h, void* d_y,
+                float* d_scales, int64_t n, int32_t d, float eps, int32_t type, int32_t weight_type, int32_t out_type,
+                void* stream);
+int fg_quantize_rows(const void* d_x, int64_t ldx, void* d_y, float* d_scales, int64_t n, int32_t d, int32_t type, void* stream);
+/* Its gradient: d_dx for x and residual alike (d_dh, the gradient that arrives at h itself, may be NULL), d_dweight
+ * (NULL = not wanted) of weight_type.  d_partial: blocks * d floats, blocks = fg_rms_norm_backward_blocks(n, d). */
+int64_t fg_rms_norm_backward_blocks(int64_t n, int32_t d);
+int fg_rms_norm_backward(const void* d_h, int64_t ldh, const void* d_weight, const void* d_dy, int64_t lddy, const void* d_dh,
+                         int64_t lddh, void* d_dx, void* d_dweight, float* d_partial, int64_t blocks, int64_t n, int32_t d,
+                         float eps, int32_t type, int32_t weight_type, void* stream);
+
+/* Choice of the k largest of `experts` logits a row, in descending order, ties to the lowest index; -inf and NaN are
+ * never chosen, and where fewer than k are left the remaining choices are -1 with weight 0.  Weights: softmax over
+ * the row (without the closed ones) or sigmoid; normalize != 0: divided by the sum over the chosen.
+ * experts <= 1024, k <= 32.  The gradient is dense ([n, experts], of the logits' type). */
+#define FG_SCORE_SOFTMAX 0
+#define FG_SCORE_SIGMOID 1
+int fg_route(const void* d_logits, int64_t ld, float* d_weights, int32_t* d_experts, int64_t n, int32_t experts, int32_t k,
+             int32_t type, int32_t scoring, int32_t normalize, void* stream);
+int fg_route_backward(const void* d_logits, int64_t ld, const float* d_weights, const int32_t* d_experts, const float* d_dweights,
+                      void* d_dlogits, int64_t n, int32_t experts, int32_t k, int32_t type, int32_t scoring, int32_t normalize,
+                      void* stream);
+
+/* Lists by group of entries with keys in [0, num_groups) (a stable counting sort): slots d_offsets[g] ..
+ * d_offsets[g + 1] belong to group g, d_order[slot] = entry, d_position[entry] = slot.  Entries with another key are
+ * in no group: position -1, and the slots from d_offsets[num_groups] on hold -1.  num_groups <= 1024. */
+int64_t fg_group_rows_workspace(int64_t num_entries, int32_t num_groups);
+int fg_group_rows(const int32_t* d_keys, int64_t num_entries, int32_t num_groups, int32_t* d_offsets, int32_t* d_order,
+                  int32_t* d_position, void* d_workspace, int64_t workspace_bytes, void* stream);
+
+/* y[p, o] = sum over i of x[row(p), i] * w[g, o, i] for the rows p of each group g; rows in no group are 0.
+ * row(p) = p where d_order is NULL, else d_order[p] / choices.  w[g, o, i] is d_w[g w_group + o w_out + i w_in].
+ * FG_E4M3: times d_x_scales[row(p)] * d_w_scales[g * outer + o], output of out_type.  y dense, [num_rows, outer].
+ * fg_grouped_matmul_wgrad: d_dw[g, o, i] = sum over the rows p of g of dy[p, o] * x[row(p), i], dense. */
+int64_t fg_grouped_matmul_workspace(int64_t num_rows, int64_t x_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type);
+int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, const void* d_w, int64_t w_group, int64_t w_out,
+                      int64_t w_in, const float* d_w_scales, const int32_t* d_offsets, const int32_t* d_order, int32_t choices,
+                      int64_t x_rows, void* d_y, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type,
+                      int32_t out_type, void* d_workspace, int64_t workspace_bytes, void* stream);
+int64_t fg_grouped_matmul_wgrad_workspace(int64_t num_rows, int64_t x_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type);
+int fg_grouped_matmul_wgrad(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const int32_t* d_offsets,
+                            const int32_t* d_order, int32_t choices, int64_t x_rows, void* d_dw, int64_t num_rows, int32_t groups,
+                            int32_t inner, int32_t outer, int32_t type, void* d_workspace, int64_t workspace_bytes, void* stream);
+
+/* out[t] = sum over j of weights[t, j] * y[position[t * k + j]] (entries with position -1 are left out; d_weights may
+ * be NULL: ones), and its gradients: d_dy [n k, d] (rows from d_offsets[num_groups] on are 0) and d_dweights [n, k],
+ * either of them NULL where it is not wanted.  k <= 32. */
+int fg_combine_rows(const void* d_y, int64_t ldy, const float* d_weights, const int32_t* d_position, void* d_out, int64_t n,
+                    int32_t k, int32_t d, int32_t type, void* stream);
+int fg_combine_rows_backward(const void* d_y, int64_t ldy, const float* d_weights, const int32_t* d_position, const int32_t* d_offsets,
+                             int32_t num_groups, const void* d_dout, int64_t ldd, void* d_dy, float* d_dweights, int64_t n, int32_t k,
+                             int32_t d, int32_t type, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
