@@ -1,143 +1,598 @@
-// Products grouped by expert (node type, relation): y[p] = W[g(p)] x[row(p)] for the rows p of each group.
+// Products grouped by expert (node type, relation): y[p] = W[g(p)] x[row(p)] for the rows p of each group, the same with
+// the weight read the other way for the gradient of x, and dW[g] = sum over p of dy[p] x[row(p)]^T.
 //
-// Simple form: 64 x 64 output tiles, 256 threads with 4 x 4 outputs each, 16 values of the inner axis at a time
-// through shared memory, 32-bit sums of fused multiply-adds.  Any strides.
+// Bound: the tensor cores where groups have many rows, the weights' bytes where they have few.  The groups' sizes are on
+// the device only, so a launch covers every way they can fall: persistent blocks, one an SM, scan the offsets into
+// shared memory once (a microsecond) and walk a numbering of 128-row tiles that never span two groups.
+//
+// A block is six warps.  Warp 0 loads: 128-byte wide tiles of both operands through TMA into a ring of stages; rows that
+// are gathered (order[p] / choices) come by row-gather loads, four rows an instruction, so no gathered copy of x is ever
+// written.  Warp 1 issues tcgen05 products of 128 x BN x 32 bytes into one of two accumulators in tensor memory.  Warps
+// 2 to 5 take a finished accumulator to the output while the other one fills.
+//
+// Rows of a tile beyond its group's end belong to the next group (or to nothing): in y they are computed and not
+// stored.  In dW they would be terms of the sum, so they are overwritten with zeros in shared memory, in both
+// operands - a zero times their infinities or NaN would still be NaN - before the last products of the group.
+//
+// fp32: no tensor-core type holds it, so x and w are each cut into three bf16 parts of 8 bits (x = a + b + c exactly up to
+// 2^-24) and six products of parts are summed, smallest first: a c', b b', c a', a b', b a', a a'; the parts left out are
+// below 2^-24 of the result's terms.  Six bf16 products against one fp32 product on the scalar units.
+//
+// An operand that TMA cannot read (a row pitch or a start off the 16-byte grid, two strides above 1) is first copied into
+// a dense workspace by the same kernel that cuts fp32 into parts.
 #include <climits>
+#include <mutex>
 
 #include "rows.cuh"
+#include "tcgen05.cuh"
 
 namespace {
 
 using fg::from_f32;
+using fg::Pack;
+using fg::store_pack;
 using fg::to_f32;
 
-struct ProductArgs {
-    const void *x, *w;
-    const float *x_scales, *w_scales;
+constexpr int kTileRows = 128, kChunkBytes = 128, kThreads = 192, kMaxGroups = 1024, kSuperRows = 16;
+
+__device__ int g_stuck;  // set when a wait ran out; fg_grouped_matmul_status reads it
+
+struct MmaArgs {
     const int32_t *offsets, *order;
-    void* y;
-    int64_t ldx, w_group, w_out, w_in, x_rows, m;
-    int32_t choices, groups, inner, outer;
+    const float *x_scales, *w_scales;
+    void* y;              // output rows, dW, or partial sums of dW
+    int64_t m, x_rows;    // slots; rows of x
+    int32_t choices, groups, inner, outer;  // inner: the summed axis (y) or x's width (dW); outer: width of y
+    int32_t type, out_type, format;
+    int32_t first_pair;   // 5: one product; 0: six products of parts
+    bool b_mn, gather, shared_weight;
+    int32_t split;        // dW: rows of one partial sum (0: a group's rows in one)
+    int32_t units;        // dW: partial sums that there is room for
 };
 
-// First row and end of row tile `tile` (tiles of `size` rows never span two groups; group `groups` stands for the rows
-// in no group).  False past the last tile.
-__device__ bool locate_tile(const int32_t* offsets, int groups, int64_t m, int size, int64_t tile, int& group, int64_t& first, int64_t& end) {
-    int64_t begin = 0;
-    for (int g = 0; g <= groups; ++g) {
-        const int64_t stop = g < groups ? min((int64_t)max(offsets[g + 1], 0), m) : m;
-        const int64_t tiles = stop > begin ? (stop - begin + size - 1) / size : 0;
-        if (tile < tiles) {
-            group = g, first = begin + tile * size, end = min(first + size, stop);
-            return true;
+// Parts multiplied in each of the six products, smallest first.
+__device__ __forceinline__ int part_a(int pair) { return (0x001102 >> (4 * pair)) & 3; }
+__device__ __forceinline__ int part_b(int pair) { return (0x010120 >> (4 * pair)) & 3; }
+
+template <int BN>
+struct Shape {
+    static constexpr int kStageBytes = (kTileRows + BN) * kChunkBytes;
+    static constexpr int kStages = 196608 / kStageBytes;
+    static constexpr int kColumns = 2 * BN;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes;
+};
+
+struct Tables {
+    uint64_t full[8], empty[8], filled[2], drained[2], last;
+    uint32_t tmem;
+    int stop;
+    int warp_sums[8];
+    int start[kMaxGroups + 1];  // first slot of each group
+    int tiles[kMaxGroups + 1];  // row tiles (partial sums of dW) before each group
+};
+
+template <typename O>
+__device__ __forceinline__ void store_32(O* out, const float (&v)[32], int left, bool vector) {
+    constexpr int kVec = 16 / sizeof(O);
+    if (vector && left >= 32) {
+#pragma unroll
+        for (int i = 0; i < 32; i += kVec) {
+            Pack<O, kVec> p;
+#pragma unroll
+            for (int j = 0; j < kVec; ++j) p.v[j] = from_f32<O>(v[i + j]);
+            store_pack<O, kVec>(out + i, p);
         }
-        tile -= tiles;
-        begin = max(begin, stop);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            if (i < left) out[i] = from_f32<O>(v[i]);
     }
-    return false;
 }
 
-template <typename T, typename O>
-__global__ void __launch_bounds__(256) product_kernel(const ProductArgs a) {
-    __shared__ float sx[16][65], sw[16][65];
-    __shared__ int64_t source[64];
-    int g;
-    int64_t first, end;
-    if (!locate_tile(a.offsets, a.groups, a.m, 64, blockIdx.y, g, first, end)) return;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, col0 = blockIdx.x * 64;
-    if (threadIdx.x < 64) {
-        const int64_t p = first + threadIdx.x;
-        int64_t r = -1;
-        if (p < end && g < a.groups) {
-            r = p;
-            if (a.order) {
-                const int e = a.order[p];
-                r = e < 0 ? -1 : e / a.choices;
-            }
-            if (r >= a.x_rows) r = -1;
+// A wait of all lanes, with one answer for all of them.
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop, bool ignore_stop = false) {
+    return __all_sync(0xffffffffu, fg::barrier_wait(bar, parity, stop, ignore_stop));
+}
+
+template <int BN, bool EIGHT, bool WGRAD>
+__global__ void __launch_bounds__(kThreads, 1)
+    product_kernel(const MmaArgs a, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
+    using S = Shape<BN>;
+    constexpr int kChunk = EIGHT ? 128 : 64;  // values of the summed axis a stage holds
+    extern __shared__ uint8_t dynamic[];
+    __shared__ Tables t;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = (fg::smem_address(dynamic) + 1023u) & ~1023u;
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S::kStages; ++s) {
+            fg::barrier_init(fg::smem_address(&t.full[s]), 1);
+            fg::barrier_init(fg::smem_address(&t.empty[s]), 1);
         }
-        source[threadIdx.x] = r;
+        for (int s = 0; s < 2; ++s) {
+            fg::barrier_init(fg::smem_address(&t.filled[s]), 1);
+            fg::barrier_init(fg::smem_address(&t.drained[s]), 4);
+        }
+        fg::barrier_init(fg::smem_address(&t.last), 1);
+        fg::barrier_init_fence();
+        t.stop = 0;
+        fg::prefetch_map(&map_a);
+        fg::prefetch_map(&map_b);
+    }
+    if (warp == 1) fg::tmem_alloc(fg::smem_address(&t.tmem), S::kColumns);
+
+    // groups' first slots and tile counts, scanned: thread i takes groups [i * each, (i + 1) * each)
+    {
+        const int each = (a.groups + kThreads - 1) / kThreads, from = min((int)threadIdx.x * each, a.groups), to = min(from + each, a.groups);
+        const int64_t unit = WGRAD ? (a.split ? a.split : (int64_t)INT_MAX) : kTileRows;
+        int own = 0;
+        for (int g = from; g < to; ++g) {
+            const int64_t b = min((int64_t)max(a.offsets[g], 0), a.m), e = min((int64_t)max(a.offsets[g + 1], 0), a.m);
+            const int64_t n = max(e - b, (int64_t)0);
+            t.start[g] = (int)b;
+            own += (int)(WGRAD ? max((n + unit - 1) / unit, (int64_t)1) : (n + unit - 1) / unit);
+        }
+        int sum = own;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (lane == 31) t.warp_sums[warp] = sum;
+        __syncthreads();
+        int before = sum - own;
+        for (int w = 0; w < warp; ++w) before += t.warp_sums[w];
+        for (int g = from; g < to; ++g) {
+            const int64_t b = t.start[g], e = min((int64_t)max(a.offsets[g + 1], 0), a.m);
+            const int64_t n = max(e - b, (int64_t)0);
+            t.tiles[g] = before;
+            before += (int)(WGRAD ? max((n + unit - 1) / unit, (int64_t)1) : (n + unit - 1) / unit);
+        }
+        if (threadIdx.x == kThreads - 1) {
+            t.tiles[a.groups] = before;
+            t.start[a.groups] = (int)min((int64_t)max(a.offsets[a.groups], 0), a.m);
+        }
+    }
+    fg::tcgen05_before_sync();
+    __syncthreads();
+    fg::tcgen05_after_sync();
+
+    const int rows_tiles = WGRAD ? (a.outer + kTileRows - 1) / kTileRows : 1;
+    const int col_tiles = ((WGRAD ? a.inner : a.outer) + BN - 1) / BN;
+    const int per_unit = WGRAD ? rows_tiles * col_tiles : col_tiles;  // output tiles for each counted row tile or partial sum
+    const int64_t total = (int64_t)t.tiles[a.groups] * per_unit;
+    const uint32_t tmem = t.tmem;
+    volatile int* stop = &t.stop;
+
+    // What output tile `index` is: its group, first row and column, the slots [begin, end) it is about.
+    struct Tile {
+        int group, unit, row, col;
+        int begin, end, chunks;
+    };
+    int cursor = 0;
+    auto locate = [&](int64_t index) {
+        Tile w;
+        while (index >= (int64_t)t.tiles[cursor + 1] * per_unit) ++cursor;
+        const int64_t local = index - (int64_t)t.tiles[cursor] * per_unit;
+        const int count = t.tiles[cursor + 1] - t.tiles[cursor];
+        const int first = t.start[cursor], stop_at = max(first, (int)min((int64_t)max(a.offsets[cursor + 1], 0), a.m));
+        w.group = cursor;
+        if (WGRAD) {
+            const int part = (int)(local / per_unit), tile = (int)(local - (int64_t)part * per_unit);
+            w.unit = min(t.tiles[cursor] + part, a.units - 1);  // lists that overlap: wrong sums, no wrong address
+            w.row = tile % rows_tiles * kTileRows;
+            w.col = tile / rows_tiles * BN;
+            w.begin = a.split ? first + part * a.split : first;
+            w.end = a.split ? min(w.begin + a.split, stop_at) : stop_at;
+            w.chunks = max(w.end - w.begin + kChunk - 1, 0) / kChunk;
+        } else {
+            // up to 16 row tiles share a column tile's weights while they are in L2, then the next column tile
+            const int super = (int)(local / ((int64_t)kSuperRows * col_tiles)), left = min(kSuperRows, count - super * kSuperRows);
+            const int rest = (int)(local - (int64_t)super * kSuperRows * col_tiles);
+            w.unit = 0;
+            w.begin = first + (super * kSuperRows + rest % left) * kTileRows;
+            w.end = min(w.begin + kTileRows, stop_at);
+            w.row = 0;
+            w.col = rest / left * BN;
+            w.chunks = (a.inner + kChunk - 1) / kChunk;
+        }
+        return w;
+    };
+    auto source_row = [&](int slot, int end) {  // the row of x behind a slot, 0 where there is none
+        if (slot >= end) return 0;
+        const int e = a.order[slot], r = e >= 0 ? e / a.choices : 0;
+        return r < a.x_rows ? r : 0;
+    };
+
+    if (warp == 0) {
+        int64_t step = 0;  // stages filled so far
+        bool live = true;
+        for (int64_t i = blockIdx.x; live && i < total; i += gridDim.x) {
+            const Tile w = locate(i);
+            // 8 KB blocks of both operands; blocks beyond the last column are not loaded, their products not stored
+            const int a_blocks = WGRAD ? min(2, (a.outer - w.row + 63) / 64) : 2;
+            const int b_blocks = WGRAD || a.b_mn ? min(BN / 64, ((WGRAD ? a.inner : a.outer) - w.col + 63) / 64) : BN / 64;
+            int rows[4] = {0, 0, 0, 0};  // y, gathered: lane l loads rows 4 l .. 4 l + 3 of the tile
+            if (!WGRAD && a.gather)
+                for (int r = 0; r < 4; ++r) rows[r] = source_row(w.begin + 4 * lane + r, w.end);
+            for (int pair = a.first_pair; live && pair < 6; ++pair) {
+                const int pa = part_a(pair), pb = part_b(pair);
+                for (int c = 0; c < w.chunks; ++c, ++step) {
+                    const int s = (int)(step % S::kStages);
+                    const uint32_t bar = fg::smem_address(&t.full[s]), at = ring + s * S::kStageBytes, bt = at + kTileRows * kChunkBytes;
+                    if (step >= S::kStages && !warp_wait(fg::smem_address(&t.empty[s]), (step / S::kStages - 1) & 1, stop)) {
+                        live = false;
+                        break;
+                    }
+                    if (lane == 0) fg::barrier_expect(bar, (a_blocks + b_blocks) * 8192);
+                    __syncwarp();
+                    const int k = c * kChunk;
+                    if (WGRAD) {
+                        const int slot = w.begin + k;
+                        if (lane == 0)  // dy: 64 slots by 64 columns, twice
+                            for (int q = 0; q < a_blocks; ++q) fg::tma_load_2d(at + q * 8192, &map_a, w.row + q * 64, slot + pa * (int)a.m, bar);
+                        if (!a.gather) {
+                            if (lane == 0)
+                                for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d(bt + q * 8192, &map_b, w.col + q * 64, slot + pb * (int)a.x_rows, bar);
+                        } else if (lane < 16) {
+                            int r[4];
+                            for (int j = 0; j < 4; ++j) r[j] = source_row(slot + 4 * lane + j, w.end) + pb * (int)a.x_rows;
+                            for (int q = 0; q < b_blocks; ++q)
+                                fg::tma_gather_4(bt + q * 8192 + lane * 512, &map_b, w.col + q * 64, r[0], r[1], r[2], r[3], bar);
+                        }
+                    } else {
+                        const int shift = pa * (int)a.x_rows;
+                        if (a.gather)
+                            fg::tma_gather_4(at + lane * 512, &map_a, k, rows[0] + shift, rows[1] + shift, rows[2] + shift, rows[3] + shift, bar);
+                        else if (lane == 0)
+                            fg::tma_load_2d(at, &map_a, k, w.begin + shift, bar);
+                        if (lane == 0) {
+                            const int g = a.shared_weight ? pb : w.group + pb * a.groups;
+                            if (!a.b_mn) {
+                                fg::tma_load_3d(bt, &map_b, k, w.col, g, bar);
+                            } else {
+                                for (int q = 0; q < b_blocks; ++q) fg::tma_load_3d(bt + q * 8192, &map_b, w.col + q * 64, k, g, bar);
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+        if (__any_sync(0xffffffffu, *stop))  // no copy may be in flight when the block ends
+            for (int64_t q = max(step - S::kStages, (int64_t)0); q < step; ++q)
+                warp_wait(fg::smem_address(&t.full[q % S::kStages]), (q / S::kStages) & 1, stop, true);
+    } else if (warp == 1) {
+        int64_t step = 0;
+        int64_t turn = 0;
+        const uint32_t descriptor = fg::product_descriptor(a.format, WGRAD, WGRAD || a.b_mn, kTileRows, BN);
+        const bool b_mn = WGRAD || a.b_mn;
+        bool live = true;
+        for (int64_t i = blockIdx.x; live && i < total; i += gridDim.x) {
+            const Tile w = locate(i);
+            if (w.chunks == 0) continue;  // an empty group's dW: nothing to add up
+            const int buffer = (int)(turn & 1);
+            const uint32_t acc = tmem + buffer * BN;
+            if (turn >= 2 && !warp_wait(fg::smem_address(&t.drained[buffer]), (turn / 2 - 1) & 1, stop)) break;
+            fg::tcgen05_after_sync();
+            bool add = false;
+            for (int pair = a.first_pair; live && pair < 6; ++pair) {
+                for (int c = 0; c < w.chunks; ++c, ++step) {
+                    const int s = (int)(step % S::kStages);
+                    const uint32_t at = ring + s * S::kStageBytes, bt = at + kTileRows * kChunkBytes;
+                    if (!warp_wait(fg::smem_address(&t.full[s]), (step / S::kStages) & 1, stop)) {
+                        live = false;
+                        break;
+                    }
+                    fg::tcgen05_after_sync();
+                    if (WGRAD && c == w.chunks - 1 && (w.end - w.begin) % kChunk != 0) {
+                        const int keep = (w.end - w.begin) % kChunk;  // rows of 128 bytes, 64 a column block
+                        const uint32_t blocks = (kTileRows + BN) / 64;
+                        for (uint32_t q = 0; q < blocks; ++q)
+                            for (int z = keep * 8 + lane; z < 64 * 8; z += 32)
+                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + q * 8192 + z * 16), "r"(0) : "memory");
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                    if (lane == 0) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            const uint64_t da = WGRAD ? fg::operand_descriptor(at + k * 2048, 8192, 1024) : fg::operand_descriptor(at + k * 32, 16, 1024);
+                            const uint64_t db = b_mn ? fg::operand_descriptor(bt + k * 2048, 8192, 1024) : fg::operand_descriptor(bt + k * 32, 16, 1024);
+                            fg::product_step<EIGHT>(acc, da, db, descriptor, add || k > 0);
+                        }
+                        fg::product_commit(fg::smem_address(&t.empty[s]));
+                    }
+                    add = true;
+                    __syncwarp();
+                }
+            }
+            if (!live) break;
+            if (lane == 0) fg::product_commit(fg::smem_address(&t.filled[buffer]));
+            __syncwarp();
+            ++turn;
+        }
+        if (__any_sync(0xffffffffu, *stop)) {  // products in flight end before the accumulators are freed
+            if (lane == 0) fg::product_commit(fg::smem_address(&t.last));
+            __syncwarp();
+            warp_wait(fg::smem_address(&t.last), 0, stop, true);
+        }
+    } else {
+        const int quarter = warp & 3;  // the lanes of tensor memory this warp can read
+        const int width = WGRAD ? a.inner : a.outer;
+        const int size = a.out_type == FG_F32 ? 4 : 2;
+        const bool vector = (int64_t)width * size % 16 == 0 && ((uintptr_t)a.y & 15) == 0;
+        int64_t turn = 0;
+        for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
+            const Tile w = locate(i);
+            const int row = quarter * 32 + lane;
+            int64_t out_row;
+            bool in, zero = false;
+            float scale = 1.0f;
+            if (WGRAD) {
+                in = w.row + row < a.outer;
+                out_row = (int64_t)(a.split ? w.unit : w.group) * a.outer + w.row + row;
+                zero = w.chunks == 0;
+            } else {
+                const int slot = w.begin + row;
+                in = slot < w.end;
+                out_row = slot;
+                int r = slot;
+                if (in && a.gather) {
+                    const int e = a.order[slot];
+                    r = e / a.choices;
+                    zero = e < 0 || r >= a.x_rows;  // a list that names no row
+                }
+                if (EIGHT && in && !zero) scale = a.x_scales[r];
+            }
+            const int buffer = (int)(turn & 1);
+            if (w.chunks) {
+                if (!warp_wait(fg::smem_address(&t.filled[buffer]), (turn / 2) & 1, stop)) break;
+                fg::tcgen05_after_sync();
+            }
+            for (int c = 0; c < BN; c += 32) {
+                if (w.col + c >= width) break;
+                float v[32];
+                if (w.chunks) {
+                    uint32_t raw[32];
+                    fg::tmem_load_32(tmem + ((uint32_t)(quarter * 32) << 16) + buffer * BN + c, raw);
+                    fg::tmem_load_wait();
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
+                }
+                const int left = width - w.col - c;
+                if (EIGHT) {
+                    const float* ws = a.w_scales + (int64_t)w.group * a.outer + w.col + c;
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = __fmul_rn(__fmul_rn(v[j], scale), j < left ? ws[j] : 0.0f);
+                }
+                if (zero) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+                }
+                if (in) {
+                    const int64_t at = out_row * width + w.col + c;
+                    if (a.out_type == FG_F32) store_32<float>(static_cast<float*>(a.y) + at, v, left, vector);
+                    else if (a.out_type == FG_F16) store_32<__half>(static_cast<__half*>(a.y) + at, v, left, vector);
+                    else store_32<__nv_bfloat16>(static_cast<__nv_bfloat16*>(a.y) + at, v, left, vector);
+                }
+                __syncwarp();
+            }
+            if (w.chunks) {
+                fg::tcgen05_before_sync();
+                __syncwarp();
+                if (lane == 0) fg::barrier_arrive(fg::smem_address(&t.drained[buffer]));
+                ++turn;
+            }
+        }
+        if (!WGRAD) {  // rows in no group
+            const int64_t first = (int64_t)t.start[a.groups] * a.outer, values = a.m * a.outer;
+            for (int64_t i = first + (int64_t)blockIdx.x * 128 + (threadIdx.x - 64); i < values; i += (int64_t)gridDim.x * 128) {
+                if (a.out_type == FG_F32) static_cast<float*>(a.y)[i] = 0.0f;
+                else static_cast<uint16_t*>(a.y)[i] = 0;
+            }
+        }
     }
     __syncthreads();
-    float acc[4][4] = {};
-    const T* w = static_cast<const T*>(a.w) + (int64_t)(g < a.groups ? g : 0) * a.w_group;
-    for (int k0 = 0; k0 < (g < a.groups ? a.inner : 0); k0 += 16) {
-        for (int i = threadIdx.x; i < 1024; i += 256) {
-            const int kk = i % 16, r = i / 16;
-            const bool in = k0 + kk < a.inner;
-            sx[kk][r] = in && source[r] >= 0 ? to_f32<T>(static_cast<const T*>(a.x)[source[r] * a.ldx + k0 + kk]) : 0.0f;
-            sw[kk][r] = in && col0 + r < a.outer ? to_f32<T>(w[(int64_t)(col0 + r) * a.w_out + (int64_t)(k0 + kk) * a.w_in]) : 0.0f;
+    if (warp == 1) fg::tmem_free(tmem, S::kColumns);
+    if (threadIdx.x == 0 && t.stop) atomicExch(&g_stuck, 1);
+}
+
+// dW[g] = its partial sums added in order.
+template <typename T>
+__global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ partial, const int32_t* __restrict__ offsets, int groups, int64_t m,
+                                                   int split, int units, int64_t cells, T* __restrict__ dw) {
+    __shared__ int first, count;
+    const int g = blockIdx.y;  // `units`: partial sums that there are
+    if (threadIdx.x == 0) {
+        int before = 0, n = 0;
+        for (int q = 0; q <= g; ++q) {
+            const int64_t b = min((int64_t)max(offsets[q], 0), m), e = min((int64_t)max(offsets[q + 1], 0), m);
+            n = (int)max((max(e - b, (int64_t)0) + split - 1) / split, (int64_t)1);
+            if (q < g) before += n;
         }
-        __syncthreads();
-#pragma unroll
-        for (int kk = 0; kk < 16; ++kk)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __fmaf_rn(sx[kk][ty * 4 + i], sw[kk][tx + 16 * j], acc[i][j]);
-        __syncthreads();
+        first = min(before, units - 1);
+        count = min(n, units - first);
     }
-    for (int i = 0; i < 4; ++i) {
-        const int64_t p = first + ty * 4 + i;
-        if (p >= end) continue;
-        for (int j = 0; j < 4; ++j) {
-            const int c = col0 + tx + 16 * j;
-            if (c >= a.outer) continue;
-            float v = acc[i][j];
-            if (a.x_scales && source[ty * 4 + i] >= 0 && g < a.groups)
-                v = __fmul_rn(__fmul_rn(v, a.x_scales[source[ty * 4 + i]]), a.w_scales[(int64_t)g * a.outer + c]);
-            static_cast<O*>(a.y)[p * a.outer + c] = from_f32<O>(v);
+    __syncthreads();
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (int64_t)gridDim.x * 256) {
+        float s = partial[(int64_t)first * cells + i];
+        for (int q = 1; q < count; ++q) s = __fadd_rn(s, partial[(int64_t)(first + q) * cells + i]);
+        dw[(int64_t)g * cells + i] = from_f32<T>(s);
+    }
+}
+
+// dst[g][r][c], c < pitch, from src at g s0 + r s1 + c s2: the same type, or the three bf16 parts of an fp32 value in
+// three consecutive copies.  Eight values a thread.
+struct PackArgs {
+    const void* src;
+    void* dst;
+    int64_t s0, s1, s2, groups, rows;
+    int32_t cols, pitch;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
+    constexpr int kPer = sizeof(T) == 1 ? 16 : 8;
+    const int per_row = a.pitch / kPer;
+    const int64_t total = a.groups * a.rows * per_row, step = (int64_t)gridDim.x * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
+        const int64_t line = i / per_row, g = line / a.rows, r = line - g * a.rows;
+        const int c = (int)(i - line * per_row) * kPer;
+        const T* src = static_cast<const T*>(a.src) + g * a.s0 + r * a.s1 + (int64_t)c * a.s2;
+        T v[kPer];
+        if (sizeof(T) == 4 && a.s2 == 1 && c + kPer <= a.cols && ((uintptr_t)src & 15) == 0) {
+            *reinterpret_cast<Pack<T, kPer / 2>*>(v) = *reinterpret_cast<const Pack<T, kPer / 2>*>(src);
+            *reinterpret_cast<Pack<T, kPer / 2>*>(v + kPer / 2) = *reinterpret_cast<const Pack<T, kPer / 2>*>(src + kPer / 2);
+        } else {
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) v[j] = c + j < a.cols ? src[j * a.s2] : T(0.0f);
+        }
+        if constexpr (sizeof(T) == 4) {
+            Pack<__nv_bfloat16, 8> p[3];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float x = v[j];
+                // a finite value that would round to infinity is cut instead; of an infinity or NaN the other parts are 0
+                const bool finite = isfinite(x);
+                __nv_bfloat16 hi = __float2bfloat16_rn(x);
+                if (finite && isinf(__bfloat162float(hi))) hi = __float2bfloat16_rz(x);
+                const float rest = finite ? __fsub_rn(x, __bfloat162float(hi)) : 0.0f;
+                const __nv_bfloat16 mid = __float2bfloat16_rn(rest);
+                p[0].v[j] = hi;
+                p[1].v[j] = mid;
+                p[2].v[j] = __float2bfloat16_rn(__fsub_rn(rest, __bfloat162float(mid)));
+            }
+            const int64_t plane = a.groups * a.rows * a.pitch, at = line * a.pitch + c;
+            for (int q = 0; q < 3; ++q) store_pack<__nv_bfloat16, 8>(static_cast<__nv_bfloat16*>(a.dst) + q * plane + at, p[q]);
+        } else {
+            Pack<T, kPer> p;
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) p.v[j] = v[j];
+            store_pack<T, kPer>(static_cast<T*>(a.dst) + line * a.pitch + c, p);
         }
     }
 }
 
-struct WeightGradArgs {
-    const void *x, *dy;
-    const int32_t *offsets, *order;
-    void* dw;
-    int64_t ldx, lddy, x_rows, m;
-    int32_t choices, groups, inner, outer;
+// ---- host side ----
+
+typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encoder() {
+    static EncodeFn fn = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        void* p = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &p, 12000, cudaEnableDefault, &found) == cudaSuccess &&
+            found == cudaDriverEntryPointSuccess)
+            fn = reinterpret_cast<EncodeFn>(p);
+    });
+    return fn;
+}
+
+// A matrix, or one for each group, as the loads see it: rows of `cols` dense values.
+struct Matrix {
+    const void* data;
+    int64_t cols, rows, groups;    // groups 0: a plain matrix
+    int64_t pitch, group_stride;   // in values
+    int32_t type;                  // as stored (bf16 for the parts of fp32)
 };
 
-template <typename T>
-__global__ void __launch_bounds__(256) weight_grad_kernel(const WeightGradArgs a) {
-    __shared__ float sx[16][65], sy[16][65];
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16, in0 = blockIdx.x * 64, out0 = blockIdx.y * 64, g = blockIdx.z;
-    const int64_t begin = min((int64_t)max(a.offsets[g], 0), a.m), end = min((int64_t)max(a.offsets[g + 1], 0), a.m);
-    float acc[4][4] = {};
-    for (int64_t p0 = begin; p0 < end; p0 += 16) {
-        for (int i = threadIdx.x; i < 1024; i += 256) {
-            const int c = i % 64, r = i / 64;
-            const int64_t p = p0 + r;
-            int64_t row = p < end ? p : -1;
-            if (row >= 0 && a.order) {
-                const int e = a.order[p];
-                row = e < 0 ? -1 : e / a.choices;
-            }
-            if (row >= a.x_rows) row = -1;
-            sx[r][c] = row >= 0 && in0 + c < a.inner ? to_f32<T>(static_cast<const T*>(a.x)[row * a.ldx + in0 + c]) : 0.0f;
-            sy[r][c] = row >= 0 && out0 + c < a.outer ? to_f32<T>(static_cast<const T*>(a.dy)[p * a.lddy + out0 + c]) : 0.0f;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __fmaf_rn(sy[r][ty * 4 + i], sx[r][tx + 16 * j], acc[i][j]);
-        __syncthreads();
-    }
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int o = out0 + ty * 4 + i, c = in0 + tx + 16 * j;
-            if (o < a.outer && c < a.inner) static_cast<T*>(a.dw)[((int64_t)g * a.outer + o) * a.inner + c] = from_f32<T>(acc[i][j]);
-        }
+int make_map(CUtensorMap* map, const Matrix& m, int box_cols, int box_rows) {
+    EncodeFn encode = encoder();
+    if (!encode) return fg::fail(FG_ERR_CUDA, "the driver has no cuTensorMapEncodeTiled");
+    const int size = fg::type_size(m.type);
+    const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)(m.groups ? m.groups : 1)};
+    const cuuint64_t strides[2] = {(cuuint64_t)(m.pitch * size), (cuuint64_t)(m.group_stride * size)};
+    const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
+    const CUtensorMapDataType type = m.type == FG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : m.type == FG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const CUresult rc = encode(map, type, m.groups ? 3 : 2, const_cast<void*>(m.data), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (rc != CUDA_SUCCESS) return fg::fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)rc);
+    return FG_OK;
 }
 
-int check_product(int64_t m, int64_t x_rows, int32_t choices, int32_t groups, int32_t inner, int32_t outer) {
-    if (m < 0 || m > INT_MAX || x_rows < 0 || x_rows > INT_MAX || choices < 1 || groups < 1 || groups > 1024 || inner < 1 || outer < 1)
-        return fg::fail(FG_ERR_INVALID_ARGUMENT, "bad sizes rows=%lld of %lld choices=%d groups=%d inner=%d outer=%d (groups <= 1024)",
-                        (long long)m, (long long)x_rows, choices, groups, inner, outer);
+int64_t round_up(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+int64_t pitch_of(int64_t cols, int32_t type) { return round_up(cols, type == FG_E4M3 ? 16 : 8); }
+// Bytes of the dense copy (three bf16 copies of fp32), on a 256-byte grid.
+int64_t packed_bytes(int64_t lines, int64_t cols, int32_t type) {
+    return round_up(lines * pitch_of(cols, type) * (type == FG_F32 ? 6 : fg::type_size(type)), 256);
+}
+bool loadable(const void* p, int64_t pitch, int64_t group_stride, int32_t type) {
+    const int size = fg::type_size(type);
+    return type != FG_F32 && fg::aligned16(p) && pitch > 0 && pitch * size % 16 == 0 && group_stride * size % 16 == 0 &&
+           pitch * size < (1ll << 40) && group_stride * size < (1ll << 40);
+}
+
+// Copies [groups][rows][cols] at strides (s0, s1, s2) into `*work`, and moves `*work` on.
+int pack(const void* src, int64_t s0, int64_t s1, int64_t s2, int64_t groups, int64_t rows, int64_t cols, int32_t type, uint8_t** work,
+         cudaStream_t s) {
+    PackArgs p{src, *work, s0, s1, s2, groups, rows, (int32_t)cols, (int32_t)pitch_of(cols, type)};
+    const int64_t threads = groups * rows * (p.pitch / (type == FG_E4M3 ? 16 : 8)), most = (int64_t)fg::device_props().sm_count * 16;
+    const unsigned blocks = (unsigned)((threads + 255) / 256 < most ? (threads + 255) / 256 : most);
+    if (threads == 0) return FG_OK;
+    if (type == FG_F32) pack_kernel<float><<<blocks, 256, 0, s>>>(p);
+    else if (type == FG_F16) pack_kernel<__half><<<blocks, 256, 0, s>>>(p);
+    else if (type == FG_BF16) pack_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(p);
+    else pack_kernel<__nv_fp8_e4m3><<<blocks, 256, 0, s>>>(p);
+    FG_CUDA_TRY(cudaGetLastError());
+    fg::count_launches(1);
+    *work += packed_bytes(groups * rows, cols, type);
+    return FG_OK;
+}
+
+// Rows [rows, cols] with a row stride as a loadable matrix, copied if need be.
+int rows_matrix(Matrix* m, const void* p, int64_t ld, int64_t rows, int64_t cols, int32_t type, uint8_t** work, cudaStream_t s) {
+    if (loadable(p, ld, 0, type)) {
+        *m = Matrix{p, cols, rows, 0, ld, 0, type};
+        return FG_OK;
+    }
+    const int parts = type == FG_F32 ? 3 : 1;
+    *m = Matrix{*work, cols, rows * parts, 0, pitch_of(cols, type), 0, type == FG_F32 ? FG_BF16 : type};
+    return pack(p, 0, ld, 1, 1, rows, cols, type, work, s);
+}
+
+template <int BN, bool EIGHT, bool WGRAD>
+int launch_shape(const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b, int64_t most_tiles, cudaStream_t s) {
+    FG_CUDA_TRY(cudaFuncSetAttribute(product_kernel<BN, EIGHT, WGRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN>::kSmem));
+    const int64_t sms = fg::device_props().sm_count;
+    product_kernel<BN, EIGHT, WGRAD><<<(unsigned)(most_tiles < sms ? most_tiles : sms), kThreads, Shape<BN>::kSmem, s>>>(a, map_a, map_b);
+    FG_CUDA_TRY(cudaGetLastError());
+    fg::count_launches(1);
+    return FG_OK;
+}
+template <bool EIGHT, bool WGRAD>
+int launch(int bn, const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b, int64_t most_tiles, cudaStream_t s) {
+    return bn == 256 ? launch_shape<256, EIGHT, WGRAD>(a, map_a, map_b, most_tiles, s)
+           : bn == 128 ? launch_shape<128, EIGHT, WGRAD>(a, map_a, map_b, most_tiles, s)
+                       : launch_shape<64, EIGHT, WGRAD>(a, map_a, map_b, most_tiles, s);
+}
+
+// Columns of an output tile: the widest whose tiles still give each SM one.
+int tile_width(int64_t units, int width) {
+    for (int bn = 256; bn > 64; bn /= 2)
+        if (width > bn / 2 && units * ((width + bn - 1) / bn) >= fg::device_props().sm_count) return bn;
+    return 64;
+}
+
+// Rows of one partial sum of dW: 0 (none) where the tiles of all groups already give each SM two, else such that they do.
+int64_t split_rows(int64_t m, int32_t groups, int64_t tiles) {
+    const int64_t want = 2ll * fg::device_props().sm_count;
+    if (groups * tiles >= want || m <= 1024) return 0;
+    const int64_t parts = (want + tiles - 1) / tiles;
+    int64_t rows = round_up((m + parts - 1) / parts, 64);
+    return rows < 512 ? 512 : rows;
+}
+int64_t wgrad_tiles(int32_t inner, int32_t outer) {
+    return (int64_t)((outer + kTileRows - 1) / kTileRows) * ((inner + 127) / 128);
+}
+
+int check_product(int64_t m, int64_t x_rows, int32_t choices, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
+    if (m < 0 || m > INT_MAX - 1024 || x_rows < 0 || x_rows > INT_MAX || choices < 1 || groups < 1 || groups > kMaxGroups || inner < 1 || outer < 1 ||
+        (type == FG_F32 && (m > INT_MAX / 4 || x_rows > INT_MAX / 4)))
+        return fg::fail(FG_ERR_INVALID_ARGUMENT, "bad sizes rows=%lld of %lld choices=%d groups=%d inner=%d outer=%d (groups <= %d)",
+                        (long long)m, (long long)x_rows, choices, groups, inner, outer, kMaxGroups);
     return FG_OK;
 }
 
@@ -145,61 +600,125 @@ int check_product(int64_t m, int64_t x_rows, int32_t choices, int32_t groups, in
 
 extern "C" {
 
+int fg_grouped_matmul_status(void* stream) {
+    int v = 0;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    FG_CUDA_TRY(cudaMemcpyFromSymbolAsync(&v, g_stuck, sizeof(v), 0, cudaMemcpyDeviceToHost, s));
+    FG_CUDA_TRY(cudaStreamSynchronize(s));
+    return v ? fg::fail(FG_ERR_CUDA, "a grouped product gave up waiting for its own copies") : FG_OK;
+}
+
 int64_t fg_grouped_matmul_workspace(int64_t num_rows, int64_t x_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
-    return 0;
+    if (num_rows <= 0 || x_rows < 0 || groups < 1 || inner < 1 || outer < 1) return 0;
+    const int64_t k_major = packed_bytes((int64_t)groups * outer, inner, type), mn_major = packed_bytes((int64_t)groups * inner, outer, type);
+    return packed_bytes(x_rows, inner, type) + (k_major > mn_major ? k_major : mn_major);
 }
 
 int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, const void* d_w, int64_t w_group, int64_t w_out,
                       int64_t w_in, const float* d_w_scales, const int32_t* d_offsets, const int32_t* d_order, int32_t choices,
                       int64_t x_rows, void* d_y, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type,
                       int32_t out_type, void* d_workspace, int64_t workspace_bytes, void* stream) {
-    if (int rc = check_product(num_rows, x_rows, choices, groups, inner, outer)) return rc;
+    if (int rc = check_product(num_rows, x_rows, choices, groups, inner, outer, type)) return rc;
     if (!fg::float_type(type) && type != FG_E4M3) return fg::fail(FG_ERR_INVALID_ARGUMENT, "unknown value type %d", type);
     if (type == FG_E4M3 ? !fg::float_type(out_type) : out_type != type)
         return fg::fail(FG_ERR_INVALID_ARGUMENT, "the output is of the inputs' type, or of a wider one for e4m3");
     if (ldx == 0) ldx = inner;
     if (ldx < inner) return fg::fail(FG_ERR_INVALID_ARGUMENT, "row strides must be 0 or >= inner=%d", inner);
+    if (w_group < 0 || w_out < 0 || w_in < 0) return fg::fail(FG_ERR_INVALID_ARGUMENT, "the weight's strides must be >= 0");
     if (num_rows == 0) return FG_OK;
     if (!d_x || !d_w || !d_offsets || !d_y || (type == FG_E4M3 && (!d_x_scales || !d_w_scales)))
         return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
-    const ProductArgs a{d_x, d_w, d_x_scales, d_w_scales, d_offsets, d_order, d_y, ldx, w_group, w_out, w_in, x_rows, num_rows, choices, groups, inner, outer};
-    const int64_t tiles = num_rows / 64 + groups + 1;
-    if (tiles > 65535) return fg::fail(FG_ERR_INVALID_ARGUMENT, "grid too large");
-    const dim3 grid((outer + 63) / 64, (unsigned)tiles);
+    if (!d_order && x_rows != num_rows) return fg::fail(FG_ERR_INVALID_ARGUMENT, "without an order x has a row for each slot");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (type == FG_F32) product_kernel<float, float><<<grid, 256, 0, s>>>(a);
-    else if (type == FG_F16) product_kernel<__half, __half><<<grid, 256, 0, s>>>(a);
-    else if (type == FG_BF16) product_kernel<__nv_bfloat16, __nv_bfloat16><<<grid, 256, 0, s>>>(a);
-    else if (out_type == FG_F32) product_kernel<__nv_fp8_e4m3, float><<<grid, 256, 0, s>>>(a);
-    else if (out_type == FG_F16) product_kernel<__nv_fp8_e4m3, __half><<<grid, 256, 0, s>>>(a);
-    else product_kernel<__nv_fp8_e4m3, __nv_bfloat16><<<grid, 256, 0, s>>>(a);
-    FG_CUDA_TRY(cudaGetLastError());
-    fg::count_launches(1);
-    return FG_OK;
+
+    // The weight is read as it is stored where its inner or its outer axis is dense (8-bit products want the inner one).
+    const bool shared = w_group == 0;
+    const int64_t count = shared ? 1 : groups;
+    const bool k_dense = w_in == 1 || inner == 1, n_dense = type != FG_E4M3 && (w_out == 1 || outer == 1);
+    const bool k_loads = k_dense && loadable(d_w, w_out, w_group, type), n_loads = n_dense && loadable(d_w, w_in, w_group, type);
+    const bool b_mn = k_loads ? false : n_loads ? true : !k_dense && n_dense;
+    const bool pack_w = !k_loads && !n_loads, pack_x = !loadable(d_x, ldx, 0, type);
+    const int64_t need = (pack_x ? packed_bytes(x_rows, inner, type) : 0) +
+                         (pack_w ? packed_bytes(count * (b_mn ? inner : outer), b_mn ? outer : inner, type) : 0);
+    if (workspace_bytes < need || (need && !d_workspace)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_grouped_matmul_workspace()");
+    uint8_t* work = static_cast<uint8_t*>(d_workspace);
+    Matrix x, w;
+    if (int rc = rows_matrix(&x, d_x, ldx, x_rows, inner, type, &work, s)) return rc;
+    const int64_t rows = b_mn ? inner : outer, cols = b_mn ? outer : inner, parts = type == FG_F32 ? 3 : 1;
+    if (!pack_w) {
+        w = Matrix{d_w, cols, rows, count, b_mn ? w_in : w_out, shared ? rows * (b_mn ? w_in : w_out) : w_group, type};
+    } else {
+        const int64_t pitch = pitch_of(cols, type);
+        w = Matrix{work, cols, rows, count * parts, pitch, rows * pitch, type == FG_F32 ? FG_BF16 : type};
+        if (int rc = pack(d_w, w_group, b_mn ? w_in : w_out, b_mn ? w_out : w_in, count, rows, cols, type, &work, s)) return rc;
+    }
+    const int64_t units = num_rows / kTileRows + (groups < num_rows ? groups : num_rows);
+    const int bn = tile_width(units, outer), chunk = type == FG_E4M3 ? 128 : 64;
+    CUtensorMap map_x, map_w;
+    if (int rc = make_map(&map_x, x, chunk, d_order ? 1 : kTileRows)) return rc;
+    if (int rc = make_map(&map_w, w, chunk, b_mn ? 64 : bn)) return rc;
+    MmaArgs a{};
+    a.offsets = d_offsets, a.order = d_order, a.x_scales = d_x_scales, a.w_scales = d_w_scales, a.y = d_y;
+    a.m = num_rows, a.x_rows = x_rows, a.choices = choices, a.groups = groups, a.inner = inner, a.outer = outer;
+    a.type = type, a.out_type = out_type, a.format = w.type == FG_BF16 ? 1 : 0, a.first_pair = type == FG_F32 ? 0 : 5;
+    a.b_mn = b_mn, a.gather = d_order != nullptr, a.shared_weight = shared;
+    const int64_t tiles = units * ((outer + bn - 1) / bn);
+    return type == FG_E4M3 ? launch<true, false>(bn, a, map_x, map_w, tiles, s) : launch<false, false>(bn, a, map_x, map_w, tiles, s);
 }
 
 int64_t fg_grouped_matmul_wgrad_workspace(int64_t num_rows, int64_t x_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
-    return 0;
+    if (num_rows <= 0 || x_rows < 0 || groups < 1 || inner < 1 || outer < 1) return 0;
+    const int64_t split = split_rows(num_rows, groups, wgrad_tiles(inner, outer));
+    const int64_t partial = split ? round_up((num_rows / split + groups) * (int64_t)inner * outer * 4, 256) : 0;
+    return packed_bytes(x_rows, inner, type) + packed_bytes(num_rows, outer, type) + partial;
 }
 
 int fg_grouped_matmul_wgrad(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const int32_t* d_offsets,
                             const int32_t* d_order, int32_t choices, int64_t x_rows, void* d_dw, int64_t num_rows, int32_t groups,
                             int32_t inner, int32_t outer, int32_t type, void* d_workspace, int64_t workspace_bytes, void* stream) {
-    if (int rc = check_product(num_rows, x_rows, choices, groups, inner, outer)) return rc;
+    if (int rc = check_product(num_rows, x_rows, choices, groups, inner, outer, type)) return rc;
     if (!fg::float_type(type)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "unknown value type %d", type);
     if (ldx == 0) ldx = inner;
     if (lddy == 0) lddy = outer;
     if (ldx < inner || lddy < outer) return fg::fail(FG_ERR_INVALID_ARGUMENT, "row strides must be 0 or >= the width");
     if (!d_dw || !d_offsets || (num_rows && (!d_x || !d_dy))) return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
-    const WeightGradArgs a{d_x, d_dy, d_offsets, d_order, d_dw, ldx, lddy, x_rows, num_rows, choices, groups, inner, outer};
-    const dim3 grid((inner + 63) / 64, (outer + 63) / 64, groups);
-    if (grid.y > 65535) return fg::fail(FG_ERR_INVALID_ARGUMENT, "grid too large");
+    if (!d_order && x_rows != num_rows) return fg::fail(FG_ERR_INVALID_ARGUMENT, "without an order x has a row for each slot");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (type == FG_F32) weight_grad_kernel<float><<<grid, 256, 0, s>>>(a);
-    else if (type == FG_F16) weight_grad_kernel<__half><<<grid, 256, 0, s>>>(a);
-    else weight_grad_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
-    FG_CUDA_TRY(cudaGetLastError());
-    fg::count_launches(1);
+    const int64_t cells = (int64_t)inner * outer;
+    if (num_rows == 0) {
+        FG_CUDA_TRY(cudaMemsetAsync(d_dw, 0, (size_t)(groups * cells * fg::type_size(type)), s));
+        return FG_OK;
+    }
+    const int64_t split = split_rows(num_rows, groups, wgrad_tiles(inner, outer));
+    const int64_t partial = split ? round_up((num_rows / split + groups) * cells * 4, 256) : 0;
+    const bool pack_x = !loadable(d_x, ldx, 0, type), pack_dy = !loadable(d_dy, lddy, 0, type);
+    const int64_t need = partial + (pack_x ? packed_bytes(x_rows, inner, type) : 0) + (pack_dy ? packed_bytes(num_rows, outer, type) : 0);
+    if (workspace_bytes < need || (need && !d_workspace)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_grouped_matmul_wgrad_workspace()");
+    uint8_t* work = static_cast<uint8_t*>(d_workspace);
+    float* sums = reinterpret_cast<float*>(work);
+    work += partial;
+    Matrix x, dy;
+    if (int rc = rows_matrix(&x, d_x, ldx, x_rows, inner, type, &work, s)) return rc;
+    if (int rc = rows_matrix(&dy, d_dy, lddy, num_rows, outer, type, &work, s)) return rc;
+    CUtensorMap map_x, map_dy;
+    if (int rc = make_map(&map_dy, dy, 64, 64)) return rc;
+    if (int rc = make_map(&map_x, x, 64, d_order ? 1 : 64)) return rc;
+    const int64_t units = split ? num_rows / split + groups : groups, rows_tiles = (outer + kTileRows - 1) / kTileRows;
+    const int bn = tile_width(units * rows_tiles, inner);
+    MmaArgs a{};
+    a.offsets = d_offsets, a.order = d_order, a.y = split ? static_cast<void*>(sums) : d_dw;
+    a.m = num_rows, a.x_rows = x_rows, a.choices = choices, a.groups = groups, a.inner = inner, a.outer = outer;
+    a.type = type, a.out_type = split ? FG_F32 : type, a.format = dy.type == FG_BF16 ? 1 : 0, a.first_pair = type == FG_F32 ? 0 : 5;
+    a.gather = d_order != nullptr, a.split = (int32_t)split, a.units = (int32_t)units;
+    if (int rc = launch<false, true>(bn, a, map_dy, map_x, units * rows_tiles * ((inner + bn - 1) / bn), s)) return rc;
+    if (split) {
+        const dim3 grid((unsigned)((cells + 1023) / 1024 < 4096 ? (cells + 1023) / 1024 : 4096), (unsigned)groups);
+        if (type == FG_F32) join_kernel<float><<<grid, 256, 0, s>>>(sums, d_offsets, groups, num_rows, (int)split, a.units, cells, static_cast<float*>(d_dw));
+        else if (type == FG_F16) join_kernel<__half><<<grid, 256, 0, s>>>(sums, d_offsets, groups, num_rows, (int)split, a.units, cells, static_cast<__half*>(d_dw));
+        else join_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(sums, d_offsets, groups, num_rows, (int)split, a.units, cells, static_cast<__nv_bfloat16*>(d_dw));
+        FG_CUDA_TRY(cudaGetLastError());
+        fg::count_launches(1);
+    }
     return FG_OK;
 }
 

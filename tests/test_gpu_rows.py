@@ -610,3 +610,9 @@ def test_refusals_that_need_a_device():
         rms_norm(x, torch.ones(8))
     with pytest.raises(ValueError, match="lives on cpu"):
         grouped_matmul(x, torch.zeros(3, 5, 8), make_groups(4, 1, 3, 1))
+
+
+def test_no_wait_ever_ran_out():
+    """Runs last: the products' bounded waits (for their own copies) all ended in time in this process."""
+    from featgraph_b200 import _native
+    assert _native.lib().fg_grouped_matmul_status(torch.cuda.current_stream().cuda_stream) == 0
