@@ -57,10 +57,10 @@ SIGNATURES = {
     "fg_group_rows_workspace": (_i64, [_i64, _i32]),
     "fg_group_rows": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
     "fg_grouped_matmul_status": (ctypes.c_int, [_vp]),
-    "fg_grouped_matmul_workspace": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    "fg_grouped_matmul_workspace": (_i64, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i32, _i32, _i32, _i32]),
     "fg_grouped_matmul": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i64, _vp, _i64, _i32, _i32, _i32,
                                          _i32, _i32, _vp, _i64, _vp]),
-    "fg_grouped_matmul_wgrad_workspace": (_i64, [_i64, _i64, _i32, _i32, _i32, _i32]),
+    "fg_grouped_matmul_wgrad_workspace": (_i64, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32]),
     "fg_grouped_matmul_wgrad": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64,
                                                _vp]),
     "fg_combine_rows": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp]),

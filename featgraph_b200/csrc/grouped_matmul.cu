@@ -5,9 +5,7 @@
 // the device only, so a launch covers every way they can fall: persistent blocks, one an SM, scan the offsets into
 // shared memory once (a microsecond) and walk a numbering of 128-row tiles that never span two groups.
 //
-// A block is six warps.  Warp 0 loads: 128-byte wide tiles of both operands through TMA into a ring of stages; rows that
-// are gathered (order[p] / choices) come by row-gather loads, four rows an instruction, so no gathered copy of x is ever
-// written.  Warp 1 issues tcgen05 products of 128 x BN x 32 bytes into one of two accumulators in tensor memory.  Warps
+// A block is six warps.  Warp 0 loads: 128-byte wide tiles of both operands through TMA into a ring of stages.  Warp 1 issues tcgen05 products of 128 x BN x 32 bytes into one of two accumulators in tensor memory.  Warps
 // 2 to 5 take a finished accumulator to the output while the other one fills.
 //
 // Rows of a tile beyond its group's end belong to the next group (or to nothing): in y they are computed and not
@@ -18,8 +16,11 @@
 // 2^-24) and six products of parts are summed, smallest first: a c', b b', c a', a b', b a', a a'; the parts left out are
 // below 2^-24 of the result's terms.  Six bf16 products against one fp32 product on the scalar units.
 //
-// An operand that TMA cannot read (a row pitch or a start off the 16-byte grid, two strides above 1) is first copied into
-// a dense workspace by the same kernel that cuts fp32 into parts.
+// Rows that are gathered (slot p reads row order[p] / choices) are first copied into slot order: every column tile reads
+// them again, and row-gather TMA loads (tile::gather4, four rows an instruction) move a 128-row tile at a fraction of the
+// tile loads' rate.  Measured at 65536 x 2048 x 4096 in bf16: 2767 us with gather loads in the ring, 922 us for rows in
+// slot order, the copy about 70 us; dW 8512 against 1241 us.  The same kernel copies an operand that TMA cannot read (a
+// row pitch or a start off the 16-byte grid, two strides above 1) and cuts fp32 into parts.
 #include <climits>
 #include <mutex>
 
@@ -45,7 +46,7 @@ struct MmaArgs {
     int32_t choices, groups, inner, outer;  // inner: the summed axis (y) or x's width (dW); outer: width of y
     int32_t type, out_type, format;
     int32_t first_pair;   // 5: one product; 0: six products of parts
-    bool b_mn, gather, shared_weight;
+    bool b_mn, shared_weight;
     int32_t split;        // dW: rows of one partial sum (0: a group's rows in one)
     int32_t units;        // dW: partial sums that there is room for
 };
@@ -198,11 +199,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         return w;
     };
-    auto source_row = [&](int slot, int end) {  // the row of x behind a slot, 0 where there is none
-        if (slot >= end) return 0;
-        const int e = a.order[slot], r = e >= 0 ? e / a.choices : 0;
-        return r < a.x_rows ? r : 0;
-    };
 
     if (warp == 0) {
         int64_t step = 0;  // stages filled so far
@@ -212,9 +208,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             // 8 KB blocks of both operands; blocks beyond the last column are not loaded, their products not stored
             const int a_blocks = WGRAD ? min(2, (a.outer - w.row + 63) / 64) : 2;
             const int b_blocks = WGRAD || a.b_mn ? min(BN / 64, ((WGRAD ? a.inner : a.outer) - w.col + 63) / 64) : BN / 64;
-            int rows[4] = {0, 0, 0, 0};  // y, gathered: lane l loads rows 4 l .. 4 l + 3 of the tile
-            if (!WGRAD && a.gather)
-                for (int r = 0; r < 4; ++r) rows[r] = source_row(w.begin + 4 * lane + r, w.end);
             for (int pair = a.first_pair; live && pair < 6; ++pair) {
                 const int pa = part_a(pair), pb = part_b(pair);
                 for (int c = 0; c < w.chunks; ++c, ++step) {
@@ -224,30 +217,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                         live = false;
                         break;
                     }
-                    if (lane == 0) fg::barrier_expect(bar, (a_blocks + b_blocks) * 8192);
-                    __syncwarp();
-                    const int k = c * kChunk;
-                    if (WGRAD) {
-                        const int slot = w.begin + k;
-                        if (lane == 0)  // dy: 64 slots by 64 columns, twice
+                    if (lane == 0) {
+                        fg::barrier_expect(bar, (a_blocks + b_blocks) * 8192);
+                        const int k = c * kChunk;
+                        if (WGRAD) {  // 64 slots by 64 columns a block
+                            const int slot = w.begin + k;
                             for (int q = 0; q < a_blocks; ++q) fg::tma_load_2d(at + q * 8192, &map_a, w.row + q * 64, slot + pa * (int)a.m, bar);
-                        if (!a.gather) {
-                            if (lane == 0)
-                                for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d(bt + q * 8192, &map_b, w.col + q * 64, slot + pb * (int)a.x_rows, bar);
-                        } else if (lane < 16) {
-                            int r[4];
-                            for (int j = 0; j < 4; ++j) r[j] = source_row(slot + 4 * lane + j, w.end) + pb * (int)a.x_rows;
-                            for (int q = 0; q < b_blocks; ++q)
-                                fg::tma_gather_4(bt + q * 8192 + lane * 512, &map_b, w.col + q * 64, r[0], r[1], r[2], r[3], bar);
-                        }
-                    } else {
-                        const int shift = pa * (int)a.x_rows;
-                        if (a.gather)
-                            fg::tma_gather_4(at + lane * 512, &map_a, k, rows[0] + shift, rows[1] + shift, rows[2] + shift, rows[3] + shift, bar);
-                        else if (lane == 0)
-                            fg::tma_load_2d(at, &map_a, k, w.begin + shift, bar);
-                        if (lane == 0) {
+                            for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d(bt + q * 8192, &map_b, w.col + q * 64, slot + pb * (int)a.m, bar);
+                        } else {
                             const int g = a.shared_weight ? pb : w.group + pb * a.groups;
+                            fg::tma_load_2d(at, &map_a, k, w.begin + pa * (int)a.m, bar);
                             if (!a.b_mn) {
                                 fg::tma_load_3d(bt, &map_b, k, w.col, g, bar);
                             } else {
@@ -337,13 +316,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int slot = w.begin + row;
                 in = slot < w.end;
                 out_row = slot;
-                int r = slot;
-                if (in && a.gather) {
-                    const int e = a.order[slot];
-                    r = e / a.choices;
-                    zero = e < 0 || r >= a.x_rows;  // a list that names no row
+                if (EIGHT && in) {
+                    const int e = a.order ? a.order[slot] : 0, r = a.order ? e / a.choices : slot;
+                    scale = e >= 0 && r < a.x_rows ? a.x_scales[r] : 0.0f;
                 }
-                if (EIGHT && in && !zero) scale = a.x_scales[r];
             }
             const int buffer = (int)(turn & 1);
             if (w.chunks) {
@@ -423,52 +399,68 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
 }
 
 // dst[g][r][c], c < pitch, from src at g s0 + r s1 + c s2: the same type, or the three bf16 parts of an fp32 value in
-// three consecutive copies.  Eight values a thread.
+// three consecutive copies.  With an order (one group), row r comes from row order[r] / choices; a slot that names no row
+// gets zeros.  16 bytes of output (of each part) a thread and step; 2^shift threads share a row.  Bound: device memory.
 struct PackArgs {
     const void* src;
     void* dst;
-    int64_t s0, s1, s2, groups, rows;
-    int32_t cols, pitch;
+    const int32_t* order;
+    int64_t s0, s1, s2, groups, rows, source_rows;
+    int32_t cols, pitch, choices, shift;
+    bool vector;  // 128-bit reads: dense columns, every row on a 16-byte boundary
 };
 template <typename T>
 __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
     constexpr int kPer = sizeof(T) == 1 ? 16 : 8;
-    const int per_row = a.pitch / kPer;
-    const int64_t total = a.groups * a.rows * per_row, step = (int64_t)gridDim.x * 256;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-        const int64_t line = i / per_row, g = line / a.rows, r = line - g * a.rows;
-        const int c = (int)(i - line * per_row) * kPer;
-        const T* src = static_cast<const T*>(a.src) + g * a.s0 + r * a.s1 + (int64_t)c * a.s2;
-        T v[kPer];
-        if (sizeof(T) == 4 && a.s2 == 1 && c + kPer <= a.cols && ((uintptr_t)src & 15) == 0) {
-            *reinterpret_cast<Pack<T, kPer / 2>*>(v) = *reinterpret_cast<const Pack<T, kPer / 2>*>(src);
-            *reinterpret_cast<Pack<T, kPer / 2>*>(v + kPer / 2) = *reinterpret_cast<const Pack<T, kPer / 2>*>(src + kPer / 2);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) v[j] = c + j < a.cols ? src[j * a.s2] : T(0.0f);
+    const int per_row = a.pitch / kPer, threads = 1 << a.shift, mine = threadIdx.x & (threads - 1);
+    const int64_t lines = a.groups * a.rows, plane = lines * a.pitch;
+    for (int64_t line = ((int64_t)blockIdx.x * 256 + threadIdx.x) >> a.shift; line < lines; line += ((int64_t)gridDim.x * 256) >> a.shift) {
+        int64_t g = 0, r = line;
+        if (a.groups > 1) g = line / a.rows, r = line - g * a.rows;
+        bool in = true;
+        if (a.order) {
+            const int e = a.order[line];
+            r = e / a.choices;
+            in = e >= 0 && r < a.source_rows;
         }
-        if constexpr (sizeof(T) == 4) {
-            Pack<__nv_bfloat16, 8> p[3];
+        const T* row = static_cast<const T*>(a.src) + (in ? g * a.s0 + r * a.s1 : 0);
+        for (int q = mine; q < per_row; q += threads) {
+            const int c = q * kPer;
+            alignas(16) T v[kPer];
+            if (!in) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float x = v[j];
-                // a finite value that would round to infinity is cut instead; of an infinity or NaN the other parts are 0
-                const bool finite = isfinite(x);
-                __nv_bfloat16 hi = __float2bfloat16_rn(x);
-                if (finite && isinf(__bfloat162float(hi))) hi = __float2bfloat16_rz(x);
-                const float rest = finite ? __fsub_rn(x, __bfloat162float(hi)) : 0.0f;
-                const __nv_bfloat16 mid = __float2bfloat16_rn(rest);
-                p[0].v[j] = hi;
-                p[1].v[j] = mid;
-                p[2].v[j] = __float2bfloat16_rn(__fsub_rn(rest, __bfloat162float(mid)));
+                for (int j = 0; j < kPer; ++j) v[j] = T(0.0f);
+            } else if (a.vector && c + kPer <= a.cols) {
+                constexpr int kHalf = 16 / sizeof(T);
+#pragma unroll
+                for (int j = 0; j < kPer; j += kHalf) *reinterpret_cast<Pack<T, kHalf>*>(v + j) = fg::load_pack<T, kHalf>(row + c + j);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) v[j] = c + j < a.cols ? row[(int64_t)(c + j) * a.s2] : T(0.0f);
             }
-            const int64_t plane = a.groups * a.rows * a.pitch, at = line * a.pitch + c;
-            for (int q = 0; q < 3; ++q) store_pack<__nv_bfloat16, 8>(static_cast<__nv_bfloat16*>(a.dst) + q * plane + at, p[q]);
-        } else {
-            Pack<T, kPer> p;
+            const int64_t at = line * a.pitch + c;
+            if constexpr (sizeof(T) == 4) {
+                Pack<__nv_bfloat16, 8> p[3];
 #pragma unroll
-            for (int j = 0; j < kPer; ++j) p.v[j] = v[j];
-            store_pack<T, kPer>(static_cast<T*>(a.dst) + line * a.pitch + c, p);
+                for (int j = 0; j < 8; ++j) {
+                    const float x = v[j];
+                    // a finite value that would round to infinity is cut instead; of an infinity or NaN the other parts are 0
+                    const bool finite = isfinite(x);
+                    __nv_bfloat16 hi = __float2bfloat16_rn(x);
+                    if (finite && isinf(__bfloat162float(hi))) hi = __float2bfloat16_rz(x);
+                    const float rest = finite ? __fsub_rn(x, __bfloat162float(hi)) : 0.0f;
+                    const __nv_bfloat16 mid = __float2bfloat16_rn(rest);
+                    p[0].v[j] = hi;
+                    p[1].v[j] = mid;
+                    p[2].v[j] = __float2bfloat16_rn(__fsub_rn(rest, __bfloat162float(mid)));
+                }
+                for (int k = 0; k < 3; ++k) store_pack<__nv_bfloat16, 8>(static_cast<__nv_bfloat16*>(a.dst) + k * plane + at, p[k]);
+            } else {
+                Pack<T, kPer> p;
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) p.v[j] = v[j];
+                store_pack<T, kPer>(static_cast<T*>(a.dst) + at, p);
+            }
         }
     }
 }
@@ -525,33 +517,54 @@ bool loadable(const void* p, int64_t pitch, int64_t group_stride, int32_t type) 
            pitch * size < (1ll << 40) && group_stride * size < (1ll << 40);
 }
 
-// Copies [groups][rows][cols] at strides (s0, s1, s2) into `*work`, and moves `*work` on.
-int pack(const void* src, int64_t s0, int64_t s1, int64_t s2, int64_t groups, int64_t rows, int64_t cols, int32_t type, uint8_t** work,
-         cudaStream_t s) {
-    PackArgs p{src, *work, s0, s1, s2, groups, rows, (int32_t)cols, (int32_t)pitch_of(cols, type)};
-    const int64_t threads = groups * rows * (p.pitch / (type == FG_E4M3 ? 16 : 8)), most = (int64_t)fg::device_props().sm_count * 16;
-    const unsigned blocks = (unsigned)((threads + 255) / 256 < most ? (threads + 255) / 256 : most);
-    if (threads == 0) return FG_OK;
-    if (type == FG_F32) pack_kernel<float><<<blocks, 256, 0, s>>>(p);
-    else if (type == FG_F16) pack_kernel<__half><<<blocks, 256, 0, s>>>(p);
-    else if (type == FG_BF16) pack_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(p);
-    else pack_kernel<__nv_fp8_e4m3><<<blocks, 256, 0, s>>>(p);
+// Copies [groups][rows][cols] at strides (s0, s1, s2) - or the rows that `order` names - into `*work`, and moves that on.
+int pack(const void* src, int64_t s0, int64_t s1, int64_t s2, int64_t groups, int64_t rows, int64_t cols, const int32_t* order, int32_t choices,
+         int64_t source_rows, int32_t type, uint8_t** work, cudaStream_t s) {
+    const int size = fg::type_size(type), per = type == FG_E4M3 ? 16 : 8;
+    PackArgs p{src, *work, order, s0, s1, s2, groups, rows, source_rows, (int32_t)cols, (int32_t)pitch_of(cols, type), choices, 0, false};
+    p.vector = s2 == 1 && fg::aligned16(src) && s0 * size % 16 == 0 && s1 * size % 16 == 0;
+    while (p.shift < 8 && (1 << p.shift) < p.pitch / per) ++p.shift;
+    const int64_t blocks = ((groups * rows << p.shift) + 255) / 256, most = (int64_t)fg::device_props().sm_count * 32;
+    if (blocks == 0) return FG_OK;
+    const unsigned grid = (unsigned)(blocks < most ? blocks : most);
+    if (type == FG_F32) pack_kernel<float><<<grid, 256, 0, s>>>(p);
+    else if (type == FG_F16) pack_kernel<__half><<<grid, 256, 0, s>>>(p);
+    else if (type == FG_BF16) pack_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
+    else pack_kernel<__nv_fp8_e4m3><<<grid, 256, 0, s>>>(p);
     FG_CUDA_TRY(cudaGetLastError());
     fg::count_launches(1);
     *work += packed_bytes(groups * rows, cols, type);
     return FG_OK;
 }
 
-// Rows [rows, cols] with a row stride as a loadable matrix, copied if need be.
-int rows_matrix(Matrix* m, const void* p, int64_t ld, int64_t rows, int64_t cols, int32_t type, uint8_t** work, cudaStream_t s) {
-    if (loadable(p, ld, 0, type)) {
-        *m = Matrix{p, cols, rows, 0, ld, 0, type};
+// The slots' rows [m, cols] as a loadable matrix: where they lie, or copied.
+bool rows_need_copy(const void* p, int64_t ld, const int32_t* order, int32_t type) { return order || !loadable(p, ld, 0, type); }
+int rows_matrix(Matrix* out, const void* p, int64_t ld, int64_t source_rows, const int32_t* order, int32_t choices, int64_t m, int64_t cols,
+                int32_t type, uint8_t** work, cudaStream_t s) {
+    if (!rows_need_copy(p, ld, order, type)) {
+        *out = Matrix{p, cols, m, 0, ld, 0, type};
         return FG_OK;
     }
     const int parts = type == FG_F32 ? 3 : 1;
-    *m = Matrix{*work, cols, rows * parts, 0, pitch_of(cols, type), 0, type == FG_F32 ? FG_BF16 : type};
-    return pack(p, 0, ld, 1, 1, rows, cols, type, work, s);
+    *out = Matrix{*work, cols, m * parts, 0, pitch_of(cols, type), 0, type == FG_F32 ? FG_BF16 : type};
+    return pack(p, 0, ld, 1, 1, m, cols, order, choices, source_rows, type, work, s);
 }
+
+// The weight is read as it is stored where its inner or its outer axis is dense (8-bit products want the inner one), or
+// copied with that axis dense; a group stride of 0 is one weight for all groups.
+struct WeightLayout {
+    int64_t count, rows, cols;
+    bool b_mn, copy;
+    WeightLayout(const void* p, int64_t w_group, int64_t w_out, int64_t w_in, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
+        const bool k_dense = w_in == 1 || inner == 1, n_dense = type != FG_E4M3 && (w_out == 1 || outer == 1);
+        const bool k_loads = k_dense && loadable(p, w_out, w_group, type), n_loads = n_dense && loadable(p, w_in, w_group, type);
+        b_mn = k_loads ? false : n_loads ? true : !k_dense && n_dense;
+        copy = !k_loads && !n_loads;
+        count = w_group == 0 ? 1 : groups;
+        rows = b_mn ? inner : outer;
+        cols = b_mn ? outer : inner;
+    }
+};
 
 template <int BN, bool EIGHT, bool WGRAD>
 int launch_shape(const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b, int64_t most_tiles, cudaStream_t s) {
@@ -588,6 +601,11 @@ int64_t wgrad_tiles(int32_t inner, int32_t outer) {
     return (int64_t)((outer + kTileRows - 1) / kTileRows) * ((inner + 127) / 128);
 }
 
+int64_t partial_bytes(int64_t m, int32_t groups, int32_t inner, int32_t outer) {
+    const int64_t split = split_rows(m, groups, wgrad_tiles(inner, outer));
+    return split ? round_up((m / split + groups) * (int64_t)inner * outer * 4, 256) : 0;
+}
+
 int check_product(int64_t m, int64_t x_rows, int32_t choices, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
     if (m < 0 || m > INT_MAX - 1024 || x_rows < 0 || x_rows > INT_MAX || choices < 1 || groups < 1 || groups > kMaxGroups || inner < 1 || outer < 1 ||
         (type == FG_F32 && (m > INT_MAX / 4 || x_rows > INT_MAX / 4)))
@@ -608,10 +626,12 @@ int fg_grouped_matmul_status(void* stream) {
     return v ? fg::fail(FG_ERR_CUDA, "a grouped product gave up waiting for its own copies") : FG_OK;
 }
 
-int64_t fg_grouped_matmul_workspace(int64_t num_rows, int64_t x_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
-    if (num_rows <= 0 || x_rows < 0 || groups < 1 || inner < 1 || outer < 1) return 0;
-    const int64_t k_major = packed_bytes((int64_t)groups * outer, inner, type), mn_major = packed_bytes((int64_t)groups * inner, outer, type);
-    return packed_bytes(x_rows, inner, type) + (k_major > mn_major ? k_major : mn_major);
+int64_t fg_grouped_matmul_workspace(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,
+                                    const int32_t* d_order, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
+    if (num_rows <= 0 || groups < 1 || inner < 1 || outer < 1) return 0;
+    const WeightLayout w(d_w, w_group, w_out, w_in, groups, inner, outer, type);
+    return (rows_need_copy(d_x, ldx ? ldx : inner, d_order, type) ? packed_bytes(num_rows, inner, type) : 0) +
+           (w.copy ? packed_bytes(w.count * w.rows, w.cols, type) : 0);
 }
 
 int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, const void* d_w, int64_t w_group, int64_t w_out,
@@ -631,46 +651,41 @@ int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, con
     if (!d_order && x_rows != num_rows) return fg::fail(FG_ERR_INVALID_ARGUMENT, "without an order x has a row for each slot");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
 
-    // The weight is read as it is stored where its inner or its outer axis is dense (8-bit products want the inner one).
-    const bool shared = w_group == 0;
-    const int64_t count = shared ? 1 : groups;
-    const bool k_dense = w_in == 1 || inner == 1, n_dense = type != FG_E4M3 && (w_out == 1 || outer == 1);
-    const bool k_loads = k_dense && loadable(d_w, w_out, w_group, type), n_loads = n_dense && loadable(d_w, w_in, w_group, type);
-    const bool b_mn = k_loads ? false : n_loads ? true : !k_dense && n_dense;
-    const bool pack_w = !k_loads && !n_loads, pack_x = !loadable(d_x, ldx, 0, type);
-    const int64_t need = (pack_x ? packed_bytes(x_rows, inner, type) : 0) +
-                         (pack_w ? packed_bytes(count * (b_mn ? inner : outer), b_mn ? outer : inner, type) : 0);
+    const WeightLayout layout(d_w, w_group, w_out, w_in, groups, inner, outer, type);
+    const int64_t need = fg_grouped_matmul_workspace(d_x, ldx, d_w, w_group, w_out, w_in, d_order, num_rows, groups, inner, outer, type);
     if (workspace_bytes < need || (need && !d_workspace)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_grouped_matmul_workspace()");
     uint8_t* work = static_cast<uint8_t*>(d_workspace);
     Matrix x, w;
-    if (int rc = rows_matrix(&x, d_x, ldx, x_rows, inner, type, &work, s)) return rc;
-    const int64_t rows = b_mn ? inner : outer, cols = b_mn ? outer : inner, parts = type == FG_F32 ? 3 : 1;
-    if (!pack_w) {
-        w = Matrix{d_w, cols, rows, count, b_mn ? w_in : w_out, shared ? rows * (b_mn ? w_in : w_out) : w_group, type};
+    if (int rc = rows_matrix(&x, d_x, ldx, x_rows, d_order, choices, num_rows, inner, type, &work, s)) return rc;
+    const bool b_mn = layout.b_mn;
+    const int64_t step = b_mn ? w_in : w_out;  // of the weight's rows as stored
+    if (!layout.copy) {
+        w = Matrix{d_w, layout.cols, layout.rows, layout.count, step, w_group ? w_group : layout.rows * step, type};
     } else {
-        const int64_t pitch = pitch_of(cols, type);
-        w = Matrix{work, cols, rows, count * parts, pitch, rows * pitch, type == FG_F32 ? FG_BF16 : type};
-        if (int rc = pack(d_w, w_group, b_mn ? w_in : w_out, b_mn ? w_out : w_in, count, rows, cols, type, &work, s)) return rc;
+        const int64_t pitch = pitch_of(layout.cols, type);
+        w = Matrix{work, layout.cols, layout.rows, layout.count * (type == FG_F32 ? 3 : 1), pitch, layout.rows * pitch, type == FG_F32 ? FG_BF16 : type};
+        if (int rc = pack(d_w, w_group, step, b_mn ? w_out : w_in, layout.count, layout.rows, layout.cols, nullptr, 1, 0, type, &work, s)) return rc;
     }
     const int64_t units = num_rows / kTileRows + (groups < num_rows ? groups : num_rows);
     const int bn = tile_width(units, outer), chunk = type == FG_E4M3 ? 128 : 64;
     CUtensorMap map_x, map_w;
-    if (int rc = make_map(&map_x, x, chunk, d_order ? 1 : kTileRows)) return rc;
+    if (int rc = make_map(&map_x, x, chunk, kTileRows)) return rc;
     if (int rc = make_map(&map_w, w, chunk, b_mn ? 64 : bn)) return rc;
     MmaArgs a{};
     a.offsets = d_offsets, a.order = d_order, a.x_scales = d_x_scales, a.w_scales = d_w_scales, a.y = d_y;
     a.m = num_rows, a.x_rows = x_rows, a.choices = choices, a.groups = groups, a.inner = inner, a.outer = outer;
     a.type = type, a.out_type = out_type, a.format = w.type == FG_BF16 ? 1 : 0, a.first_pair = type == FG_F32 ? 0 : 5;
-    a.b_mn = b_mn, a.gather = d_order != nullptr, a.shared_weight = shared;
+    a.b_mn = b_mn, a.shared_weight = w_group == 0;
     const int64_t tiles = units * ((outer + bn - 1) / bn);
     return type == FG_E4M3 ? launch<true, false>(bn, a, map_x, map_w, tiles, s) : launch<false, false>(bn, a, map_x, map_w, tiles, s);
 }
 
-int64_t fg_grouped_matmul_wgrad_workspace(int64_t num_rows, int64_t x_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
-    if (num_rows <= 0 || x_rows < 0 || groups < 1 || inner < 1 || outer < 1) return 0;
-    const int64_t split = split_rows(num_rows, groups, wgrad_tiles(inner, outer));
-    const int64_t partial = split ? round_up((num_rows / split + groups) * (int64_t)inner * outer * 4, 256) : 0;
-    return packed_bytes(x_rows, inner, type) + packed_bytes(num_rows, outer, type) + partial;
+int64_t fg_grouped_matmul_wgrad_workspace(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const int32_t* d_order,
+                                          int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
+    if (num_rows <= 0 || groups < 1 || inner < 1 || outer < 1) return 0;
+    return partial_bytes(num_rows, groups, inner, outer) +
+           (rows_need_copy(d_x, ldx ? ldx : inner, d_order, type) ? packed_bytes(num_rows, inner, type) : 0) +
+           (rows_need_copy(d_dy, lddy ? lddy : outer, nullptr, type) ? packed_bytes(num_rows, outer, type) : 0);
 }
 
 int fg_grouped_matmul_wgrad(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const int32_t* d_offsets,
@@ -690,26 +705,24 @@ int fg_grouped_matmul_wgrad(const void* d_x, int64_t ldx, const void* d_dy, int6
         return FG_OK;
     }
     const int64_t split = split_rows(num_rows, groups, wgrad_tiles(inner, outer));
-    const int64_t partial = split ? round_up((num_rows / split + groups) * cells * 4, 256) : 0;
-    const bool pack_x = !loadable(d_x, ldx, 0, type), pack_dy = !loadable(d_dy, lddy, 0, type);
-    const int64_t need = partial + (pack_x ? packed_bytes(x_rows, inner, type) : 0) + (pack_dy ? packed_bytes(num_rows, outer, type) : 0);
+    const int64_t need = fg_grouped_matmul_wgrad_workspace(d_x, ldx, d_dy, lddy, d_order, num_rows, groups, inner, outer, type);
     if (workspace_bytes < need || (need && !d_workspace)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_grouped_matmul_wgrad_workspace()");
     uint8_t* work = static_cast<uint8_t*>(d_workspace);
     float* sums = reinterpret_cast<float*>(work);
-    work += partial;
+    work += partial_bytes(num_rows, groups, inner, outer);
     Matrix x, dy;
-    if (int rc = rows_matrix(&x, d_x, ldx, x_rows, inner, type, &work, s)) return rc;
-    if (int rc = rows_matrix(&dy, d_dy, lddy, num_rows, outer, type, &work, s)) return rc;
+    if (int rc = rows_matrix(&x, d_x, ldx, x_rows, d_order, choices, num_rows, inner, type, &work, s)) return rc;
+    if (int rc = rows_matrix(&dy, d_dy, lddy, num_rows, nullptr, 1, num_rows, outer, type, &work, s)) return rc;
     CUtensorMap map_x, map_dy;
     if (int rc = make_map(&map_dy, dy, 64, 64)) return rc;
-    if (int rc = make_map(&map_x, x, 64, d_order ? 1 : 64)) return rc;
+    if (int rc = make_map(&map_x, x, 64, 64)) return rc;
     const int64_t units = split ? num_rows / split + groups : groups, rows_tiles = (outer + kTileRows - 1) / kTileRows;
     const int bn = tile_width(units * rows_tiles, inner);
     MmaArgs a{};
     a.offsets = d_offsets, a.order = d_order, a.y = split ? static_cast<void*>(sums) : d_dw;
     a.m = num_rows, a.x_rows = x_rows, a.choices = choices, a.groups = groups, a.inner = inner, a.outer = outer;
     a.type = type, a.out_type = split ? FG_F32 : type, a.format = dy.type == FG_BF16 ? 1 : 0, a.first_pair = type == FG_F32 ? 0 : 5;
-    a.gather = d_order != nullptr, a.split = (int32_t)split, a.units = (int32_t)units;
+    a.split = (int32_t)split, a.units = (int32_t)units;
     if (int rc = launch<false, true>(bn, a, map_dy, map_x, units * rows_tiles * ((inner + bn - 1) / bn), s)) return rc;
     if (split) {
         const dim3 grid((unsigned)((cells + 1023) / 1024 < 4096 ? (cells + 1023) / 1024 : 4096), (unsigned)groups);

@@ -1,5 +1,5 @@
 // Thin wrappers of the sm_100a instructions the grouped product is built from: mbarriers with bounded waits, TMA tile
-// loads and row gathers, tcgen05 products with their accumulators in tensor memory.
+// loads, tcgen05 products with their accumulators in tensor memory.
 #pragma once
 #include <cuda.h>
 
@@ -53,14 +53,6 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
     asm volatile(
         "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
         "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-        : "memory");
-}
-// Four rows of a 2-D map (its box is one row high) into consecutive rows of the tile.
-__device__ __forceinline__ void tma_gather_4(uint32_t dst, const CUtensorMap* map, int x, int r0, int r1, int r2, int r3, uint32_t bar) {
-    asm volatile(
-        "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
-            dst),
-        "l"(map), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
         : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }

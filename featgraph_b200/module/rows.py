@@ -318,11 +318,11 @@ def route(logits, k, scoring="softmax", normalize=True):
 def _product(x, ldx, x_scales, w, strides, w_scales, groups, gather, x_rows, inner, outer, out_dtype):
     device, kind = x.device, _TYPES[x.dtype]
     y = torch.empty((groups.num_entries, outer), dtype=out_dtype, device=device)
-    size = dev.lib().fg_grouped_matmul_workspace(groups.num_entries, x_rows, groups.num_groups, inner, outer, kind)
+    order, m = (groups.order.data_ptr() if gather else None), groups.num_entries
+    size = dev.lib().fg_grouped_matmul_workspace(x.data_ptr(), ldx, w.data_ptr(), *strides, order, m, groups.num_groups, inner, outer, kind)
     work = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
     _call("fg_grouped_matmul", device, x.data_ptr(), ldx, _ptr(x_scales), w.data_ptr(), *strides, _ptr(w_scales), groups.offsets.data_ptr(),
-          groups.order.data_ptr() if gather else None, groups.choices, x_rows, y.data_ptr(), groups.num_entries, groups.num_groups, inner,
-          outer, kind, _TYPES[out_dtype], _ptr(work), size)
+          order, groups.choices, x_rows, y.data_ptr(), m, groups.num_groups, inner, outer, kind, _TYPES[out_dtype], _ptr(work), size)
     return y
 
 
@@ -351,11 +351,11 @@ class _Product(torch.autograd.Function):
             xr, ldx = _as_rows(x)
             kind = _TYPES[x.dtype]
             dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
-            size = dev.lib().fg_grouped_matmul_wgrad_workspace(groups.num_entries, x.shape[0], groups.num_groups, inner, outer, kind)
+            order, m = (groups.order.data_ptr() if gather else None), groups.num_entries
+            size = dev.lib().fg_grouped_matmul_wgrad_workspace(xr.data_ptr(), ldx, dyr.data_ptr(), ldy, order, m, groups.num_groups, inner, outer, kind)
             work = torch.empty((size,), dtype=torch.uint8, device=w.device) if size else None
             _call("fg_grouped_matmul_wgrad", x.device, xr.data_ptr(), ldx, dyr.data_ptr(), ldy, groups.offsets.data_ptr(),
-                  groups.order.data_ptr() if gather else None, groups.choices, x.shape[0], dw.data_ptr(), groups.num_entries,
-                  groups.num_groups, inner, outer, kind, _ptr(work), size)
+                  order, groups.choices, x.shape[0], dw.data_ptr(), m, groups.num_groups, inner, outer, kind, _ptr(work), size)
         return dx, dw, None, None
 
 

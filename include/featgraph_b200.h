@@ -379,19 +379,22 @@ int64_t fg_group_rows_workspace(int64_t num_entries, int32_t num_groups);
 int fg_group_rows(const int32_t* d_keys, int64_t num_entries, int32_t num_groups, int32_t* d_offsets, int32_t* d_order,
                   int32_t* d_position, void* d_workspace, int64_t workspace_bytes, void* stream);
 
-/* y[p, o] = sum over i of x[row(p), i] * w[g, o, i] for the rows p of each group g; rows in no group are 0.
+/* Workspaces: as large as the *_workspace call says for the same arguments.
+ * y[p, o] = sum over i of x[row(p), i] * w[g, o, i] for the rows p of each group g; rows in no group are 0.
  * row(p) = p where d_order is NULL, else d_order[p] / choices.  w[g, o, i] is d_w[g w_group + o w_out + i w_in].
  * FG_E4M3: times d_x_scales[row(p)] * d_w_scales[g * outer + o], output of out_type.  y dense, [num_rows, outer].
  * The products wait for their own copies with a limit: fg_grouped_matmul_status synchronises `stream` and returns
  * FG_ERR_CUDA if one ever ran out on this device (its output is then wrong).
  * fg_grouped_matmul_wgrad: d_dw[g, o, i] = sum over the rows p of g of dy[p, o] * x[row(p), i], dense. */
 int fg_grouped_matmul_status(void* stream);
-int64_t fg_grouped_matmul_workspace(int64_t num_rows, int64_t x_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type);
+int64_t fg_grouped_matmul_workspace(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,
+                                    const int32_t* d_order, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type);
 int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, const void* d_w, int64_t w_group, int64_t w_out,
                       int64_t w_in, const float* d_w_scales, const int32_t* d_offsets, const int32_t* d_order, int32_t choices,
                       int64_t x_rows, void* d_y, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type,
                       int32_t out_type, void* d_workspace, int64_t workspace_bytes, void* stream);
-int64_t fg_grouped_matmul_wgrad_workspace(int64_t num_rows, int64_t x_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type);
+int64_t fg_grouped_matmul_wgrad_workspace(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const int32_t* d_order,
+                                          int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type);
 int fg_grouped_matmul_wgrad(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const int32_t* d_offsets,
                             const int32_t* d_order, int32_t choices, int64_t x_rows, void* d_dw, int64_t num_rows, int32_t groups,
                             int32_t inner, int32_t outer, int32_t type, void* d_workspace, int64_t workspace_bytes, void* stream);
