@@ -52,7 +52,7 @@ SIGNATURES = {
     "fg_rms_norm_backward_blocks": (_i64, [_i64, _i32]),
     "fg_rms_norm_backward": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i32, _f32, _i32, _i32,
                                             _vp]),
-    "fg_route": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp]),
+    "fg_route": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
     "fg_route_backward": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp]),
     "fg_group_rows_workspace": (_i64, [_i64, _i32]),
     "fg_group_rows": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),

@@ -60,7 +60,8 @@ struct Shape {
     static constexpr int kStageBytes = (kTileRows + BN) * kChunkBytes;
     static constexpr int kStages = 196608 / kStageBytes;
     static constexpr int kColumns = 2 * BN;
-    static constexpr int kSmem = 1024 + kStages * kStageBytes;
+    static constexpr int kStaging = kStages * kStageBytes;  // 4 KB for each output warp
+    static constexpr int kSmem = 1024 + kStaging + 4 * 4096;
 };
 
 struct Tables {
@@ -72,21 +73,66 @@ struct Tables {
     int tiles[kMaxGroups + 1];  // row tiles (partial sums of dW) before each group
 };
 
-template <typename O>
-__device__ __forceinline__ void store_32(O* out, const float (&v)[32], int left, bool vector) {
-    constexpr int kVec = 16 / sizeof(O);
-    if (vector && left >= 32) {
+// Takes a warp's 32 rows of an accumulator, from `tmem` on, to the output rows from `out` on (row pitch `width`; rows >=
+// `rows` and columns >= `left` are not stored).  A thread holds a row in tensor memory's layout, so 128-byte wide pieces go
+// through the warp's 4 KB of shared memory (16-byte cells, XOR-swizzled: no bank conflicts either way) and leave as whole
+// 128-byte lines, 8 lanes a row.  Stored straight from the threads, 16 bytes in each of 32 rows at a time, the output
+// of a 65536 x 4096 product kept the products waiting.
+template <typename O, int BN, bool EIGHT>
+__device__ __forceinline__ void store_rows(uint32_t tmem, bool filled, O* out, int64_t width, int rows, int left, bool vector, uint32_t staging,
+                                           float scale, const float* column_scales) {
+    constexpr int kCols = 128 / sizeof(O), kCells = 16 / sizeof(O);
+    const int lane = threadIdx.x & 31;
+    for (int c = 0; c < BN; c += kCols, left -= kCols) {
+        if (left <= 0) break;
+        uint32_t raw[kCols / 32][32];
+        if (filled) {
 #pragma unroll
-        for (int i = 0; i < 32; i += kVec) {
-            Pack<O, kVec> p;
+            for (int h = 0; h < kCols / 32; ++h) fg::tmem_load_32(tmem + c + h * 32, raw[h]);
+            fg::tmem_load_wait();
+        } else {
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) p.v[j] = from_f32<O>(v[i + j]);
-            store_pack<O, kVec>(out + i, p);
+            for (int j = 0; j < kCols; ++j) raw[j / 32][j % 32] = 0;
         }
-    } else {
 #pragma unroll
-        for (int i = 0; i < 32; ++i)
-            if (i < left) out[i] = from_f32<O>(v[i]);
+        for (int q = 0; q < 8; ++q) {
+            Pack<O, kCells> p;
+#pragma unroll
+            for (int j = 0; j < kCells; ++j) {
+                const int k = q * kCells + j;
+                float v = __uint_as_float(raw[k / 32][k % 32]);
+                if (EIGHT) v = __fmul_rn(__fmul_rn(v, scale), k < left ? column_scales[c + k] : 0.0f);
+                p.v[j] = from_f32<O>(v);
+            }
+            const uint32_t* word = reinterpret_cast<const uint32_t*>(&p);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 128 + ((q ^ (lane & 7)) << 4)), "r"(word[0]), "r"(word[1]),
+                         "r"(word[2]), "r"(word[3])
+                         : "memory");
+        }
+        __syncwarp();
+        if (vector) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = i * 4 + (lane >> 3), q = lane & 7;
+                Pack<uint32_t, 4> p;
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(p.v[0]), "=r"(p.v[1]), "=r"(p.v[2]), "=r"(p.v[3])
+                             : "r"(staging + r * 128 + ((q ^ (r & 7)) << 4))
+                             : "memory");
+                if (r < rows && q * kCells < left) store_pack<uint32_t, 4>(reinterpret_cast<uint32_t*>(out + r * width + c + q * kCells), p);
+            }
+        } else {
+            for (int r = 0; r < min(rows, 32); ++r)
+#pragma unroll
+                for (int k = lane; k < kCols; k += 32) {
+                    const uint32_t at = staging + r * 128 + (((k / kCells) ^ (r & 7)) << 4) + (k % kCells) * sizeof(O);
+                    O v;
+                    if constexpr (sizeof(O) == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(*reinterpret_cast<uint32_t*>(&v)) : "r"(at) : "memory");
+                    else asm volatile("ld.shared.b16 %0, [%1];" : "=h"(*reinterpret_cast<uint16_t*>(&v)) : "r"(at) : "memory");
+                    if (k < left) out[r * width + c + k] = v;
+                }
+        }
+        __syncwarp();
     }
 }
 
@@ -298,62 +344,40 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
     } else {
         const int quarter = warp & 3;  // the lanes of tensor memory this warp can read
+        const uint32_t staging = ring + S::kStaging + quarter * 4096;
         const int width = WGRAD ? a.inner : a.outer;
         const int size = a.out_type == FG_F32 ? 4 : 2;
         const bool vector = (int64_t)width * size % 16 == 0 && ((uintptr_t)a.y & 15) == 0;
         int64_t turn = 0;
         for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
             const Tile w = locate(i);
-            const int row = quarter * 32 + lane;
-            int64_t out_row;
-            bool in, zero = false;
-            float scale = 1.0f;
-            if (WGRAD) {
-                in = w.row + row < a.outer;
-                out_row = (int64_t)(a.split ? w.unit : w.group) * a.outer + w.row + row;
-                zero = w.chunks == 0;
-            } else {
-                const int slot = w.begin + row;
-                in = slot < w.end;
-                out_row = slot;
-                if (EIGHT && in) {
+            const int above = quarter * 32;
+            const int rows = (WGRAD ? a.outer - w.row : w.end - w.begin) - above;
+            const int64_t first = (WGRAD ? (int64_t)(a.split ? w.unit : w.group) * a.outer + w.row : w.begin) + above;
+            float scale = 0.0f;
+            const float* column_scales = nullptr;
+            if (EIGHT) {
+                const int slot = w.begin + above + lane;
+                if (slot < w.end) {
                     const int e = a.order ? a.order[slot] : 0, r = a.order ? e / a.choices : slot;
-                    scale = e >= 0 && r < a.x_rows ? a.x_scales[r] : 0.0f;
+                    if (e >= 0 && r < a.x_rows) scale = a.x_scales[r];
                 }
+                column_scales = a.w_scales + (int64_t)w.group * a.outer + w.col;
             }
             const int buffer = (int)(turn & 1);
             if (w.chunks) {
                 if (!warp_wait(fg::smem_address(&t.filled[buffer]), (turn / 2) & 1, stop)) break;
                 fg::tcgen05_after_sync();
             }
-            for (int c = 0; c < BN; c += 32) {
-                if (w.col + c >= width) break;
-                float v[32];
-                if (w.chunks) {
-                    uint32_t raw[32];
-                    fg::tmem_load_32(tmem + ((uint32_t)(quarter * 32) << 16) + buffer * BN + c, raw);
-                    fg::tmem_load_wait();
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(raw[j]);
-                }
-                const int left = width - w.col - c;
-                if (EIGHT) {
-                    const float* ws = a.w_scales + (int64_t)w.group * a.outer + w.col + c;
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __fmul_rn(__fmul_rn(v[j], scale), j < left ? ws[j] : 0.0f);
-                }
-                if (zero) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-                }
-                if (in) {
-                    const int64_t at = out_row * width + w.col + c;
-                    if (a.out_type == FG_F32) store_32<float>(static_cast<float*>(a.y) + at, v, left, vector);
-                    else if (a.out_type == FG_F16) store_32<__half>(static_cast<__half*>(a.y) + at, v, left, vector);
-                    else store_32<__nv_bfloat16>(static_cast<__nv_bfloat16*>(a.y) + at, v, left, vector);
-                }
-                __syncwarp();
-            }
+            const uint32_t acc = tmem + ((uint32_t)above << 16) + buffer * BN;
+            const int64_t at = first * width + w.col;
+            if (a.out_type == FG_F32)
+                store_rows<float, BN, EIGHT>(acc, w.chunks > 0, static_cast<float*>(a.y) + at, width, rows, width - w.col, vector, staging, scale, column_scales);
+            else if (a.out_type == FG_F16)
+                store_rows<__half, BN, EIGHT>(acc, w.chunks > 0, static_cast<__half*>(a.y) + at, width, rows, width - w.col, vector, staging, scale, column_scales);
+            else
+                store_rows<__nv_bfloat16, BN, EIGHT>(acc, w.chunks > 0, static_cast<__nv_bfloat16*>(a.y) + at, width, rows, width - w.col, vector, staging, scale,
+                                                     column_scales);
             if (w.chunks) {
                 fg::tcgen05_before_sync();
                 __syncwarp();
@@ -568,7 +592,12 @@ struct WeightLayout {
 
 template <int BN, bool EIGHT, bool WGRAD>
 int launch_shape(const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b, int64_t most_tiles, cudaStream_t s) {
-    FG_CUDA_TRY(cudaFuncSetAttribute(product_kernel<BN, EIGHT, WGRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN>::kSmem));
+    static bool ready[fg::kMaxDevices];  // set once a device; setting it twice does no harm
+    const int slot = fg::current_device_slot();
+    if (slot < 0 || !ready[slot]) {
+        FG_CUDA_TRY(cudaFuncSetAttribute(product_kernel<BN, EIGHT, WGRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN>::kSmem));
+        if (slot >= 0) ready[slot] = true;
+    }
     const int64_t sms = fg::device_props().sm_count;
     product_kernel<BN, EIGHT, WGRAD><<<(unsigned)(most_tiles < sms ? most_tiles : sms), kThreads, Shape<BN>::kSmem, s>>>(a, map_a, map_b);
     FG_CUDA_TRY(cudaGetLastError());

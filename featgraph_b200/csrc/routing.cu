@@ -50,10 +50,8 @@ struct RouteArgs {
 // keeps the j-th choice.  Bound: the n * E logits are read once (65,536 x 128: 33.6 MB, 5 us), but k rounds of two
 // warp-wide reductions a row are what the time goes to.
 template <typename T, int NE>
-__global__ void __launch_bounds__(256) route_kernel(const RouteArgs a) {
+__device__ __forceinline__ void route_row(const RouteArgs& a, int64_t row) {
     const int lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-    if (row >= a.n) return;
     const T* x = static_cast<const T*>(a.logits) + row * a.ld;
     uint32_t key[NE];
 #pragma unroll
@@ -102,6 +100,12 @@ __global__ void __launch_bounds__(256) route_kernel(const RouteArgs a) {
         a.weights[row * a.k + lane] = score;
         a.chosen[row * a.k + lane] = mine;
     }
+}
+
+template <typename T, int NE>
+__global__ void __launch_bounds__(256) route_kernel(const RouteArgs a) {
+    const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+    if (row < a.n) route_row<T, NE>(a, row);
 }
 
 struct RouteGradArgs {
@@ -189,35 +193,6 @@ __global__ void __launch_bounds__(256) route_grad_kernel(const RouteGradArgs a) 
     }
 }
 
-// Calls f.template operator()<T, NE>() with the smallest NE that covers the experts.
-template <typename T, typename F>
-void by_experts(int experts, F&& f) {
-    if (experts <= 32) f.template operator()<T, 1>();
-    else if (experts <= 64) f.template operator()<T, 2>();
-    else if (experts <= 128) f.template operator()<T, 4>();
-    else if (experts <= 256) f.template operator()<T, 8>();
-    else if (experts <= 512) f.template operator()<T, 16>();
-    else f.template operator()<T, 32>();
-}
-template <typename F>
-void by_logit_type(int32_t type, int experts, F&& f) {
-    if (type == FG_F32) by_experts<float>(experts, f);
-    else if (type == FG_F16) by_experts<__half>(experts, f);
-    else by_experts<__nv_bfloat16>(experts, f);
-}
-struct LaunchRoute {
-    const RouteArgs& a;
-    cudaStream_t s;
-    template <typename T, int NE>
-    void operator()() const { route_kernel<T, NE><<<(unsigned)((a.n + 7) / 8), 256, 0, s>>>(a); }
-};
-struct LaunchRouteGrad {
-    const RouteGradArgs& a;
-    cudaStream_t s;
-    template <typename T, int NE>
-    void operator()() const { route_grad_kernel<T, NE><<<(unsigned)((a.n + 7) / 8), 256, 0, s>>>(a); }
-};
-
 // ---- lists ----
 
 // Entries are cut into chunks, a block each; in a chunk every warp owns a run of consecutive entries.  Pass 1 counts
@@ -291,8 +266,7 @@ __global__ void __launch_bounds__(1024) group_scan_kernel(const GroupArgs a) {
 }
 
 template <bool SINGLE>
-__global__ void __launch_bounds__(1024) group_place_kernel(const GroupArgs a) {
-    extern __shared__ int cell[];  // [warps][groups + 1]
+__device__ __forceinline__ void place_entries(const GroupArgs& a, int* cell) {  // cell: [warps][groups + 1]
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, bins = a.groups + 1;
     for (int i = threadIdx.x; i < warps * bins; i += blockDim.x) cell[i] = 0;
     __syncthreads();
@@ -341,6 +315,62 @@ __global__ void __launch_bounds__(1024) group_place_kernel(const GroupArgs a) {
         }
     }
 }
+
+template <bool SINGLE>
+__global__ void __launch_bounds__(1024) group_place_kernel(const GroupArgs a) {
+    extern __shared__ int cell[];
+    place_entries<SINGLE>(a, cell);
+}
+
+// Choice and lists of a few rows in one launch: one block chooses for all rows, a warp a row, and then lists them.
+template <typename T, int NE>
+__global__ void __launch_bounds__(512) route_lists_kernel(const RouteArgs a, const GroupArgs g) {
+    extern __shared__ int cell[];
+    for (int64_t row = threadIdx.x >> 5; row < a.n; row += blockDim.x >> 5) route_row<T, NE>(a, row);
+    __syncthreads();  // the choices are in global memory, written by this block
+    place_entries<true>(g, cell);
+}
+
+// Calls f.template operator()<T, NE>() with the smallest NE that covers the experts.
+template <typename T, typename F>
+void by_experts(int experts, F&& f) {
+    if (experts <= 32) f.template operator()<T, 1>();
+    else if (experts <= 64) f.template operator()<T, 2>();
+    else if (experts <= 128) f.template operator()<T, 4>();
+    else if (experts <= 256) f.template operator()<T, 8>();
+    else if (experts <= 512) f.template operator()<T, 16>();
+    else f.template operator()<T, 32>();
+}
+template <typename F>
+void by_logit_type(int32_t type, int experts, F&& f) {
+    if (type == FG_F32) by_experts<float>(experts, f);
+    else if (type == FG_F16) by_experts<__half>(experts, f);
+    else by_experts<__nv_bfloat16>(experts, f);
+}
+struct LaunchRoute {
+    const RouteArgs& a;
+    cudaStream_t s;
+    template <typename T, int NE>
+    void operator()() const { route_kernel<T, NE><<<(unsigned)((a.n + 7) / 8), 256, 0, s>>>(a); }
+};
+struct LaunchRouteLists {
+    const RouteArgs& a;
+    const GroupArgs& g;
+    cudaStream_t s;
+    template <typename T, int NE>
+    void operator()() const {
+        const int warps = a.n <= 4 ? 4 : a.n <= 8 ? 8 : 16;
+        const size_t smem = (size_t)warps * (g.groups + 1) * 4;
+        if (smem > 48 * 1024) (void)cudaFuncSetAttribute(route_lists_kernel<T, NE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+        route_lists_kernel<T, NE><<<1, warps * 32, smem, s>>>(a, g);
+    }
+};
+struct LaunchRouteGrad {
+    const RouteGradArgs& a;
+    cudaStream_t s;
+    template <typename T, int NE>
+    void operator()() const { route_grad_kernel<T, NE><<<(unsigned)((a.n + 7) / 8), 256, 0, s>>>(a); }
+};
 
 // ---- weighted sum back ----
 
@@ -460,6 +490,9 @@ int check_route(int64_t n, int32_t experts, int32_t k, int32_t type, int32_t sco
     return FG_OK;
 }
 
+// Rows that one block chooses and lists by itself: a second launch costs about 3 us, a warp some 2 us a row.
+constexpr int64_t kOneBlockRows = 32;
+
 // 8192 entries or fewer are one chunk; above that chunks of at least 2048, at most 1024 of them.
 int64_t chunk_size(int64_t m) {
     if (m <= 8192) return 8192;
@@ -471,20 +504,6 @@ int64_t chunk_size(int64_t m) {
 }  // namespace
 
 extern "C" {
-
-int fg_route(const void* d_logits, int64_t ld, float* d_weights, int32_t* d_experts, int64_t n, int32_t experts, int32_t k,
-             int32_t type, int32_t scoring, int32_t normalize, void* stream) {
-    if (int rc = check_route(n, experts, k, type, scoring)) return rc;
-    if (ld == 0) ld = experts;
-    if (ld < experts) return fg::fail(FG_ERR_INVALID_ARGUMENT, "the row stride must be 0 or >= experts=%d", experts);
-    if (n == 0) return FG_OK;
-    if (!d_logits || !d_weights || !d_experts) return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
-    const RouteArgs a{d_logits, ld, n, experts, k, scoring == FG_SCORE_SIGMOID, normalize != 0, d_weights, d_experts};
-    by_logit_type(type, experts, LaunchRoute{a, static_cast<cudaStream_t>(stream)});
-    FG_CUDA_TRY(cudaGetLastError());
-    fg::count_launches(1);
-    return FG_OK;
-}
 
 int fg_route_backward(const void* d_logits, int64_t ld, const float* d_weights, const int32_t* d_experts, const float* d_dweights,
                       void* d_dlogits, int64_t n, int32_t experts, int32_t k, int32_t type, int32_t scoring, int32_t normalize,
@@ -541,6 +560,31 @@ int fg_group_rows(const int32_t* d_keys, int64_t num_entries, int32_t num_groups
     FG_CUDA_TRY(cudaGetLastError());
     fg::count_launches(3);
     return FG_OK;
+}
+
+int fg_route(const void* d_logits, int64_t ld, float* d_weights, int32_t* d_experts, int32_t* d_offsets, int32_t* d_order,
+             int32_t* d_position, int64_t n, int32_t experts, int32_t k, int32_t type, int32_t scoring, int32_t normalize,
+             void* d_workspace, int64_t workspace_bytes, void* stream) {
+    if (int rc = check_route(n, experts, k, type, scoring)) return rc;
+    if (ld == 0) ld = experts;
+    if (ld < experts) return fg::fail(FG_ERR_INVALID_ARGUMENT, "the row stride must be 0 or >= experts=%d", experts);
+    if (n == 0) return d_offsets ? fg_group_rows(d_experts, 0, experts, d_offsets, d_order, d_position, d_workspace, workspace_bytes, stream) : FG_OK;
+    if (!d_logits || !d_weights || !d_experts || (d_offsets && (!d_order || !d_position))) return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
+    if (d_offsets && workspace_bytes < fg_group_rows_workspace(n * k, experts))
+        return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_group_rows_workspace()");
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const RouteArgs a{d_logits, ld, n, experts, k, scoring == FG_SCORE_SIGMOID, normalize != 0, d_weights, d_experts};
+    if (d_offsets && n <= kOneBlockRows) {
+        const GroupArgs g{d_experts, n * k, experts, (int32_t)(n * k), 1, nullptr, d_offsets, d_order, d_position};
+        by_logit_type(type, experts, LaunchRouteLists{a, g, s});
+        FG_CUDA_TRY(cudaGetLastError());
+        fg::count_launches(1);
+        return FG_OK;
+    }
+    by_logit_type(type, experts, LaunchRoute{a, s});
+    FG_CUDA_TRY(cudaGetLastError());
+    fg::count_launches(1);
+    return d_offsets ? fg_group_rows(d_experts, n * k, experts, d_offsets, d_order, d_position, d_workspace, workspace_bytes, stream) : FG_OK;
 }
 
 int fg_combine_rows(const void* d_y, int64_t ldy, const float* d_weights, const int32_t* d_position, void* d_out, int64_t n,

@@ -81,13 +81,30 @@ class Routing(NamedTuple):
     groups: RowGroups
 
 
-def _call(name, device, *args):
-    fn = getattr(dev.lib(), name)
-    if torch.cuda.current_device() == device.index:
-        dev.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+_entries = {}
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _call(name, index, *args):
+    """One library call on the current stream of device ``index``.  A small call's time is mostly spent on the way to it,
+    so the way is short: entry points are looked up once, the stream's address is read without a Stream object."""
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(dev.lib(), name)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(device):
-            dev.check(fn(*args, torch.cuda.current_stream(device).cuda_stream))
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        dev.check(rc)
+
+
+def _size(name, *args):
+    fn = _entries.get(name)
+    if fn is None:
+        fn = _entries[name] = getattr(dev.lib(), name)
+    return fn(*args)
 
 
 def _ptr(t):
@@ -104,20 +121,28 @@ def _tensor(t, what, dtypes, dims=None):
     return t
 
 
-def _on(device, **tensors):
-    dev.resolve_device(device)
-    for what, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError("%s lives on %s, the rows on %s" % (what, t.device, device))
+def _on(x, *others):
+    """The rows' device index; the tensors of ``others`` (name, tensor or None, ...) must be there too."""
+    if not x.is_cuda:
+        dev.resolve_device(x.device)
+    index = x.get_device()
+    for i in range(1, len(others), 2):
+        t = others[i]
+        if t is not None and (not t.is_cuda or t.get_device() != index):
+            raise ValueError("%s lives on %s, the rows on %s" % (others[i - 1], t.device, x.device))
+    return index
 
 
 def _as_rows(t):
     """t as a 2-D tensor whose rows are dense (a row stride of its own is kept), and that stride."""
     if t.dim() != 2:
-        t = t.reshape(-1, t.shape[-1]) if t.dim() else t
-    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.reshape(-1, t.shape[-1])
+    n, d = t.shape
+    ld, step = t.stride()
+    if d > 1 and step != 1 or n > 1 and ld < d:
         t = t.contiguous()
-    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+        ld = d
+    return t, (ld if n > 1 else d)
 
 
 def _wants_grad(*tensors):
@@ -127,17 +152,25 @@ def _wants_grad(*tensors):
 # ---- norm ----
 
 def _norm_forward(x, weight, residual, eps, quantize):
-    shape, d = x.shape, x.shape[-1]
     xr, ldx = _as_rows(x)
-    n = xr.shape[0]
-    rr, ldr = (None, 0) if residual is None else _as_rows(residual)
-    h = None if residual is None else torch.empty((n, d), dtype=x.dtype, device=x.device)
-    y = torch.empty((n, d), dtype=torch.float8_e4m3fn if quantize else x.dtype, device=x.device)
-    scales = torch.empty((n,), dtype=torch.float32, device=x.device) if quantize else None
-    kind = _TYPES[x.dtype]
-    _call("fg_rms_norm", x.device, xr.data_ptr(), ldx, _ptr(rr), ldr, _ptr(weight), _ptr(h), y.data_ptr(), _ptr(scales), n, d, eps, kind,
+    n, d = xr.shape
+    device, kind = x.device, _TYPES[x.dtype]
+    rr, ldr, h = None, 0, None
+    if residual is not None:
+        rr, ldr = _as_rows(residual)
+        h = torch.empty(n, d, dtype=x.dtype, device=device)
+    scales = None
+    if quantize:
+        y = torch.empty(n, d, dtype=torch.float8_e4m3fn, device=device)
+        scales = torch.empty(n, dtype=torch.float32, device=device)
+    else:
+        y = torch.empty(n, d, dtype=x.dtype, device=device)
+    _call("fg_rms_norm", x.get_device(), xr.data_ptr(), ldx, _ptr(rr), ldr, _ptr(weight), _ptr(h), y.data_ptr(), _ptr(scales), n, d, eps, kind,
           kind if weight is None else _TYPES[weight.dtype], 3 if quantize else kind)
-    return y.view(shape), None if h is None else h.view(shape), None if scales is None else scales.view(shape[:-1])
+    if x.dim() != 2:
+        shape = x.shape
+        y, h, scales = y.view(shape), None if h is None else h.view(shape), None if scales is None else scales.view(shape[:-1])
+    return y, h, scales
 
 
 class _Norm(torch.autograd.Function):
@@ -161,14 +194,14 @@ class _Norm(torch.autograd.Function):
         gr, ldg = _as_rows(dy)
         sr, lds = (None, 0) if dh is None else _as_rows(dh)
         n = hr.shape[0]
-        dx = torch.empty((n, d), dtype=h.dtype, device=h.device)
+        dx = torch.empty(n, d, dtype=h.dtype, device=h.device)
         dw = torch.empty_like(weight) if weight is not None and ctx.needs_input_grad[1] else None
         partial = None
-        blocks = dev.lib().fg_rms_norm_backward_blocks(n, d)
+        blocks = _size("fg_rms_norm_backward_blocks", n, d)
         if dw is not None:
-            partial = torch.empty((blocks, d), dtype=torch.float32, device=h.device)
+            partial = torch.empty(blocks, d, dtype=torch.float32, device=h.device)
         kind = _TYPES[h.dtype]
-        _call("fg_rms_norm_backward", h.device, hr.data_ptr(), ldh, _ptr(weight), gr.data_ptr(), ldg, _ptr(sr), lds, dx.data_ptr(), _ptr(dw),
+        _call("fg_rms_norm_backward", h.get_device(), hr.data_ptr(), ldh, _ptr(weight), gr.data_ptr(), ldg, _ptr(sr), lds, dx.data_ptr(), _ptr(dw),
               _ptr(partial), blocks, n, d, ctx.eps, kind, kind if weight is None else _TYPES[weight.dtype])
         dx = dx.view(h.shape)
         return dx if ctx.needs_input_grad[0] else None, dw, dx if ctx.needs_input_grad[2] else None, None
@@ -197,7 +230,7 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, quantize=False):
     eps = float(eps)
     if not eps >= 0.0:
         raise ValueError("eps must be >= 0, got %r" % eps)
-    _on(x.device, weight=weight, residual=residual)
+    _on(x, "weight", weight, "residual", residual)
     if weight is not None:
         weight = weight.contiguous()
     if _wants_grad(x, weight, residual):
@@ -216,14 +249,14 @@ def quantize_rows(x):
     _tensor(x, "x", _FLOATS)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
         raise ValueError("x must have rows of 1 to %d values, has shape %s" % (MAX_WIDTH, tuple(x.shape)))
-    _on(x.device)
+    _on(x)
     if _wants_grad(x):
         raise ValueError("the 8-bit output has no gradient: call it under torch.no_grad() or on detached tensors")
     xr, ldx = _as_rows(x)
     n, d = xr.shape
-    y = torch.empty((n, d), dtype=torch.float8_e4m3fn, device=x.device)
-    scales = torch.empty((n,), dtype=torch.float32, device=x.device)
-    _call("fg_quantize_rows", x.device, xr.data_ptr(), ldx, y.data_ptr(), scales.data_ptr(), n, d, _TYPES[x.dtype])
+    y = torch.empty(n, d, dtype=torch.float8_e4m3fn, device=x.device)
+    scales = torch.empty(n, dtype=torch.float32, device=x.device)
+    _call("fg_quantize_rows", x.get_device(), xr.data_ptr(), ldx, y.data_ptr(), scales.data_ptr(), n, d, _TYPES[x.dtype])
     return QuantizedRows(y.view(x.shape), scales.view(x.shape[:-1]))
 
 
@@ -243,50 +276,60 @@ def group_rows(keys, num_groups):
         raise ValueError("num_groups must be 1 to %d, got %d" % (MAX_GROUPS, num_groups))
     if keys.numel() >= 2 ** 31:
         raise ValueError("%d entries: fewer than 2^31 are wanted" % keys.numel())
-    _on(keys.device)
+    _on(keys)
     if keys.dtype == torch.int64:
         keys = keys.clamp(-1, num_groups).int()
     return _group(keys.contiguous(), num_groups)
 
 
+def _lists(n, k, num_groups, device):
+    """Unfilled lists, and the workspace that filling them takes."""
+    m = n * k
+    g = object.__new__(RowGroups)  # by construction what RowGroups() checks
+    g.offsets = torch.empty(num_groups + 1, dtype=torch.int32, device=device)
+    g.order = torch.empty(m, dtype=torch.int32, device=device)
+    g.position = torch.empty(n, k, dtype=torch.int32, device=device)
+    size = _size("fg_group_rows_workspace", m, num_groups)
+    return g, (torch.empty(size, dtype=torch.uint8, device=device) if size else None), size
+
+
 def _group(keys, num_groups):
-    m, device = keys.numel(), keys.device
-    offsets = torch.empty((num_groups + 1,), dtype=torch.int32, device=device)
-    order = torch.empty((m,), dtype=torch.int32, device=device)
-    position = torch.empty_like(keys)
-    size = dev.lib().fg_group_rows_workspace(m, num_groups)
-    work = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
-    _call("fg_group_rows", device, keys.data_ptr(), m, num_groups, offsets.data_ptr(), order.data_ptr(), position.data_ptr(), _ptr(work), size)
-    return RowGroups(offsets, order, position)
+    g, work, size = _lists(keys.shape[0], keys.shape[1], num_groups, keys.device)
+    _call("fg_group_rows", keys.get_device(), keys.data_ptr(), g.num_entries, num_groups, g.offsets.data_ptr(), g.order.data_ptr(), g.position.data_ptr(),
+          _ptr(work), size)
+    return g
 
 
 def _choose(logits, k, scoring, normalize):
     x, ld = _as_rows(logits)
     n, experts = x.shape
-    weights = torch.empty((n, k), dtype=torch.float32, device=x.device)
-    chosen = torch.empty((n, k), dtype=torch.int32, device=x.device)
-    _call("fg_route", x.device, x.data_ptr(), ld, weights.data_ptr(), chosen.data_ptr(), n, experts, k, _TYPES[x.dtype], scoring, normalize)
-    return weights, chosen
+    device = x.device
+    weights = torch.empty(n, k, dtype=torch.float32, device=device)
+    chosen = torch.empty(n, k, dtype=torch.int32, device=device)
+    g, work, size = _lists(n, k, experts, device)
+    _call("fg_route", x.get_device(), x.data_ptr(), ld, weights.data_ptr(), chosen.data_ptr(), g.offsets.data_ptr(), g.order.data_ptr(),
+          g.position.data_ptr(), n, experts, k, _TYPES[x.dtype], scoring, normalize, _ptr(work), size)
+    return weights, chosen, g
 
 
 class _Route(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, k, scoring, normalize):
-        weights, chosen = _choose(logits, k, scoring, normalize)
-        ctx.mark_non_differentiable(chosen)
+        weights, chosen, g = _choose(logits, k, scoring, normalize)
+        ctx.mark_non_differentiable(chosen, g.offsets, g.order, g.position)
         ctx.save_for_backward(logits, weights, chosen)
         ctx.args = (k, scoring, normalize)
-        return weights, chosen
+        return weights, chosen, g.offsets, g.order, g.position
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dweights, _):
+    def backward(ctx, dweights, *_):
         logits, weights, chosen = ctx.saved_tensors
         x, ld = _as_rows(logits)
         dweights = dweights.contiguous()
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         k, scoring, normalize = ctx.args
-        _call("fg_route_backward", x.device, x.data_ptr(), ld, weights.data_ptr(), chosen.data_ptr(), dweights.data_ptr(), dx.data_ptr(),
+        _call("fg_route_backward", x.get_device(), x.data_ptr(), ld, weights.data_ptr(), chosen.data_ptr(), dweights.data_ptr(), dx.data_ptr(),
               x.shape[0], x.shape[1], k, _TYPES[x.dtype], scoring, normalize)
         return dx, None, None, None
 
@@ -307,22 +350,24 @@ def route(logits, k, scoring="softmax", normalize=True):
         raise ValueError("k must be 1 to %d, got %d" % (min(experts, MAX_CHOICES), k))
     if n * k >= 2 ** 31:
         raise ValueError("%d entries: fewer than 2^31 are wanted" % (n * k))
-    _on(logits.device)
+    _on(logits)
     args = (k, _SCORING[scoring], 1 if normalize else 0)
-    weights, chosen = _Route.apply(logits, *args) if _wants_grad(logits) else _choose(logits, *args)
-    return Routing(weights, chosen, _group(chosen, experts))
+    if _wants_grad(logits):
+        weights, chosen, *lists = _Route.apply(logits, *args)
+        return Routing(weights, chosen, RowGroups(*lists))
+    return Routing(*_choose(logits, *args))
 
 
 # ---- products ----
 
 def _product(x, ldx, x_scales, w, strides, w_scales, groups, gather, x_rows, inner, outer, out_dtype):
-    device, kind = x.device, _TYPES[x.dtype]
-    y = torch.empty((groups.num_entries, outer), dtype=out_dtype, device=device)
-    order, m = (groups.order.data_ptr() if gather else None), groups.num_entries
-    size = dev.lib().fg_grouped_matmul_workspace(x.data_ptr(), ldx, w.data_ptr(), *strides, order, m, groups.num_groups, inner, outer, kind)
-    work = torch.empty((size,), dtype=torch.uint8, device=device) if size else None
-    _call("fg_grouped_matmul", device, x.data_ptr(), ldx, _ptr(x_scales), w.data_ptr(), *strides, _ptr(w_scales), groups.offsets.data_ptr(),
-          order, groups.choices, x_rows, y.data_ptr(), m, groups.num_groups, inner, outer, kind, _TYPES[out_dtype], _ptr(work), size)
+    device, kind, m, g = x.device, _TYPES[x.dtype], groups.order.numel(), groups.offsets.numel() - 1
+    y = torch.empty(m, outer, dtype=out_dtype, device=device)
+    xp, wp, order = x.data_ptr(), w.data_ptr(), groups.order.data_ptr() if gather else None
+    size = _size("fg_grouped_matmul_workspace", xp, ldx, wp, *strides, order, m, g, inner, outer, kind)
+    work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+    _call("fg_grouped_matmul", x.get_device(), xp, ldx, _ptr(x_scales), wp, *strides, _ptr(w_scales), groups.offsets.data_ptr(), order,
+          groups.position.shape[1], x_rows, y.data_ptr(), m, g, inner, outer, kind, _TYPES[out_dtype], _ptr(work), size)
     return y
 
 
@@ -352,9 +397,9 @@ class _Product(torch.autograd.Function):
             kind = _TYPES[x.dtype]
             dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
             order, m = (groups.order.data_ptr() if gather else None), groups.num_entries
-            size = dev.lib().fg_grouped_matmul_wgrad_workspace(xr.data_ptr(), ldx, dyr.data_ptr(), ldy, order, m, groups.num_groups, inner, outer, kind)
-            work = torch.empty((size,), dtype=torch.uint8, device=w.device) if size else None
-            _call("fg_grouped_matmul_wgrad", x.device, xr.data_ptr(), ldx, dyr.data_ptr(), ldy, groups.offsets.data_ptr(),
+            size = _size("fg_grouped_matmul_wgrad_workspace", xr.data_ptr(), ldx, dyr.data_ptr(), ldy, order, m, groups.num_groups, inner, outer, kind)
+            work = torch.empty(size, dtype=torch.uint8, device=w.device) if size else None
+            _call("fg_grouped_matmul_wgrad", x.get_device(), xr.data_ptr(), ldx, dyr.data_ptr(), ldy, groups.offsets.data_ptr(),
                   order, groups.choices, x.shape[0], dw.data_ptr(), m, groups.num_groups, inner, outer, kind, _ptr(work), size)
         return dx, dw, None, None
 
@@ -399,7 +444,7 @@ def grouped_matmul(x, weight, groups, gather=False, out_dtype=None):
     want = groups.num_rows if gather else groups.num_entries
     if x.shape[0] != want:
         raise ValueError("x has %d rows, the groups %d%s" % (x.shape[0], want, "" if gather else " slots"))
-    _on(x.device, weight=weight, groups=groups.offsets, scales=x_scales, weight_scales=w_scales)
+    _on(x, "weight", weight, "groups", groups.offsets, "scales", x_scales, "weight_scales", w_scales)
     gather = bool(gather)
     if not eight and _wants_grad(x, weight):
         return _Product.apply(x, weight, groups, gather)
@@ -414,8 +459,8 @@ def grouped_matmul(x, weight, groups, gather=False, out_dtype=None):
 def _combine(y, groups, weights):
     yr, ldy = _as_rows(y)
     n, k, d = groups.num_rows, groups.choices, y.shape[1]
-    out = torch.empty((n, d), dtype=y.dtype, device=y.device)
-    _call("fg_combine_rows", y.device, yr.data_ptr(), ldy, _ptr(weights), groups.position.data_ptr(), out.data_ptr(), n, k, d, _TYPES[y.dtype])
+    out = torch.empty(n, d, dtype=y.dtype, device=y.device)
+    _call("fg_combine_rows", y.get_device(), yr.data_ptr(), ldy, _ptr(weights), groups.position.data_ptr(), out.data_ptr(), n, k, d, _TYPES[y.dtype])
     return out
 
 
@@ -434,9 +479,9 @@ class _Combine(torch.autograd.Function):
         yr, ldy = _as_rows(y)
         gr, ldd = _as_rows(dout)
         n, k, d = groups.num_rows, groups.choices, y.shape[1]
-        dy = torch.empty((n * k, d), dtype=y.dtype, device=y.device) if ctx.needs_input_grad[0] else None
-        dw = torch.empty((n, k), dtype=torch.float32, device=y.device) if weights is not None and ctx.needs_input_grad[2] else None
-        _call("fg_combine_rows_backward", y.device, yr.data_ptr(), ldy, _ptr(weights), groups.position.data_ptr(), groups.offsets.data_ptr(),
+        dy = torch.empty(n * k, d, dtype=y.dtype, device=y.device) if ctx.needs_input_grad[0] else None
+        dw = torch.empty(n, k, dtype=torch.float32, device=y.device) if weights is not None and ctx.needs_input_grad[2] else None
+        _call("fg_combine_rows_backward", y.get_device(), yr.data_ptr(), ldy, _ptr(weights), groups.position.data_ptr(), groups.offsets.data_ptr(),
               groups.num_groups, gr.data_ptr(), ldd, _ptr(dy), _ptr(dw), n, k, d, _TYPES[y.dtype])
         return dy, None, dw
 
@@ -454,7 +499,7 @@ def combine_rows(y, groups, weights=None):
         _tensor(weights, "weights", (torch.float32,), 2)
         if weights.shape != groups.position.shape:
             raise ValueError("weights have shape %s, the choices %s" % (tuple(weights.shape), tuple(groups.position.shape)))
-    _on(y.device, groups=groups.offsets, weights=weights)
+    _on(y, "groups", groups.offsets, "weights", weights)
     if weights is not None:
         weights = weights.contiguous()
     if _wants_grad(y, weights):

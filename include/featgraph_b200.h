@@ -363,11 +363,14 @@ int fg_rms_norm_backward(const void* d_h, int64_t ldh, const void* d_weight, con
 /* Choice of the k largest of `experts` logits a row, in descending order, ties to the lowest index; -inf and NaN are
  * never chosen, and where fewer than k are left the remaining choices are -1 with weight 0.  Weights: softmax over
  * the row (without the closed ones) or sigmoid; normalize != 0: divided by the sum over the chosen.
- * experts <= 1024, k <= 32.  The gradient is dense ([n, experts], of the logits' type). */
+ * experts <= 1024, k <= 32.  The same call builds the lists of the chosen experts, as fg_group_rows would from
+ * d_experts (workspace: fg_group_rows_workspace(n * k, experts)); d_offsets NULL leaves them out.  The gradient is dense
+ * ([n, experts], of the logits' type). */
 #define FG_SCORE_SOFTMAX 0
 #define FG_SCORE_SIGMOID 1
-int fg_route(const void* d_logits, int64_t ld, float* d_weights, int32_t* d_experts, int64_t n, int32_t experts, int32_t k,
-             int32_t type, int32_t scoring, int32_t normalize, void* stream);
+int fg_route(const void* d_logits, int64_t ld, float* d_weights, int32_t* d_experts, int32_t* d_offsets, int32_t* d_order,
+             int32_t* d_position, int64_t n, int32_t experts, int32_t k, int32_t type, int32_t scoring, int32_t normalize,
+             void* d_workspace, int64_t workspace_bytes, void* stream);
 int fg_route_backward(const void* d_logits, int64_t ld, const float* d_weights, const int32_t* d_experts, const float* d_dweights,
                       void* d_dlogits, int64_t n, int32_t experts, int32_t k, int32_t type, int32_t scoring, int32_t normalize,
                       void* stream);

@@ -91,8 +91,10 @@ def test_c_entries_report_bad_arguments():
     refused("fg_rms_norm", 1, 0, None, 0, None, None, 1, None, 4, 8, 1e-6, 0, 0, 1, None, text=b"rows' type")
     refused("fg_quantize_rows", None, 0, 1, 1, 4, 8, 0, None, text=b"NULL")
     refused("fg_rms_norm_backward", 1, 0, None, 1, 0, None, 0, 1, None, None, 0, 4, 8, 1e-6, 0, 0, None, text=b"blocks")
-    refused("fg_route", 1, 0, 1, 1, 4, 8, 9, 0, 0, 0, None, text=b"bad sizes")
-    refused("fg_route", 1, 0, 1, 1, 4, 8, 2, 0, 5, 0, None, text=b"scoring")
+    refused("fg_route", 1, 0, 1, 1, None, None, None, 4, 8, 9, 0, 0, 0, None, 0, None, text=b"bad sizes")
+    refused("fg_route", 1, 0, 1, 1, None, None, None, 4, 8, 2, 0, 5, 0, None, 0, None, text=b"scoring")
+    refused("fg_route", 1, 0, 1, 1, 1, 1, 1, 1 << 20, 8, 2, 0, 0, 0, None, 0, None, text=b"workspace")
+    refused("fg_route", 1, 0, 1, 1, 1, None, 1, 4, 8, 2, 0, 0, 0, None, 0, None, text=b"NULL")
     refused("fg_route_backward", 1, 0, 1, 1, None, 1, 4, 8, 2, 0, 0, 0, None, text=b"NULL")
     refused("fg_group_rows", 1, 4, 1025, 1, 1, 1, None, 0, None, text=b"bad sizes")
     refused("fg_group_rows", 1, 1 << 20, 8, 1, 1, 1, None, 0, None, text=b"workspace")
