@@ -417,7 +417,15 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
     __syncthreads();
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (int64_t)gridDim.x * 256) {
         float s = partial[(int64_t)first * cells + i];
-        for (int q = 1; q < count; ++q) s = __fadd_rn(s, partial[(int64_t)(first + q) * cells + i]);
+        int q = 1;
+        for (; q + 8 <= count; q += 8) {  // eight loads in flight, added in order
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = partial[(int64_t)(first + q + j) * cells + i];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) s = __fadd_rn(s, v[j]);
+        }
+        for (; q < count; ++q) s = __fadd_rn(s, partial[(int64_t)(first + q) * cells + i]);
         dw[(int64_t)g * cells + i] = from_f32<T>(s);
     }
 }
@@ -754,7 +762,7 @@ int fg_grouped_matmul_wgrad(const void* d_x, int64_t ldx, const void* d_dy, int6
     a.split = (int32_t)split, a.units = (int32_t)units;
     if (int rc = launch<false, true>(bn, a, map_dy, map_x, units * rows_tiles * ((inner + bn - 1) / bn), s)) return rc;
     if (split) {
-        const dim3 grid((unsigned)((cells + 1023) / 1024 < 4096 ? (cells + 1023) / 1024 : 4096), (unsigned)groups);
+        const dim3 grid((unsigned)((cells + 255) / 256 < 4096 ? (cells + 255) / 256 : 4096), (unsigned)groups);
         if (type == FG_F32) join_kernel<float><<<grid, 256, 0, s>>>(sums, d_offsets, groups, num_rows, (int)split, a.units, cells, static_cast<float*>(d_dw));
         else if (type == FG_F16) join_kernel<__half><<<grid, 256, 0, s>>>(sums, d_offsets, groups, num_rows, (int)split, a.units, cells, static_cast<__half*>(d_dw));
         else join_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(sums, d_offsets, groups, num_rows, (int)split, a.units, cells, static_cast<__nv_bfloat16*>(d_dw));

@@ -45,60 +45,87 @@ struct RouteArgs {
     int32_t* chosen;
 };
 
-// A warp owns a row; lane l holds experts l, l + 32, ...  Each of the k rounds takes the largest remaining key (one
-// warp-wide maximum) and the lowest index that has it (one warp-wide minimum), so ties go to the lowest index; lane j
-// keeps the j-th choice.  Bound: the n * E logits are read once (65,536 x 128: 33.6 MB, 5 us), but k rounds of two
-// warp-wide reductions a row are what the time goes to.
+// A warp owns a row; lane l holds experts l, l + 32, ...  Each of the k rounds is one warp-wide maximum of the lanes'
+// largest keys and a vote; where several lanes hold it (equal logits), a warp-wide minimum of the indices breaks
+// the tie, so it goes to the lowest.  The winner moves to its next largest: up to 4 keys a lane are sorted at the start
+// (adjacent swaps of strictly smaller ones, so equal keys stay in order), more are searched again.  Lane j keeps the
+// j-th choice.  Bound: instructions, some 40 a row and round; the n * E logits are read once (65,536 x 128: 33.6 MB, 5 us).
 template <typename T, int NE>
 __device__ __forceinline__ void route_row(const RouteArgs& a, int64_t row) {
+    constexpr bool kSorted = NE <= 4;
     const int lane = threadIdx.x & 31;
     const T* x = static_cast<const T*>(a.logits) + row * a.ld;
-    uint32_t key[NE];
+    uint32_t key[NE], index[NE];
 #pragma unroll
     for (int i = 0; i < NE; ++i) {
         const int e = i * 32 + lane;
         key[i] = e < a.experts ? order_key(to_f32<T>(x[e])) : 0u;
+        index[i] = e;
+    }
+    uint32_t best = key[0], slot = 0;
+    auto search = [&]() {  // the lane's largest key, and which of its NE it is (the lowest)
+        best = key[0], slot = 0;
+#pragma unroll
+        for (int i = 1; i < NE; ++i)
+            if (key[i] > best) best = key[i], slot = i;
+    };
+    if (kSorted) {
+#pragma unroll
+        for (int pass = 0; pass < NE; ++pass)
+#pragma unroll
+            for (int i = pass & 1; i + 1 < NE; i += 2)
+                if (key[i + 1] > key[i]) {
+                    const uint32_t k0 = key[i], i0 = index[i];
+                    key[i] = key[i + 1], index[i] = index[i + 1];
+                    key[i + 1] = k0, index[i + 1] = i0;
+                }
+        best = key[0];
+    } else {
+        search();
     }
     float all = 0.0f, top = 0.0f;
-    if (!a.sigmoid) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < NE; ++i) m = max(m, key[i]);
-        m = __reduce_max_sync(0xffffffffu, m);
+    if (!a.sigmoid && !a.normalize) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, best);
         top = m ? key_value(m) : 0.0f;
-        if (!a.normalize) {
-#pragma unroll
-            for (int i = 0; i < NE; ++i)
-                if (key[i]) all = __fadd_rn(all, expf(__fsub_rn(key_value(key[i]), top)));
-            all = fg::warp_sum(all);
-        }
-    }
-    int mine = -1;
-    float score = 0.0f;
-    for (int j = 0; j < a.k; ++j) {
-        uint32_t m = 0;
-#pragma unroll
-        for (int i = 0; i < NE; ++i) m = max(m, key[i]);
-        m = __reduce_max_sync(0xffffffffu, m);
-        if (m == 0) break;
-        uint32_t at = 0xffffffffu;
-#pragma unroll
-        for (int i = NE - 1; i >= 0; --i)
-            if (key[i] == m) at = i * 32 + lane;
-        at = __reduce_min_sync(0xffffffffu, at);
 #pragma unroll
         for (int i = 0; i < NE; ++i)
-            if (at == (uint32_t)(i * 32 + lane)) key[i] = 0;
-        if (lane == j) {
-            mine = (int)at;
-            score = a.sigmoid ? sigmoid(key_value(m)) : expf(__fsub_rn(key_value(m), top));
+            if (key[i]) all = __fadd_rn(all, expf(__fsub_rn(key_value(key[i]), top)));
+        all = fg::warp_sum(all);
+    }
+    uint32_t mine = 0, at_mine = 0;
+    for (int j = 0; j < a.k; ++j) {
+        const uint32_t m = __reduce_max_sync(0xffffffffu, best);
+        if (m == 0) break;
+        const uint32_t holders = __ballot_sync(0xffffffffu, best == m);
+        uint32_t at = kSorted ? index[0] : slot * 32 + lane;
+        if (holders & (holders - 1)) at = __reduce_min_sync(0xffffffffu, best == m ? at : 0xffffffffu);
+        else at = __shfl_sync(0xffffffffu, at, __ffs(holders) - 1);
+        if (lane == j) mine = m, at_mine = at;
+        if ((at & 31) == lane) {
+            if (kSorted) {
+#pragma unroll
+                for (int i = 0; i + 1 < NE; ++i) key[i] = key[i + 1], index[i] = index[i + 1];
+                key[NE - 1] = 0;
+                best = key[0];
+            } else {
+#pragma unroll
+                for (int i = 0; i < NE; ++i)
+                    if (i == (int)(at >> 5)) key[i] = 0;
+                search();
+            }
         }
     }
+    float score = 0.0f;
+    if (!a.sigmoid && a.normalize) {
+        const uint32_t m = __shfl_sync(0xffffffffu, mine, 0);
+        top = m ? key_value(m) : 0.0f;
+    }
+    if (mine) score = a.sigmoid ? sigmoid(key_value(mine)) : expf(__fsub_rn(key_value(mine), top));
     if (a.normalize) all = fg::warp_sum(score);
     if (a.normalize || !a.sigmoid) score = all > 0.0f || all != all ? __fdiv_rn(score, all) : 0.0f;
     if (lane < a.k) {
         a.weights[row * a.k + lane] = score;
-        a.chosen[row * a.k + lane] = mine;
+        a.chosen[row * a.k + lane] = mine ? (int)at_mine : -1;
     }
 }
 
@@ -121,7 +148,8 @@ struct RouteGradArgs {
 // softmax, normalised:   dx_i = w_i (g_i - sum g w) for the chosen, 0 elsewhere (the other logits cancel out)
 // softmax over all:      dx_i = p_i ([i chosen] g_i - sum g w)
 // sigmoid, normalised:   dx_i = s_i (1 - s_i) (g_i - sum g w) / sum s;   not normalised: dx_i = s_i (1 - s_i) g_i
-// A warp owns a row and writes all of it, zeros first; lane j holds choice j.
+// A warp owns a row: it writes what the row gets without the choice (zeros, or -p sum g w), then lane j writes choice j's
+// value over it - for a chosen logit of the softmax over all, p is the weight itself.  Bound: the dense rows' bytes.
 template <typename T, int NE>
 __global__ void __launch_bounds__(256) route_grad_kernel(const RouteGradArgs a) {
     const int lane = threadIdx.x & 31;
@@ -139,26 +167,11 @@ __global__ void __launch_bounds__(256) route_grad_kernel(const RouteGradArgs a) 
         if (mine < 0) g = 0.0f;
     }
     const float dot = fg::warp_sum(__fmul_rn(g, w));
-    float value = 0.0f;  // what lane j adds to its expert's gradient
-    float out[NE];
+    if (a.sigmoid || a.normalize) {
 #pragma unroll
-    for (int i = 0; i < NE; ++i) out[i] = 0.0f;
-    if (a.sigmoid) {
-        float s = 0.0f, other = 0.0f;
-        if (mine >= 0) {
-            const float v = to_f32<T>(x[mine]);
-            s = sigmoid(v);
-            other = sigmoid(-v);
-        }
-        value = __fmul_rn(__fmul_rn(s, other), g);
-        if (a.normalize) {
-            const float total = fg::warp_sum(s);
-            value = total > 0.0f ? __fdiv_rn(__fmul_rn(__fmul_rn(s, other), __fsub_rn(g, dot)), total) : 0.0f;
-        }
-    } else if (a.normalize) {
-        value = __fmul_rn(w, __fsub_rn(g, dot));
+        for (int i = 0; i < NE; ++i)
+            if (i * 32 + lane < a.experts) dx[i * 32 + lane] = from_f32<T>(0.0f);
     } else {
-        value = __fmul_rn(w, g);
         uint32_t key[NE], m = 0;
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
@@ -168,35 +181,41 @@ __global__ void __launch_bounds__(256) route_grad_kernel(const RouteGradArgs a) 
         }
         m = __reduce_max_sync(0xffffffffu, m);
         const float top = m ? key_value(m) : 0.0f;
-        float all = 0.0f;
+        float all = 0.0f, p[NE];
 #pragma unroll
         for (int i = 0; i < NE; ++i) {
-            out[i] = key[i] ? expf(__fsub_rn(key_value(key[i]), top)) : 0.0f;
-            all = __fadd_rn(all, out[i]);
+            p[i] = key[i] ? expf(__fsub_rn(key_value(key[i]), top)) : 0.0f;
+            all = __fadd_rn(all, p[i]);
         }
         all = fg::warp_sum(all);
 #pragma unroll
-        for (int i = 0; i < NE; ++i) out[i] = m ? -__fmul_rn(__fdiv_rn(out[i], all), dot) : 0.0f;
-    }
-    for (int j = 0; j < a.k; ++j) {
-        const int e = __shfl_sync(0xffffffffu, mine, j);
-        const float v = __shfl_sync(0xffffffffu, value, j);
-        if (e < 0) continue;
-#pragma unroll
         for (int i = 0; i < NE; ++i)
-            if (e == i * 32 + lane) out[i] = __fadd_rn(out[i], v);
+            if (i * 32 + lane < a.experts) dx[i * 32 + lane] = from_f32<T>(m ? -__fmul_rn(__fdiv_rn(p[i], all), dot) : 0.0f);
     }
-#pragma unroll
-    for (int i = 0; i < NE; ++i) {
-        const int e = i * 32 + lane;
-        if (e < a.experts) dx[e] = from_f32<T>(out[i]);
+    __syncwarp();  // the stores above come before those below
+    float s = 0.0f, slope = 0.0f;
+    if (a.sigmoid) {
+        if (mine >= 0) {
+            const float v = to_f32<T>(x[mine]);
+            s = sigmoid(v);
+            slope = __fmul_rn(s, sigmoid(-v));
+        }
+        if (a.normalize) {
+            const float total = fg::warp_sum(s);
+            slope = total > 0.0f ? __fdiv_rn(__fmul_rn(slope, __fsub_rn(g, dot)), total) : 0.0f;
+        } else {
+            slope = __fmul_rn(slope, g);
+        }
+    } else {
+        slope = __fmul_rn(w, __fsub_rn(g, dot));
     }
+    if (mine >= 0) dx[mine] = from_f32<T>(slope);
 }
 
 // ---- lists ----
 
 // Entries are cut into chunks, a block each; in a chunk every warp owns a run of consecutive entries.  Pass 1 counts
-// keys per chunk, pass 2 turns the counts into first slots (group-major, chunks in order), pass 3 counts per warp,
+// keys per chunk, pass 2 sums a group's counts over the chunks before (a warp a group), pass 3 scans the totals, counts per warp,
 // and walks each run 32 entries at a time: an entry's rank among its warp's equal keys is the number of lower lanes
 // with the same key (match_any), so the order is stable.  Key `groups` stands for "in no group".  When one chunk
 // holds all entries, pass 3 alone does everything.
@@ -204,7 +223,7 @@ struct GroupArgs {
     const int32_t* keys;
     int64_t m;
     int32_t groups, chunk, chunks;
-    int32_t *counts;  // [groups + 1][chunks]: counts, then first slots
+    int32_t *counts;  // [groups + 1][chunks]: counts, then the entries of the group in earlier chunks; then a total each
     int32_t *offsets, *order, *position;
 };
 
@@ -223,7 +242,7 @@ __global__ void __launch_bounds__(256) group_count_kernel(const GroupArgs a) {
     for (int g = threadIdx.x; g <= a.groups; g += blockDim.x) a.counts[(int64_t)g * a.chunks + blockIdx.x] = hist[g];
 }
 
-// Exclusive scan of v over the block (blockDim.x = 1024); total by reference.
+// Exclusive scan of v over the block; total by reference.
 __device__ int block_scan(int v, int& total) {
     __shared__ int sums[32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
@@ -250,28 +269,38 @@ __device__ int block_scan(int v, int& total) {
     return s - v + (warp ? sums[warp - 1] : 0);
 }
 
-__global__ void __launch_bounds__(1024) group_scan_kernel(const GroupArgs a) {
-    const int64_t cells = (int64_t)(a.groups + 1) * a.chunks;
-    int carry = 0;
-    for (int64_t base = 0; base < cells; base += 1024) {
-        const int64_t i = base + threadIdx.x;
-        int total;
-        const int first = carry + block_scan(i < cells ? a.counts[i] : 0, total);
-        if (i < cells) {
-            a.counts[i] = first;
-            if (i % a.chunks == 0) a.offsets[i / a.chunks] = first;  // group `groups` starts where the last group ends
-        }
-        carry += total;
+__global__ void __launch_bounds__(128) group_scan_kernel(const GroupArgs a) {
+    const int lane = threadIdx.x & 31, bins = a.groups + 1, each = (a.chunks + 31) / 32, g = blockIdx.x * 4 + (threadIdx.x >> 5);
+    if (g >= bins) return;
+    int32_t* row = a.counts + (int64_t)g * a.chunks;
+    const int from = min(lane * each, a.chunks), to = min(from + each, a.chunks);
+    int own = 0;
+#pragma unroll 8
+    for (int c = from; c < to; ++c) own += row[c];
+    int sum = own;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += v;
+    }
+    if (lane == 31) a.counts[(int64_t)bins * a.chunks + g] = sum;
+    int before = sum - own;
+#pragma unroll 8
+    for (int c = from; c < to; ++c) {
+        const int n = row[c];
+        row[c] = before;
+        before += n;
     }
 }
 
 template <bool SINGLE>
 __device__ __forceinline__ void place_entries(const GroupArgs& a, int* cell) {  // cell: [warps][groups + 1]
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, bins = a.groups + 1;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, bins = a.groups + 1, threads = blockDim.x >> 5;
+    const int64_t begin = (int64_t)blockIdx.x * a.chunk, end = min(begin + a.chunk, a.m);
+    const int run = ((a.chunk + threads - 1) / threads + 31) / 32 * 32;
+    const int warps = (a.chunk + run - 1) / run;  // that have entries
     for (int i = threadIdx.x; i < warps * bins; i += blockDim.x) cell[i] = 0;
     __syncthreads();
-    const int64_t begin = (int64_t)blockIdx.x * a.chunk, end = min(begin + a.chunk, a.m);
-    const int run = ((a.chunk + warps - 1) / warps + 31) / 32 * 32;
     const int64_t first = min(begin + (int64_t)warp * run, end), last = min(first + run, end);
     int* mine = cell + warp * bins;
     for (int64_t e = first + lane; e < last; e += 32) atomicAdd(&mine[key_of(a, e)], 1);
@@ -279,18 +308,14 @@ __device__ __forceinline__ void place_entries(const GroupArgs& a, int* cell) {  
     int carry = 0;
     for (int base = 0; base < bins; base += blockDim.x) {
         const int g = base + threadIdx.x;
-        int sum = 0;
-        if (g < bins)
+        int sum = 0, total;  // the group's entries: counted here, or in the passes before
+        if (SINGLE && g < bins)
             for (int w = 0; w < warps; ++w) sum += cell[w * bins + g];
-        int start = 0;
-        if (SINGLE) {
-            int total;
-            start = carry + block_scan(sum, total);
-            carry += total;
-            if (g < bins) a.offsets[g] = start;
-        } else if (g < bins) {
-            start = a.counts[(int64_t)g * a.chunks + blockIdx.x];
-        }
+        if (!SINGLE && g < bins) sum = a.counts[(int64_t)bins * a.chunks + g];
+        int start = carry + block_scan(sum, total);
+        carry += total;
+        if (g < bins && blockIdx.x == 0) a.offsets[g] = start;  // group `groups` starts where the last group ends
+        if (!SINGLE && g < bins) start += a.counts[(int64_t)g * a.chunks + blockIdx.x];
         if (g < bins)
             for (int w = 0; w < warps; ++w) {
                 const int c = cell[w * bins + g];
@@ -324,7 +349,7 @@ __global__ void __launch_bounds__(1024) group_place_kernel(const GroupArgs a) {
 
 // Choice and lists of a few rows in one launch: one block chooses for all rows, a warp a row, and then lists them.
 template <typename T, int NE>
-__global__ void __launch_bounds__(512) route_lists_kernel(const RouteArgs a, const GroupArgs g) {
+__global__ void __launch_bounds__(1024) route_lists_kernel(const RouteArgs a, const GroupArgs g) {
     extern __shared__ int cell[];
     for (int64_t row = threadIdx.x >> 5; row < a.n; row += blockDim.x >> 5) route_row<T, NE>(a, row);
     __syncthreads();  // the choices are in global memory, written by this block
@@ -359,9 +384,9 @@ struct LaunchRouteLists {
     cudaStream_t s;
     template <typename T, int NE>
     void operator()() const {
-        const int warps = a.n <= 4 ? 4 : a.n <= 8 ? 8 : 16;
+        const int warps = a.n <= 4 ? 4 : a.n <= 8 ? 8 : a.n <= 16 ? 16 : 32;
         const size_t smem = (size_t)warps * (g.groups + 1) * 4;
-        if (smem > 48 * 1024) (void)cudaFuncSetAttribute(route_lists_kernel<T, NE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 80 * 1024);
+        if (smem > 40 * 1024) (void)cudaFuncSetAttribute(route_lists_kernel<T, NE>, cudaFuncAttributeMaxDynamicSharedMemorySize, 140 * 1024);
         route_lists_kernel<T, NE><<<1, warps * 32, smem, s>>>(a, g);
     }
 };
@@ -490,7 +515,7 @@ int check_route(int64_t n, int32_t experts, int32_t k, int32_t type, int32_t sco
     return FG_OK;
 }
 
-// Rows that one block chooses and lists by itself: a second launch costs about 3 us, a warp some 2 us a row.
+// Rows that one block chooses and lists by itself, a warp each: one launch instead of two.
 constexpr int64_t kOneBlockRows = 32;
 
 // 8192 entries or fewer are one chunk; above that chunks of at least 2048, at most 1024 of them.
@@ -523,7 +548,7 @@ int fg_route_backward(const void* d_logits, int64_t ld, const float* d_weights, 
 int64_t fg_group_rows_workspace(int64_t num_entries, int32_t num_groups) {
     if (num_entries <= 0 || num_groups < 1) return 0;
     const int64_t chunk = chunk_size(num_entries), chunks = (num_entries + chunk - 1) / chunk;
-    return chunks <= 1 ? 0 : chunks * ((int64_t)num_groups + 1) * 4;
+    return chunks <= 1 ? 0 : (chunks + 1) * ((int64_t)num_groups + 1) * 4;
 }
 
 int fg_group_rows(const int32_t* d_keys, int64_t num_entries, int32_t num_groups, int32_t* d_offsets, int32_t* d_order,
@@ -546,7 +571,7 @@ int fg_group_rows(const int32_t* d_keys, int64_t num_entries, int32_t num_groups
         GroupArgs one = a;
         one.chunk = (int32_t)num_entries;
         const size_t smem = (size_t)warps * bins * 4;
-        if (smem > 48 * 1024) FG_CUDA_TRY(cudaFuncSetAttribute(group_place_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+        if (smem > 40 * 1024) FG_CUDA_TRY(cudaFuncSetAttribute(group_place_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
         group_place_kernel<true><<<1, warps * 32, smem, s>>>(one);
         FG_CUDA_TRY(cudaGetLastError());
         fg::count_launches(1);
@@ -554,7 +579,7 @@ int fg_group_rows(const int32_t* d_keys, int64_t num_entries, int32_t num_groups
     }
     group_count_kernel<<<(unsigned)chunks, 256, (size_t)bins * 4, s>>>(a);
     FG_CUDA_TRY(cudaGetLastError());
-    group_scan_kernel<<<1, 1024, 0, s>>>(a);
+    group_scan_kernel<<<(unsigned)((bins + 3) / 4), 128, 0, s>>>(a);
     FG_CUDA_TRY(cudaGetLastError());
     group_place_kernel<false><<<(unsigned)chunks, 256, (size_t)8 * bins * 4, s>>>(a);
     FG_CUDA_TRY(cudaGetLastError());

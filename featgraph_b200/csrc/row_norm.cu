@@ -173,37 +173,69 @@ struct NormGradArgs {
     bool weight_f32;
 };
 
+// Two sums over the TPR threads of a row, through one of two buffers in turn, so that a row needs one barrier.
+template <int TPR>
+__device__ __forceinline__ void row_sums(float& x, float& y, float2* buffer) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, o));
+        y = __fadd_rn(y, __shfl_xor_sync(0xffffffffu, y, o));
+    }
+    if (TPR == 32) return;
+    constexpr int kWarps = TPR / 32;
+    const int first = (threadIdx.x / TPR) * kWarps;
+    if ((threadIdx.x & 31) == 0) buffer[threadIdx.x >> 5] = make_float2(x, y);
+    __syncthreads();
+    const float2 v = buffer[first];
+    x = v.x, y = v.y;
+#pragma unroll
+    for (int i = 1; i < kWarps; ++i) {
+        const float2 w = buffer[first + i];
+        x = __fadd_rn(x, w.x), y = __fadd_rn(y, w.y);
+    }
+}
+
+// Where a row is shared by several warps, the next row's values are requested before the current one's sums, so that loads
+// are in flight across the barrier (32768 x 4096 bf16 with dh: 325 -> 253 us).  A row of one warp meets no barrier, and
+// there the registers are worth more as warps (100003 x 331 fp32: 122 us without, 211 us with); rows of 1024 threads
+// have 64 registers a thread and no room.
 template <typename T, int VEC, int TPR, int E>
 __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(const NormGradArgs a) {
     constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR, NV = E / VEC;
-    __shared__ float buffer[2][kThreads / 32];
+    __shared__ float2 buffer[2][kThreads / 32];
     __shared__ float across[kRows > 1 ? kRows * TPR * E : 1];
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
+    const int64_t step = (int64_t)gridDim.x * kRows;
     float acc[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.n; base += (int64_t)gridDim.x * kRows) {
-        const int64_t row = base + sub;
+    struct Row {
+        Pack<T, VEC> h[NV], g[NV], d[NV];
+    };
+    auto request = [&](Row& r, int64_t row) {
         const bool live = row < a.n;
         const T* h = static_cast<const T*>(a.h) + (live ? row : 0) * a.ldh;
         const T* dy = static_cast<const T*>(a.dy) + (live ? row : 0) * a.lddy;
-        Pack<T, VEC> ph[NV], pg[NV], pd[NV];
+        const T* dh = static_cast<const T*>(a.dh) + (live ? row : 0) * a.lddh;
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
             const int i = (c * TPR + t) * VEC;
             if (live && i < a.d) {
-                ph[c] = load_pack<T, VEC>(h + i);
-                pg[c] = load_pack<T, VEC>(dy + i);
+                r.h[c] = load_pack<T, VEC>(h + i);
+                r.g[c] = load_pack<T, VEC>(dy + i);
+                if (a.dh != nullptr) r.d[c] = load_pack<T, VEC>(dh + i);
             }
         }
-        if (a.dh != nullptr) {
-            const T* dh = static_cast<const T*>(a.dh) + (live ? row : 0) * a.lddh;
-#pragma unroll
-            for (int c = 0; c < NV; ++c) {
-                const int i = (c * TPR + t) * VEC;
-                if (live && i < a.d) pd[c] = load_pack<T, VEC>(dh + i);
-            }
-        }
+    };
+    constexpr bool kAhead = VEC > 1 && TPR >= 64 && TPR <= 512;
+    Row now, next;
+    int turn = 0;
+    if (kAhead) request(now, (int64_t)blockIdx.x * kRows + sub);
+    for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.n; base += step, turn ^= 1) {
+        const int64_t row = base + sub;
+        const bool live = row < a.n;
+        if (kAhead) request(next, row + step);
+        else request(now, row);
         float ss = 0.0f, sg = 0.0f;
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
@@ -211,15 +243,14 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(const 
             if (live && i < a.d) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float u = to_f32<T>(ph[c].v[j]);
-                    const float g = __fmul_rn(to_f32<T>(pg[c].v[j]), weight_at(a.weight, a.weight_f32, i + j, T()));
+                    const float u = to_f32<T>(now.h[c].v[j]);
+                    const float g = __fmul_rn(to_f32<T>(now.g[c].v[j]), weight_at(a.weight, a.weight_f32, i + j, T()));
                     ss = __fmaf_rn(u, u, ss);
                     sg = __fmaf_rn(u, g, sg);
                 }
             }
         }
-        ss = row_reduce<TPR, false>(ss, buffer[0]);
-        sg = row_reduce<TPR, false>(sg, buffer[1]);
+        row_sums<TPR>(ss, sg, buffer[turn]);
         const float r = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.d), a.eps));
         const float along = __fmul_rn(__fmul_rn(r, r), __fmul_rn(r, __fdiv_rn(sg, (float)a.d)));
         T* dx = static_cast<T*>(a.dx) + row * a.d;
@@ -230,63 +261,81 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(const 
                 Pack<T, VEC> o;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float u = to_f32<T>(ph[c].v[j]), dyj = to_f32<T>(pg[c].v[j]);
+                    const float u = to_f32<T>(now.h[c].v[j]), dyj = to_f32<T>(now.g[c].v[j]);
                     const float g = __fmul_rn(dyj, weight_at(a.weight, a.weight_f32, i + j, T()));
                     float v = __fmaf_rn(-u, along, __fmul_rn(r, g));
-                    if (a.dh != nullptr) v = __fadd_rn(v, to_f32<T>(pd[c].v[j]));
+                    if (a.dh != nullptr) v = __fadd_rn(v, to_f32<T>(now.d[c].v[j]));
                     o.v[j] = from_f32<T>(v);
                     acc[c * VEC + j] = __fmaf_rn(dyj, __fmul_rn(u, r), acc[c * VEC + j]);
                 }
                 store_pack<T, VEC>(dx + i, o);
             }
         }
+        if (kAhead) now = next;
     }
     if (a.partial == nullptr) return;
     float* out = a.partial + (int64_t)blockIdx.x * a.d;
     if (kRows > 1) {  // the block's row groups hold the same columns: add them in order
+#pragma unroll
         for (int e = 0; e < E; ++e) across[(sub * E + e) * TPR + t] = acc[e];
         __syncthreads();
         if (sub != 0) return;
         for (int s = 1; s < kRows; ++s)
+#pragma unroll
             for (int e = 0; e < E; ++e) acc[e] = __fadd_rn(acc[e], across[(s * E + e) * TPR + t]);
     }
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
         const int i = (c * TPR + t) * VEC;
+#pragma unroll
         for (int j = 0; j < VEC; ++j)
             if (i + j < a.d) out[i + j] = acc[c * VEC + j];
     }
 }
 
-// dw[c] = sum of partial[0 .. rows)[c]: 32 columns a block, 8 row sequences each, joined in order.
+// dw[c] = sum of partial[0 .. rows)[c]: 32 columns a block, 32 row sequences each, joined in order.
 template <typename W>
-__global__ void __launch_bounds__(256) weight_grad_kernel(const float* __restrict__ partial, int rows, int d, W* __restrict__ dw) {
-    __shared__ float part[8][33];
+__global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restrict__ partial, int rows, int d, W* __restrict__ dw) {
+    __shared__ float part[32][33];
     const int lane = threadIdx.x & 31, seq = threadIdx.x >> 5;
     const int c = blockIdx.x * 32 + lane;
     float s = 0.0f;
     if (c < d)
-        for (int r = seq; r < rows; r += 8) s = __fadd_rn(s, partial[(int64_t)r * d + c]);
+#pragma unroll 8
+        for (int r = seq; r < rows; r += 32) s = __fadd_rn(s, partial[(int64_t)r * d + c]);
     part[seq][lane] = s;
     __syncthreads();
     if (seq == 0 && c < d) {
-        for (int q = 1; q < 8; ++q) s = __fadd_rn(s, part[q][lane]);
+#pragma unroll
+        for (int q = 1; q < 32; ++q) s = __fadd_rn(s, part[q][lane]);
         dw[c] = from_f32<W>(s);
     }
 }
 
 constexpr int kMaxWidth = 16384;
 
-// Calls f.template operator()<T, VEC, TPR, E>() with the smallest TPR * E that covers d.
+// Calls f.template operator()<T, VEC, TPR, E>() with the smallest TPR * E that covers d.  Single-value accesses cost an
+// address and a register each, so there a thread holds 8 values rather than 16 (100003 x 331 fp32, backward: 16 values a
+// thread leave 16 warps an SM, 122 us).
 template <typename T, int VEC, typename F>
 void by_width(int d, F&& f) {
-    if (d <= 256) f.template operator()<T, VEC, 32, 8>();
-    else if (d <= 512) f.template operator()<T, VEC, 32, 16>();
-    else if (d <= 1024) f.template operator()<T, VEC, 64, 16>();
-    else if (d <= 2048) f.template operator()<T, VEC, 128, 16>();
-    else if (d <= 4096) f.template operator()<T, VEC, 256, 16>();
-    else if (d <= 8192) f.template operator()<T, VEC, 512, 16>();
-    else f.template operator()<T, VEC, 1024, 16>();
+    if constexpr (VEC == 1) {
+        if (d <= 256) f.template operator()<T, VEC, 32, 8>();
+        else if (d <= 512) f.template operator()<T, VEC, 64, 8>();
+        else if (d <= 1024) f.template operator()<T, VEC, 128, 8>();
+        else if (d <= 2048) f.template operator()<T, VEC, 256, 8>();
+        else if (d <= 4096) f.template operator()<T, VEC, 512, 8>();
+        else if (d <= 8192) f.template operator()<T, VEC, 1024, 8>();
+        else f.template operator()<T, VEC, 1024, 16>();
+    } else {
+        if (d <= 256) f.template operator()<T, VEC, 32, 8>();
+        else if (d <= 512) f.template operator()<T, VEC, 32, 16>();
+        else if (d <= 1024) f.template operator()<T, VEC, 64, 16>();
+        else if (d <= 2048) f.template operator()<T, VEC, 128, 16>();
+        else if (d <= 4096) f.template operator()<T, VEC, 256, 16>();
+        else if (d <= 8192) f.template operator()<T, VEC, 512, 16>();
+        else f.template operator()<T, VEC, 1024, 16>();
+    }
 }
 template <typename F>
 void by_type(int32_t type, bool vec, int d, F&& f) {
@@ -295,6 +344,7 @@ void by_type(int32_t type, bool vec, int d, F&& f) {
     else vec ? by_width<__nv_bfloat16, 8>(d, f) : by_width<__nv_bfloat16, 1>(d, f);
 }
 
+// Rows that a block of the backward pass walks at a time, at most.
 int rows_per_block(int d) { return d <= 512 ? 8 : d <= 1024 ? 4 : d <= 2048 ? 2 : 1; }
 
 // 128-bit accesses need every row to start on a 16-byte boundary.
@@ -402,9 +452,9 @@ int fg_rms_norm_backward(const void* d_h, int64_t ldh, const void* d_weight, con
     fg::count_launches(1);
     if (d_dweight) {
         const unsigned grid = (unsigned)((d + 31) / 32);
-        if (weight_type == FG_F32) weight_grad_kernel<float><<<grid, 256, 0, s>>>(d_partial, (int)blocks, d, static_cast<float*>(d_dweight));
-        else if (weight_type == FG_F16) weight_grad_kernel<__half><<<grid, 256, 0, s>>>(d_partial, (int)blocks, d, static_cast<__half*>(d_dweight));
-        else weight_grad_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(d_partial, (int)blocks, d, static_cast<__nv_bfloat16*>(d_dweight));
+        if (weight_type == FG_F32) weight_grad_kernel<float><<<grid, 1024, 0, s>>>(d_partial, (int)blocks, d, static_cast<float*>(d_dweight));
+        else if (weight_type == FG_F16) weight_grad_kernel<__half><<<grid, 1024, 0, s>>>(d_partial, (int)blocks, d, static_cast<__half*>(d_dweight));
+        else weight_grad_kernel<__nv_bfloat16><<<grid, 1024, 0, s>>>(d_partial, (int)blocks, d, static_cast<__nv_bfloat16*>(d_dweight));
         FG_CUDA_TRY(cudaGetLastError());
         fg::count_launches(1);
     }
