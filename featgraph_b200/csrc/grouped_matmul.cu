@@ -45,19 +45,24 @@ struct MmaArgs {
     int64_t m, x_rows;    // slots; rows of x
     int32_t choices, groups, inner, outer;  // inner: the summed axis (y) or x's width (dW); outer: width of y
     int32_t type, out_type, format;
-    int32_t first_pair;   // 5: one product; 0: six products of parts
     bool b_mn, shared_weight;
     int32_t split;        // dW: rows of one partial sum (0: a group's rows in one)
     int32_t units;        // dW: partial sums that there is room for
 };
 
-// Parts multiplied in each of the six products, smallest first.
-__device__ __forceinline__ int part_a(int pair) { return (0x001102 >> (4 * pair)) & 3; }
-__device__ __forceinline__ int part_b(int pair) { return (0x010120 >> (4 * pair)) & 3; }
+enum Kind { kHalf, kEight, kParts };  // 16-bit values, e4m3, fp32 in three bf16 parts
 
-template <int BN>
+// Parts multiplied in each of the six products, smallest first.
+__host__ __device__ constexpr int part_a(int pair) { return (0x001102 >> (4 * pair)) & 3; }
+__host__ __device__ constexpr int part_b(int pair) { return (0x010120 >> (4 * pair)) & 3; }
+
+// A stage holds 128 bytes of the summed axis of both operands, of all parts: each is loaded once for its three, two
+// or one products (loaded for each product anew, 100003 x 256 x 128 took 66 us against the copy engines' rate).
+template <int BN, Kind KIND>
 struct Shape {
-    static constexpr int kStageBytes = (kTileRows + BN) * kChunkBytes;
+    static constexpr int kParts = KIND == Kind::kParts ? 3 : 1;
+    static constexpr int kA = kTileRows * kChunkBytes, kB = BN * kChunkBytes;  // bytes of one part
+    static constexpr int kStageBytes = kParts * (kA + kB);
     static constexpr int kStages = 196608 / kStageBytes;
     static constexpr int kColumns = 2 * BN;
     static constexpr int kStaging = kStages * kStageBytes;  // 4 KB for each output warp
@@ -141,10 +146,11 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
     return __all_sync(0xffffffffu, fg::barrier_wait(bar, parity, stop, ignore_stop));
 }
 
-template <int BN, bool EIGHT, bool WGRAD>
+template <int BN, Kind KIND, bool WGRAD>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const MmaArgs a, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
-    using S = Shape<BN>;
+    using S = Shape<BN, KIND>;
+    constexpr bool EIGHT = KIND == kEight;
     constexpr int kChunk = EIGHT ? 128 : 64;  // values of the summed axis a stage holds
     extern __shared__ uint8_t dynamic[];
     __shared__ Tables t;
@@ -254,25 +260,26 @@ __global__ void __launch_bounds__(kThreads, 1)
             // 8 KB blocks of both operands; blocks beyond the last column are not loaded, their products not stored
             const int a_blocks = WGRAD ? min(2, (a.outer - w.row + 63) / 64) : 2;
             const int b_blocks = WGRAD || a.b_mn ? min(BN / 64, ((WGRAD ? a.inner : a.outer) - w.col + 63) / 64) : BN / 64;
-            for (int pair = a.first_pair; live && pair < 6; ++pair) {
-                const int pa = part_a(pair), pb = part_b(pair);
-                for (int c = 0; c < w.chunks; ++c, ++step) {
-                    const int s = (int)(step % S::kStages);
-                    const uint32_t bar = fg::smem_address(&t.full[s]), at = ring + s * S::kStageBytes, bt = at + kTileRows * kChunkBytes;
-                    if (step >= S::kStages && !warp_wait(fg::smem_address(&t.empty[s]), (step / S::kStages - 1) & 1, stop)) {
-                        live = false;
-                        break;
-                    }
-                    if (lane == 0) {
-                        fg::barrier_expect(bar, (a_blocks + b_blocks) * 8192);
-                        const int k = c * kChunk;
+            for (int c = 0; c < w.chunks; ++c, ++step) {
+                const int s = (int)(step % S::kStages);
+                const uint32_t bar = fg::smem_address(&t.full[s]), stage = ring + s * S::kStageBytes;
+                if (step >= S::kStages && !warp_wait(fg::smem_address(&t.empty[s]), (step / S::kStages - 1) & 1, stop)) {
+                    live = false;
+                    break;
+                }
+                if (lane == 0) {
+                    fg::barrier_expect(bar, (a_blocks + b_blocks) * 8192 * S::kParts);
+                    const int k = c * kChunk;
+#pragma unroll
+                    for (int p = 0; p < S::kParts; ++p) {
+                        const uint32_t at = stage + p * S::kA, bt = stage + S::kParts * S::kA + p * S::kB;
                         if (WGRAD) {  // 64 slots by 64 columns a block
-                            const int slot = w.begin + k;
-                            for (int q = 0; q < a_blocks; ++q) fg::tma_load_2d(at + q * 8192, &map_a, w.row + q * 64, slot + pa * (int)a.m, bar);
-                            for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d(bt + q * 8192, &map_b, w.col + q * 64, slot + pb * (int)a.m, bar);
+                            const int slot = w.begin + k + p * (int)a.m;
+                            for (int q = 0; q < a_blocks; ++q) fg::tma_load_2d(at + q * 8192, &map_a, w.row + q * 64, slot, bar);
+                            for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d(bt + q * 8192, &map_b, w.col + q * 64, slot, bar);
                         } else {
-                            const int g = a.shared_weight ? pb : w.group + pb * a.groups;
-                            fg::tma_load_2d(at, &map_a, k, w.begin + pa * (int)a.m, bar);
+                            const int g = a.shared_weight ? p : w.group + p * a.groups;
+                            fg::tma_load_2d(at, &map_a, k, w.begin + p * (int)a.m, bar);
                             if (!a.b_mn) {
                                 fg::tma_load_3d(bt, &map_b, k, w.col, g, bar);
                             } else {
@@ -280,8 +287,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                             }
                         }
                     }
-                    __syncwarp();
                 }
+                __syncwarp();
             }
         }
         if (__any_sync(0xffffffffu, *stop))  // no copy may be in flight when the block ends
@@ -301,36 +308,37 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (turn >= 2 && !warp_wait(fg::smem_address(&t.drained[buffer]), (turn / 2 - 1) & 1, stop)) break;
             fg::tcgen05_after_sync();
             bool add = false;
-            for (int pair = a.first_pair; live && pair < 6; ++pair) {
-                for (int c = 0; c < w.chunks; ++c, ++step) {
-                    const int s = (int)(step % S::kStages);
-                    const uint32_t at = ring + s * S::kStageBytes, bt = at + kTileRows * kChunkBytes;
-                    if (!warp_wait(fg::smem_address(&t.full[s]), (step / S::kStages) & 1, stop)) {
-                        live = false;
-                        break;
-                    }
-                    fg::tcgen05_after_sync();
-                    if (WGRAD && c == w.chunks - 1 && (w.end - w.begin) % kChunk != 0) {
-                        const int keep = (w.end - w.begin) % kChunk;  // rows of 128 bytes, 64 a column block
-                        const uint32_t blocks = (kTileRows + BN) / 64;
-                        for (uint32_t q = 0; q < blocks; ++q)
-                            for (int z = keep * 8 + lane; z < 64 * 8; z += 32)
-                                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(at + q * 8192 + z * 16), "r"(0) : "memory");
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                    }
-                    if (lane == 0) {
+            for (int c = 0; c < w.chunks; ++c, ++step) {
+                const int s = (int)(step % S::kStages);
+                const uint32_t stage = ring + s * S::kStageBytes;
+                if (!warp_wait(fg::smem_address(&t.full[s]), (step / S::kStages) & 1, stop)) {
+                    live = false;
+                    break;
+                }
+                fg::tcgen05_after_sync();
+                if (WGRAD && c == w.chunks - 1 && (w.end - w.begin) % kChunk != 0) {
+                    const int keep = (w.end - w.begin) % kChunk;  // rows of 128 bytes, 64 a column block
+                    for (int q = 0; q < S::kStageBytes / 8192; ++q)
+                        for (int z = keep * 8 + lane; z < 64 * 8; z += 32)
+                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage + q * 8192 + z * 16), "r"(0) : "memory");
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                if (lane == 0) {
+#pragma unroll
+                    for (int pair = S::kParts == 3 ? 0 : 5; pair < 6; ++pair) {
+                        const uint32_t at = stage + part_a(pair) * S::kA, bt = stage + S::kParts * S::kA + part_b(pair) * S::kB;
 #pragma unroll
                         for (int k = 0; k < 4; ++k) {
                             const uint64_t da = WGRAD ? fg::operand_descriptor(at + k * 2048, 8192, 1024) : fg::operand_descriptor(at + k * 32, 16, 1024);
                             const uint64_t db = b_mn ? fg::operand_descriptor(bt + k * 2048, 8192, 1024) : fg::operand_descriptor(bt + k * 32, 16, 1024);
-                            fg::product_step<EIGHT>(acc, da, db, descriptor, add || k > 0);
+                            fg::product_step<EIGHT>(acc, da, db, descriptor, add);
+                            add = true;
                         }
-                        fg::product_commit(fg::smem_address(&t.empty[s]));
                     }
-                    add = true;
-                    __syncwarp();
+                    fg::product_commit(fg::smem_address(&t.empty[s]));
                 }
+                __syncwarp();
             }
             if (!live) break;
             if (lane == 0) fg::product_commit(fg::smem_address(&t.filled[buffer]));
@@ -598,30 +606,31 @@ struct WeightLayout {
     }
 };
 
-template <int BN, bool EIGHT, bool WGRAD>
+template <int BN, Kind KIND, bool WGRAD>
 int launch_shape(const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b, int64_t most_tiles, cudaStream_t s) {
+    constexpr int kSmem = Shape<BN, KIND>::kSmem;
     static bool ready[fg::kMaxDevices];  // set once a device; setting it twice does no harm
     const int slot = fg::current_device_slot();
     if (slot < 0 || !ready[slot]) {
-        FG_CUDA_TRY(cudaFuncSetAttribute(product_kernel<BN, EIGHT, WGRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<BN>::kSmem));
+        FG_CUDA_TRY(cudaFuncSetAttribute(product_kernel<BN, KIND, WGRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         if (slot >= 0) ready[slot] = true;
     }
     const int64_t sms = fg::device_props().sm_count;
-    product_kernel<BN, EIGHT, WGRAD><<<(unsigned)(most_tiles < sms ? most_tiles : sms), kThreads, Shape<BN>::kSmem, s>>>(a, map_a, map_b);
+    product_kernel<BN, KIND, WGRAD><<<(unsigned)(most_tiles < sms ? most_tiles : sms), kThreads, kSmem, s>>>(a, map_a, map_b);
     FG_CUDA_TRY(cudaGetLastError());
     fg::count_launches(1);
     return FG_OK;
 }
-template <bool EIGHT, bool WGRAD>
+template <Kind KIND, bool WGRAD>
 int launch(int bn, const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b, int64_t most_tiles, cudaStream_t s) {
-    return bn == 256 ? launch_shape<256, EIGHT, WGRAD>(a, map_a, map_b, most_tiles, s)
-           : bn == 128 ? launch_shape<128, EIGHT, WGRAD>(a, map_a, map_b, most_tiles, s)
-                       : launch_shape<64, EIGHT, WGRAD>(a, map_a, map_b, most_tiles, s);
+    if constexpr (KIND != kParts)
+        if (bn == 256) return launch_shape<256, KIND, WGRAD>(a, map_a, map_b, most_tiles, s);
+    return bn == 128 ? launch_shape<128, KIND, WGRAD>(a, map_a, map_b, most_tiles, s) : launch_shape<64, KIND, WGRAD>(a, map_a, map_b, most_tiles, s);
 }
 
-// Columns of an output tile: the widest whose tiles still give each SM one.
-int tile_width(int64_t units, int width) {
-    for (int bn = 256; bn > 64; bn /= 2)
+// Columns of an output tile: the widest whose tiles still give each SM one (and of which two stages of parts fit).
+int tile_width(int64_t units, int width, int32_t type) {
+    for (int bn = type == FG_F32 ? 128 : 256; bn > 64; bn /= 2)
         if (width > bn / 2 && units * ((width + bn - 1) / bn) >= fg::device_props().sm_count) return bn;
     return 64;
 }
@@ -704,17 +713,19 @@ int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, con
         if (int rc = pack(d_w, w_group, step, b_mn ? w_out : w_in, layout.count, layout.rows, layout.cols, nullptr, 1, 0, type, &work, s)) return rc;
     }
     const int64_t units = num_rows / kTileRows + (groups < num_rows ? groups : num_rows);
-    const int bn = tile_width(units, outer), chunk = type == FG_E4M3 ? 128 : 64;
+    const int bn = tile_width(units, outer, type), chunk = type == FG_E4M3 ? 128 : 64;
     CUtensorMap map_x, map_w;
     if (int rc = make_map(&map_x, x, chunk, kTileRows)) return rc;
     if (int rc = make_map(&map_w, w, chunk, b_mn ? 64 : bn)) return rc;
     MmaArgs a{};
     a.offsets = d_offsets, a.order = d_order, a.x_scales = d_x_scales, a.w_scales = d_w_scales, a.y = d_y;
     a.m = num_rows, a.x_rows = x_rows, a.choices = choices, a.groups = groups, a.inner = inner, a.outer = outer;
-    a.type = type, a.out_type = out_type, a.format = w.type == FG_BF16 ? 1 : 0, a.first_pair = type == FG_F32 ? 0 : 5;
+    a.type = type, a.out_type = out_type, a.format = w.type == FG_BF16 ? 1 : 0;
     a.b_mn = b_mn, a.shared_weight = w_group == 0;
     const int64_t tiles = units * ((outer + bn - 1) / bn);
-    return type == FG_E4M3 ? launch<true, false>(bn, a, map_x, map_w, tiles, s) : launch<false, false>(bn, a, map_x, map_w, tiles, s);
+    return type == FG_E4M3  ? launch<kEight, false>(bn, a, map_x, map_w, tiles, s)
+           : type == FG_F32 ? launch<kParts, false>(bn, a, map_x, map_w, tiles, s)
+                            : launch<kHalf, false>(bn, a, map_x, map_w, tiles, s);
 }
 
 int64_t fg_grouped_matmul_wgrad_workspace(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const int32_t* d_order,
@@ -754,13 +765,14 @@ int fg_grouped_matmul_wgrad(const void* d_x, int64_t ldx, const void* d_dy, int6
     if (int rc = make_map(&map_dy, dy, 64, 64)) return rc;
     if (int rc = make_map(&map_x, x, 64, 64)) return rc;
     const int64_t units = split ? num_rows / split + groups : groups, rows_tiles = (outer + kTileRows - 1) / kTileRows;
-    const int bn = tile_width(units * rows_tiles, inner);
+    const int bn = tile_width(units * rows_tiles, inner, type);
     MmaArgs a{};
     a.offsets = d_offsets, a.order = d_order, a.y = split ? static_cast<void*>(sums) : d_dw;
     a.m = num_rows, a.x_rows = x_rows, a.choices = choices, a.groups = groups, a.inner = inner, a.outer = outer;
-    a.type = type, a.out_type = split ? FG_F32 : type, a.format = dy.type == FG_BF16 ? 1 : 0, a.first_pair = type == FG_F32 ? 0 : 5;
+    a.type = type, a.out_type = split ? FG_F32 : type, a.format = dy.type == FG_BF16 ? 1 : 0;
     a.split = (int32_t)split, a.units = (int32_t)units;
-    if (int rc = launch<false, true>(bn, a, map_dy, map_x, units * rows_tiles * ((inner + bn - 1) / bn), s)) return rc;
+    const int64_t tiles = units * rows_tiles * ((inner + bn - 1) / bn);
+    if (int rc = type == FG_F32 ? launch<kParts, true>(bn, a, map_dy, map_x, tiles, s) : launch<kHalf, true>(bn, a, map_dy, map_x, tiles, s)) return rc;
     if (split) {
         const dim3 grid((unsigned)((cells + 255) / 256 < 4096 ? (cells + 255) / 256 : 4096), (unsigned)groups);
         if (type == FG_F32) join_kernel<float><<<grid, 256, 0, s>>>(sums, d_offsets, groups, num_rows, (int)split, a.units, cells, static_cast<float*>(d_dw));

@@ -314,16 +314,17 @@ def _choose(logits, k, scoring, normalize):
 
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, k, scoring, normalize):
+    def forward(ctx, logits, k, scoring, normalize, lists):
         weights, chosen, g = _choose(logits, k, scoring, normalize)
-        ctx.mark_non_differentiable(chosen, g.offsets, g.order, g.position)
+        lists.append(chosen)  # what has no gradient does not pass through autograd
+        lists.append(g)
         ctx.save_for_backward(logits, weights, chosen)
         ctx.args = (k, scoring, normalize)
-        return weights, chosen, g.offsets, g.order, g.position
+        return weights
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dweights, *_):
+    def backward(ctx, dweights):
         logits, weights, chosen = ctx.saved_tensors
         x, ld = _as_rows(logits)
         dweights = dweights.contiguous()
@@ -331,7 +332,7 @@ class _Route(torch.autograd.Function):
         k, scoring, normalize = ctx.args
         _call("fg_route_backward", x.get_device(), x.data_ptr(), ld, weights.data_ptr(), chosen.data_ptr(), dweights.data_ptr(), dx.data_ptr(),
               x.shape[0], x.shape[1], k, _TYPES[x.dtype], scoring, normalize)
-        return dx, None, None, None
+        return dx, None, None, None, None
 
 
 def route(logits, k, scoring="softmax", normalize=True):
@@ -353,8 +354,9 @@ def route(logits, k, scoring="softmax", normalize=True):
     _on(logits)
     args = (k, _SCORING[scoring], 1 if normalize else 0)
     if _wants_grad(logits):
-        weights, chosen, *lists = _Route.apply(logits, *args)
-        return Routing(weights, chosen, RowGroups(*lists))
+        lists = []
+        weights = _Route.apply(logits, *args, lists)
+        return Routing(weights, *lists)
     return Routing(*_choose(logits, *args))
 
 
