@@ -34,7 +34,7 @@ using fg::Pack;
 using fg::store_pack;
 using fg::to_f32;
 
-constexpr int kTileRows = 128, kChunkBytes = 128, kThreads = 192, kMaxGroups = 1024, kSuperRows = 16;
+constexpr int kTileRows = 128, kChunkBytes = 128, kMaxGroups = 1024, kSuperRows = 16;
 
 __device__ int g_stuck;  // set when a wait ran out; fg_grouped_matmul_status reads it
 
@@ -48,6 +48,7 @@ struct MmaArgs {
     bool b_mn, shared_weight;
     int32_t split;        // dW: rows of one partial sum (0: a group's rows in one)
     int32_t units;        // dW: partial sums that there is room for
+    int32_t box_rows;     // y: rows of a tile that are loaded (all that a group can have, where that is fewer than a tile's)
 };
 
 enum Kind { kHalf, kEight, kParts };  // 16-bit values, e4m3, fp32 in three bf16 parts
@@ -58,19 +59,26 @@ __host__ __device__ constexpr int part_b(int pair) { return (0x010120 >> (4 * pa
 
 // A stage holds 128 bytes of the summed axis of both operands, of all parts: each is loaded once for its three, two
 // or one products (loaded for each product anew, 100003 x 256 x 128 took 66 us against the copy engines' rate).
-template <int BN, Kind KIND>
+//
+// FEW: at most 32 slots in all.  Only 4 KB of a stage hold rows; the products read 16 KB from there on, which for the rows
+// that are not stored is whatever lies in the stages behind.
+//
+// BLOCKS = 2: a pair of blocks computes 256 x BN; each loads 128 rows of the one operand and half the columns of the other,
+// and the first one's products read both shared memories (cta_group::2).
+template <int BN, Kind KIND, bool FEW, int BLOCKS>
 struct Shape {
     static constexpr int kParts = KIND == Kind::kParts ? 3 : 1;
-    static constexpr int kA = kTileRows * kChunkBytes, kB = BN * kChunkBytes;  // bytes of one part
+    static constexpr int kOwnCols = BN / BLOCKS;
+    static constexpr int kA = (FEW ? 32 : kTileRows) * kChunkBytes, kB = kOwnCols * kChunkBytes;  // bytes of one part
     static constexpr int kStageBytes = kParts * (kA + kB);
-    static constexpr int kStages = 196608 / kStageBytes;
+    static constexpr int kStages = 196608 / kStageBytes < 16 ? 196608 / kStageBytes : 16;
     static constexpr int kColumns = 2 * BN;
     static constexpr int kStaging = kStages * kStageBytes;  // 4 KB for each output warp
     static constexpr int kSmem = 1024 + kStaging + 4 * 4096;
 };
 
 struct Tables {
-    uint64_t full[8], empty[8], filled[2], drained[2], last;
+    uint64_t full[16], empty[16], filled[2], drained[2], ask, tail, last;
     uint32_t tmem;
     int stop;
     int warp_sums[8];
@@ -142,19 +150,25 @@ __device__ __forceinline__ void store_rows(uint32_t tmem, bool filled, O* out, i
 }
 
 // A wait of all lanes, with one answer for all of them.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop, bool ignore_stop = false) {
-    return __all_sync(0xffffffffu, fg::barrier_wait(bar, parity, stop, ignore_stop));
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop) {
+    return __all_sync(0xffffffffu, fg::barrier_wait<CLUSTER>(bar, parity, stop));
 }
 
-template <int BN, Kind KIND, bool WGRAD>
-__global__ void __launch_bounds__(kThreads, 1)
+template <bool WGRAD>
+constexpr int kThreads = WGRAD ? 224 : 192;
+
+template <int BN, Kind KIND, bool WGRAD, bool FEW, int BLOCKS>
+__global__ void __launch_bounds__(kThreads<WGRAD>, 1)
     product_kernel(const MmaArgs a, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
-    using S = Shape<BN, KIND>;
+    using S = Shape<BN, KIND, FEW, BLOCKS>;
     constexpr bool EIGHT = KIND == kEight;
     constexpr int kChunk = EIGHT ? 128 : 64;  // values of the summed axis a stage holds
+    constexpr int kRows = kTileRows * BLOCKS;
     extern __shared__ uint8_t dynamic[];
     __shared__ Tables t;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int rank = BLOCKS == 2 ? (int)fg::cluster_rank() : 0;
     const uint32_t ring = (fg::smem_address(dynamic) + 1023u) & ~1023u;
 
     if (threadIdx.x == 0) {
@@ -164,20 +178,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int s = 0; s < 2; ++s) {
             fg::barrier_init(fg::smem_address(&t.filled[s]), 1);
-            fg::barrier_init(fg::smem_address(&t.drained[s]), 4);
+            fg::barrier_init(fg::smem_address(&t.drained[s]), 4 * BLOCKS);
         }
+        fg::barrier_init(fg::smem_address(&t.ask), 1);
+        fg::barrier_init(fg::smem_address(&t.tail), BLOCKS);
         fg::barrier_init(fg::smem_address(&t.last), 1);
         fg::barrier_init_fence();
         t.stop = 0;
         fg::prefetch_map(&map_a);
         fg::prefetch_map(&map_b);
     }
-    if (warp == 1) fg::tmem_alloc(fg::smem_address(&t.tmem), S::kColumns);
+    if (warp == 1) fg::tmem_alloc<BLOCKS>(fg::smem_address(&t.tmem), S::kColumns);
 
     // groups' first slots and tile counts, scanned: thread i takes groups [i * each, (i + 1) * each)
     {
-        const int each = (a.groups + kThreads - 1) / kThreads, from = min((int)threadIdx.x * each, a.groups), to = min(from + each, a.groups);
-        const int64_t unit = WGRAD ? (a.split ? a.split : (int64_t)INT_MAX) : kTileRows;
+        constexpr int kAll = kThreads<WGRAD>;
+        const int each = (a.groups + kAll - 1) / kAll, from = min((int)threadIdx.x * each, a.groups), to = min(from + each, a.groups);
+        const int64_t unit = WGRAD ? (a.split ? a.split : (int64_t)INT_MAX) : kRows;
         int own = 0;
         for (int g = from; g < to; ++g) {
             const int64_t b = min((int64_t)max(a.offsets[g], 0), a.m), e = min((int64_t)max(a.offsets[g + 1], 0), a.m);
@@ -201,23 +218,25 @@ __global__ void __launch_bounds__(kThreads, 1)
             t.tiles[g] = before;
             before += (int)(WGRAD ? max((n + unit - 1) / unit, (int64_t)1) : (n + unit - 1) / unit);
         }
-        if (threadIdx.x == kThreads - 1) {
+        if (threadIdx.x == kAll - 1) {
             t.tiles[a.groups] = before;
             t.start[a.groups] = (int)min((int64_t)max(a.offsets[a.groups], 0), a.m);
         }
     }
     fg::tcgen05_before_sync();
     __syncthreads();
+    if (BLOCKS == 2) fg::cluster_sync();  // the other block's barriers are there
     fg::tcgen05_after_sync();
 
-    const int rows_tiles = WGRAD ? (a.outer + kTileRows - 1) / kTileRows : 1;
+    const int rows_tiles = WGRAD ? (a.outer + kRows - 1) / kRows : 1;
     const int col_tiles = ((WGRAD ? a.inner : a.outer) + BN - 1) / BN;
     const int per_unit = WGRAD ? rows_tiles * col_tiles : col_tiles;  // output tiles for each counted row tile or partial sum
     const int64_t total = (int64_t)t.tiles[a.groups] * per_unit;
+    const int64_t start = blockIdx.x / BLOCKS, stride = gridDim.x / BLOCKS;
     const uint32_t tmem = t.tmem;
     volatile int* stop = &t.stop;
 
-    // What output tile `index` is: its group, first row and column, the slots [begin, end) it is about.
+    // What output tile `index` is for this block: its group, first row and column, the slots [begin, end) it is about.
     struct Tile {
         int group, unit, row, col;
         int begin, end, chunks;
@@ -233,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (WGRAD) {
             const int part = (int)(local / per_unit), tile = (int)(local - (int64_t)part * per_unit);
             w.unit = min(t.tiles[cursor] + part, a.units - 1);  // lists that overlap: wrong sums, no wrong address
-            w.row = tile % rows_tiles * kTileRows;
+            w.row = tile % rows_tiles * kRows + rank * kTileRows;
             w.col = tile / rows_tiles * BN;
             w.begin = a.split ? first + part * a.split : first;
             w.end = a.split ? min(w.begin + a.split, stop_at) : stop_at;
@@ -243,7 +262,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int super = (int)(local / ((int64_t)kSuperRows * col_tiles)), left = min(kSuperRows, count - super * kSuperRows);
             const int rest = (int)(local - (int64_t)super * kSuperRows * col_tiles);
             w.unit = 0;
-            w.begin = first + (super * kSuperRows + rest % left) * kTileRows;
+            w.begin = first + (super * kSuperRows + rest % left) * kRows + rank * kTileRows;
             w.end = min(w.begin + kTileRows, stop_at);
             w.row = 0;
             w.col = rest / left * BN;
@@ -253,78 +272,79 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
 
     if (warp == 0) {
-        int64_t step = 0;  // stages filled so far
-        bool live = true;
-        for (int64_t i = blockIdx.x; live && i < total; i += gridDim.x) {
-            const Tile w = locate(i);
-            // 8 KB blocks of both operands; blocks beyond the last column are not loaded, their products not stored
-            const int a_blocks = WGRAD ? min(2, (a.outer - w.row + 63) / 64) : 2;
-            const int b_blocks = WGRAD || a.b_mn ? min(BN / 64, ((WGRAD ? a.inner : a.outer) - w.col + 63) / 64) : BN / 64;
-            for (int c = 0; c < w.chunks; ++c, ++step) {
-                const int s = (int)(step % S::kStages);
-                const uint32_t bar = fg::smem_address(&t.full[s]), stage = ring + s * S::kStageBytes;
-                if (step >= S::kStages && !warp_wait(fg::smem_address(&t.empty[s]), (step / S::kStages - 1) & 1, stop)) {
-                    live = false;
-                    break;
-                }
-                if (lane == 0) {
-                    fg::barrier_expect(bar, (a_blocks + b_blocks) * 8192 * S::kParts);
+        if (fg::elect_one()) {
+            int64_t step = 0;  // stages filled so far
+            bool live = true;
+            for (int64_t i = start; live && i < total; i += stride) {
+                const Tile w = locate(i);
+                const int col = w.col + rank * S::kOwnCols;
+                // 8 KB blocks of both operands; blocks beyond the last column are not loaded, their products not stored
+                auto blocks_a = [&](int row) { return WGRAD ? max(min(2, (a.outer - row + 63) / 64), 0) : 0; };
+                auto blocks_b = [&](int at) {
+                    return WGRAD || a.b_mn ? max(min(S::kOwnCols / 64, ((WGRAD ? a.inner : a.outer) - at + 63) / 64), 0) : S::kOwnCols / 64;
+                };
+                const int a_blocks = blocks_a(w.row), b_blocks = blocks_b(col);
+                uint32_t bytes = ((WGRAD ? a_blocks * 8192 : a.box_rows * kChunkBytes) + b_blocks * 8192) * S::kParts;
+                if (BLOCKS == 2)  // the first block's barrier counts the second one's loads too
+                    bytes += ((WGRAD ? blocks_a(w.row + kTileRows) * 8192 : a.box_rows * kChunkBytes) + blocks_b(col + S::kOwnCols) * 8192) * S::kParts;
+                for (int c = 0; c < w.chunks; ++c, ++step) {
+                    const int s = (int)(step % S::kStages);
+                    const uint32_t bar = fg::smem_address(&t.full[s]), stage = ring + s * S::kStageBytes;
+                    if (step >= S::kStages && !fg::barrier_wait(fg::smem_address(&t.empty[s]), (step / S::kStages - 1) & 1, stop)) {
+                        live = false;
+                        break;
+                    }
+                    if (rank == 0) fg::barrier_expect(bar, bytes);
                     const int k = c * kChunk;
 #pragma unroll
                     for (int p = 0; p < S::kParts; ++p) {
                         const uint32_t at = stage + p * S::kA, bt = stage + S::kParts * S::kA + p * S::kB;
                         if (WGRAD) {  // 64 slots by 64 columns a block
                             const int slot = w.begin + k + p * (int)a.m;
-                            for (int q = 0; q < a_blocks; ++q) fg::tma_load_2d(at + q * 8192, &map_a, w.row + q * 64, slot, bar);
-                            for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d(bt + q * 8192, &map_b, w.col + q * 64, slot, bar);
+                            for (int q = 0; q < a_blocks; ++q) fg::tma_load_2d<BLOCKS>(at + q * 8192, &map_a, w.row + q * 64, slot, bar);
+                            for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d<BLOCKS>(bt + q * 8192, &map_b, col + q * 64, slot, bar);
                         } else {
                             const int g = a.shared_weight ? p : w.group + p * a.groups;
-                            fg::tma_load_2d(at, &map_a, k, w.begin + p * (int)a.m, bar);
+                            fg::tma_load_2d<BLOCKS>(at, &map_a, k, w.begin + p * (int)a.m, bar);
                             if (!a.b_mn) {
-                                fg::tma_load_3d(bt, &map_b, k, w.col, g, bar);
+                                fg::tma_load_3d<BLOCKS>(bt, &map_b, k, col, g, bar);
                             } else {
-                                for (int q = 0; q < b_blocks; ++q) fg::tma_load_3d(bt + q * 8192, &map_b, w.col + q * 64, k, g, bar);
+                                for (int q = 0; q < b_blocks; ++q) fg::tma_load_3d<BLOCKS>(bt + q * 8192, &map_b, col + q * 64, k, g, bar);
                             }
                         }
                     }
                 }
-                __syncwarp();
             }
+            if (*stop && rank == 0)  // no copy may be in flight when the block (or its pair) ends
+                for (int64_t q = max(step - S::kStages, (int64_t)0); q < step; ++q)
+                    fg::barrier_wait(fg::smem_address(&t.full[q % S::kStages]), (q / S::kStages) & 1, stop, true);
         }
-        if (__any_sync(0xffffffffu, *stop))  // no copy may be in flight when the block ends
-            for (int64_t q = max(step - S::kStages, (int64_t)0); q < step; ++q)
-                warp_wait(fg::smem_address(&t.full[q % S::kStages]), (q / S::kStages) & 1, stop, true);
+        __syncwarp();
     } else if (warp == 1) {
-        int64_t step = 0;
-        int64_t turn = 0;
-        const uint32_t descriptor = fg::product_descriptor(a.format, WGRAD, WGRAD || a.b_mn, kTileRows, BN);
-        const bool b_mn = WGRAD || a.b_mn;
-        bool live = true;
-        for (int64_t i = blockIdx.x; live && i < total; i += gridDim.x) {
-            const Tile w = locate(i);
-            if (w.chunks == 0) continue;  // an empty group's dW: nothing to add up
-            const int buffer = (int)(turn & 1);
-            const uint32_t acc = tmem + buffer * BN;
-            if (turn >= 2 && !warp_wait(fg::smem_address(&t.drained[buffer]), (turn / 2 - 1) & 1, stop)) break;
-            fg::tcgen05_after_sync();
-            bool add = false;
-            for (int c = 0; c < w.chunks; ++c, ++step) {
-                const int s = (int)(step % S::kStages);
-                const uint32_t stage = ring + s * S::kStageBytes;
-                if (!warp_wait(fg::smem_address(&t.full[s]), (step / S::kStages) & 1, stop)) {
-                    live = false;
-                    break;
-                }
+        if (rank == 0 && fg::elect_one()) {
+            int64_t step = 0, turn = 0, tails = 0;
+            const uint32_t descriptor = fg::product_descriptor(a.format, WGRAD, WGRAD || a.b_mn, kRows, BN);
+            const bool b_mn = WGRAD || a.b_mn;
+            bool live = true;
+            for (int64_t i = start; live && i < total; i += stride) {
+                const Tile w = locate(i);
+                if (w.chunks == 0) continue;  // an empty group's dW: nothing to add up
+                const bool tail = WGRAD && (w.end - w.begin) % kChunk != 0;
+                const int buffer = (int)(turn & 1);
+                const uint32_t acc = tmem + buffer * BN;
+                if (turn >= 2 && !fg::barrier_wait<BLOCKS == 2>(fg::smem_address(&t.drained[buffer]), (turn / 2 - 1) & 1, stop)) break;
                 fg::tcgen05_after_sync();
-                if (WGRAD && c == w.chunks - 1 && (w.end - w.begin) % kChunk != 0) {
-                    const int keep = (w.end - w.begin) % kChunk;  // rows of 128 bytes, 64 a column block
-                    for (int q = 0; q < S::kStageBytes / 8192; ++q)
-                        for (int z = keep * 8 + lane; z < 64 * 8; z += 32)
-                            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage + q * 8192 + z * 16), "r"(0) : "memory");
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                    __syncwarp();
-                }
-                if (lane == 0) {
+                for (int c = 0; c < w.chunks; ++c, ++step) {
+                    const int s = (int)(step % S::kStages);
+                    const uint32_t stage = ring + s * S::kStageBytes, parity = (step / S::kStages) & 1;
+                    live = fg::barrier_wait(fg::smem_address(&t.full[s]), parity, stop);
+                    if (live && tail && c == w.chunks - 1) {
+                        fg::barrier_arrive(fg::smem_address(&t.ask));
+                        if (BLOCKS == 2) fg::barrier_arrive_at(fg::smem_address(&t.ask), 1);
+                        live = fg::barrier_wait<BLOCKS == 2>(fg::smem_address(&t.tail), tails++ & 1, stop);
+                    }
+                    if (!live) break;
+                    fg::tcgen05_after_sync();
 #pragma unroll
                     for (int pair = S::kParts == 3 ? 0 : 5; pair < 6; ++pair) {
                         const uint32_t at = stage + part_a(pair) * S::kA, bt = stage + S::kParts * S::kA + part_b(pair) * S::kB;
@@ -332,23 +352,43 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int k = 0; k < 4; ++k) {
                             const uint64_t da = WGRAD ? fg::operand_descriptor(at + k * 2048, 8192, 1024) : fg::operand_descriptor(at + k * 32, 16, 1024);
                             const uint64_t db = b_mn ? fg::operand_descriptor(bt + k * 2048, 8192, 1024) : fg::operand_descriptor(bt + k * 32, 16, 1024);
-                            fg::product_step<EIGHT>(acc, da, db, descriptor, add);
-                            add = true;
+                            fg::product_step<BLOCKS, EIGHT>(acc, da, db, descriptor, c > 0 || pair > (S::kParts == 3 ? 0 : 5) || k > 0);
                         }
                     }
-                    fg::product_commit(fg::smem_address(&t.empty[s]));
+                    fg::product_commit<BLOCKS>(fg::smem_address(&t.empty[s]));
                 }
-                __syncwarp();
+                if (!live) break;
+                fg::product_commit<BLOCKS>(fg::smem_address(&t.filled[buffer]));
+                ++turn;
             }
-            if (!live) break;
-            if (lane == 0) fg::product_commit(fg::smem_address(&t.filled[buffer]));
-            __syncwarp();
-            ++turn;
+            if (*stop) {  // products in flight end before the accumulators are freed
+                fg::product_commit<BLOCKS>(fg::smem_address(&t.last));
+                fg::barrier_wait(fg::smem_address(&t.last), 0, stop, true);
+            }
         }
-        if (__any_sync(0xffffffffu, *stop)) {  // products in flight end before the accumulators are freed
-            if (lane == 0) fg::product_commit(fg::smem_address(&t.last));
+        __syncwarp();
+    } else if (WGRAD && warp == 6) {
+        // The rows of a group's last chunk that are not its own become zeros, on being asked once the chunk is there: 128
+        // bytes a row, 64 rows a column block.
+        int64_t step = 0, tails = 0;
+        for (int64_t i = start; i < total; i += stride) {
+            const Tile w = locate(i);
+            step += w.chunks;
+            const int keep = (w.end - w.begin) % kChunk;
+            if (w.chunks == 0 || keep == 0) continue;
+            const int s = (int)((step - 1) % S::kStages);
+            const uint32_t stage = ring + s * S::kStageBytes;
+            if (!warp_wait<BLOCKS == 2>(fg::smem_address(&t.ask), tails++ & 1, stop)) break;
+            for (int q = 0; q < S::kStageBytes / 8192; ++q)
+                for (int z = keep * 8 + lane; z < 64 * 8; z += 32)
+                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage + q * 8192 + z * 16), "r"(0) : "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
-            warp_wait(fg::smem_address(&t.last), 0, stop, true);
+            if (lane == 0) {
+                if (BLOCKS == 2) fg::barrier_arrive_at(fg::smem_address(&t.tail), 0);
+                else fg::barrier_arrive(fg::smem_address(&t.tail));
+            }
+            __syncwarp();
         }
     } else {
         const int quarter = warp & 3;  // the lanes of tensor memory this warp can read
@@ -357,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int size = a.out_type == FG_F32 ? 4 : 2;
         const bool vector = (int64_t)width * size % 16 == 0 && ((uintptr_t)a.y & 15) == 0;
         int64_t turn = 0;
-        for (int64_t i = blockIdx.x; i < total; i += gridDim.x) {
+        for (int64_t i = start; i < total; i += stride) {
             const Tile w = locate(i);
             const int above = quarter * 32;
             const int rows = (WGRAD ? a.outer - w.row : w.end - w.begin) - above;
@@ -389,21 +429,180 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (w.chunks) {
                 fg::tcgen05_before_sync();
                 __syncwarp();
-                if (lane == 0) fg::barrier_arrive(fg::smem_address(&t.drained[buffer]));
+                if (lane == 0) {
+                    if (BLOCKS == 2) fg::barrier_arrive_at(fg::smem_address(&t.drained[buffer]), 0);
+                    else fg::barrier_arrive(fg::smem_address(&t.drained[buffer]));
+                }
                 ++turn;
             }
         }
         if (!WGRAD) {  // rows in no group
-            const int64_t first = (int64_t)t.start[a.groups] * a.outer, values = a.m * a.outer;
-            for (int64_t i = first + (int64_t)blockIdx.x * 128 + (threadIdx.x - 64); i < values; i += (int64_t)gridDim.x * 128) {
+            const int64_t from = (int64_t)t.start[a.groups] * a.outer, values = a.m * a.outer;
+            for (int64_t i = from + (int64_t)blockIdx.x * 128 + (threadIdx.x - 64); i < values; i += (int64_t)gridDim.x * 128) {
                 if (a.out_type == FG_F32) static_cast<float*>(a.y)[i] = 0.0f;
                 else static_cast<uint16_t*>(a.y)[i] = 0;
             }
         }
     }
+    fg::tcgen05_before_sync();
     __syncthreads();
-    if (warp == 1) fg::tmem_free(tmem, S::kColumns);
+    if (BLOCKS == 2) fg::cluster_sync();  // nothing of the other block is still to arrive here
+    if (warp == 1) fg::tmem_free<BLOCKS>(tmem, S::kColumns);
     if (threadIdx.x == 0 && t.stop) atomicExch(&g_stuck, 1);
+}
+
+// ---- few rows ----
+
+// The form for single tokens: at most kFewRows slots in all.  Bound: the touched weights' bytes, read once for the rows of
+// a group (up to 8 at a time).  A tile of the tensor cores would be nearly empty and its column tiles too few for the
+// SMs: 4 rows x 2 of 16 experts x 2048 x 4096 in bf16 took 34 us there after a 4 us copy of the gathered rows.  Here a
+// block takes 64 columns of the j-th group that has rows, holds up to 8 of its rows in shared memory, and a warp computes
+// four columns at a time, its lanes side by side along the dense inner axis: 16-byte loads, four in flight a lane, each
+// row's values fetched from shared memory once for the four columns; 32-bit multiply-adds and a sum across the warp.
+constexpr int kFewRows = 32, kFewCols = 64;
+
+template <typename T>
+__device__ __forceinline__ void widen(const Pack<T, 16 / sizeof(T)>& p, float (&v)[16 / sizeof(T)]) {
+#pragma unroll
+    for (int j = 0; j < (int)(16 / sizeof(T)); ++j) v[j] = to_f32<T>(p.v[j]);
+}
+
+struct FewArgs {
+    const void *x, *w;
+    const float *x_scales, *w_scales;
+    const int32_t *offsets, *order;
+    void* y;
+    int64_t ldx, w_group, w_out, x_rows;
+    int32_t m, choices, groups, inner, outer, out_type, pitch;  // pitch: values of a row in shared memory
+    bool vector, vector_rows;                                   // weights, rows on the 16-byte grid
+};
+
+template <typename T, int R>
+__device__ __forceinline__ void few_columns(const FewArgs& a, const T* rows, const T* w, int col, int count, int first, int n, const float* scales,
+                                            const float* column_scales) {
+    constexpr int kPer = 16 / sizeof(T);
+    const int lane = threadIdx.x & 31;
+    float acc[R][4];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[r][c] = 0.0f;
+    const T* column[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) column[c] = w + (int64_t)(col + min(c, count - 1)) * a.w_out;
+#pragma unroll 2
+    for (int k = lane * kPer; k < a.inner; k += 32 * kPer) {
+        float v[4][kPer];
+        if (a.vector && k + kPer <= a.inner) {
+            Pack<T, kPer> p[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) p[c] = fg::load_pack<T, kPer>(column[c] + k);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) widen<T>(p[c], v[c]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) v[c][j] = k + j < a.inner ? to_f32<T>(column[c][k + j]) : 0.0f;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float x[kPer];
+            widen<T>(fg::load_pack<T, kPer>(rows + r * a.pitch + k), x);  // zeros beyond the inner axis
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) acc[r][c] = __fmaf_rn(x[j], v[c][j], acc[r][c]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[r][c] = fg::warp_sum(acc[r][c]);
+        if (r >= n) break;
+        if (lane < count) {
+            float v = lane == 0 ? acc[r][0] : lane == 1 ? acc[r][1] : lane == 2 ? acc[r][2] : acc[r][3];
+            if (scales) v = __fmul_rn(__fmul_rn(v, scales[r]), column_scales[col + lane]);
+            const int64_t at = (int64_t)(first + r) * a.outer + col + lane;
+            if (a.out_type == FG_F32) static_cast<float*>(a.y)[at] = v;
+            else if (a.out_type == FG_F16) static_cast<__half*>(a.y)[at] = from_f32<__half>(v);
+            else static_cast<__nv_bfloat16*>(a.y)[at] = from_f32<__nv_bfloat16>(v);
+        }
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) few_rows_kernel(const FewArgs a) {
+    extern __shared__ __align__(16) uint8_t dynamic[];
+    __shared__ int offsets[kMaxGroups + 1];
+    __shared__ int group;
+    __shared__ float scales[8];
+    T* rows = reinterpret_cast<T*>(dynamic);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, rank = blockIdx.y, col0 = blockIdx.x * kFewCols;
+    for (int g = threadIdx.x; g <= a.groups; g += 256) offsets[g] = min(max(a.offsets[g], 0), a.m);
+    if (threadIdx.x == 0) group = -1;
+    __syncthreads();
+    if (warp == 0) {  // the group of this rank among those with rows
+        int before = 0;
+        for (int base = 0; base < a.groups; base += 32) {
+            const int g = base + lane;
+            const bool some = g < a.groups && offsets[g + 1] > offsets[g];
+            const unsigned vote = __ballot_sync(0xffffffffu, some);
+            if (some && before + __popc(vote & ((1u << lane) - 1u)) == rank) group = g;
+            before += __popc(vote);
+            if (before > rank) break;
+        }
+    }
+    if (rank == 0) {  // rows in no group
+        const int from = offsets[a.groups], cols = min(kFewCols, a.outer - col0);
+        for (int i = threadIdx.x; i < (a.m - from) * cols; i += 256) {
+            const int64_t at = (int64_t)(from + i / cols) * a.outer + col0 + i % cols;
+            if (a.out_type == FG_F32) static_cast<float*>(a.y)[at] = 0.0f;
+            else static_cast<uint16_t*>(a.y)[at] = 0;
+        }
+    }
+    __syncthreads();
+    if (group < 0) return;
+    const int begin = offsets[group], end = offsets[group + 1];
+    const T* w = static_cast<const T*>(a.w) + (int64_t)group * a.w_group;
+    const float* column_scales = a.w_scales ? a.w_scales + (int64_t)group * a.outer : nullptr;
+    for (int first = begin; first < end; first += 8) {
+        const int n = min(8, end - first), held = n <= 2 ? n : n <= 4 ? 4 : 8;
+        constexpr int kPer = 16 / sizeof(T);
+        const int pieces = a.pitch / kPer;
+        for (int i = threadIdx.x; i < held * pieces; i += 256) {  // 16 bytes of a row a thread
+            const int r = i / pieces, k = (i - r * pieces) * kPer;
+            int64_t source = -1;
+            if (r < n) {
+                source = first + r;
+                if (a.order) {
+                    const int e = a.order[first + r];
+                    source = e >= 0 ? e / a.choices : -1;
+                }
+                if (source >= a.x_rows) source = -1;
+            }
+            const T* x = static_cast<const T*>(a.x) + (source < 0 ? 0 : source) * a.ldx + k;
+            Pack<T, kPer> p;
+            if (source >= 0 && a.vector_rows && k + kPer <= a.inner) {
+                p = fg::load_pack<T, kPer>(x);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) p.v[j] = source >= 0 && k + j < a.inner ? x[j] : T(0.0f);
+            }
+            store_pack<T, kPer>(rows + r * a.pitch + k, p);
+            if (k == 0) scales[r] = a.x_scales && source >= 0 ? a.x_scales[source] : 0.0f;
+        }
+        __syncthreads();
+        for (int c = warp * 4; c < kFewCols && col0 + c < a.outer; c += 32) {
+            const int col = col0 + c, count = min(4, a.outer - col);
+            const float* sc = a.x_scales ? scales : nullptr;
+            if (n == 1) few_columns<T, 1>(a, rows, w, col, count, first, n, sc, column_scales);
+            else if (n == 2) few_columns<T, 2>(a, rows, w, col, count, first, n, sc, column_scales);
+            else if (n <= 4) few_columns<T, 4>(a, rows, w, col, count, first, n, sc, column_scales);
+            else few_columns<T, 8>(a, rows, w, col, count, first, n, sc, column_scales);
+        }
+        __syncthreads();
+    }
 }
 
 // dW[g] = its partial sums added in order.
@@ -590,6 +789,22 @@ int rows_matrix(Matrix* out, const void* p, int64_t ld, int64_t source_rows, con
     return pack(p, 0, ld, 1, 1, m, cols, order, choices, source_rows, type, work, s);
 }
 
+// Few rows, a dense inner axis and 8 rows of it in shared memory: the form without tiles.
+bool few_rows(int64_t num_rows, int64_t w_in, int32_t inner, int32_t type) {
+    return type == FG_F32 && num_rows <= kFewRows && (w_in == 1 || inner == 1) && round_up(inner, 16) * 8 * fg::type_size(type) <= 192 * 1024;
+}
+template <typename T>
+int launch_few(const FewArgs& a, cudaStream_t s) {
+    const int held = a.m < 8 ? (a.m <= 2 ? a.m : a.m <= 4 ? 4 : 8) : 8;
+    const size_t smem = (size_t)held * a.pitch * sizeof(T);
+    if (smem > 40 * 1024) FG_CUDA_TRY(cudaFuncSetAttribute(few_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 200 * 1024));
+    const dim3 grid((a.outer + kFewCols - 1) / kFewCols, a.m < a.groups ? a.m : a.groups);
+    few_rows_kernel<T><<<grid, 256, smem, s>>>(a);
+    FG_CUDA_TRY(cudaGetLastError());
+    fg::count_launches(1);
+    return FG_OK;
+}
+
 // The weight is read as it is stored where its inner or its outer axis is dense (8-bit products want the inner one), or
 // copied with that axis dense; a group stride of 0 is one weight for all groups.
 struct WeightLayout {
@@ -606,26 +821,48 @@ struct WeightLayout {
     }
 };
 
-template <int BN, Kind KIND, bool WGRAD>
+template <int BN, Kind KIND, bool WGRAD, bool FEW, int BLOCKS>
 int launch_shape(const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b, int64_t most_tiles, cudaStream_t s) {
-    constexpr int kSmem = Shape<BN, KIND>::kSmem;
-    static bool ready[fg::kMaxDevices];  // set once a device; setting it twice does no harm
+    constexpr int kSmem = Shape<BN, KIND, FEW, BLOCKS>::kSmem;
+    const auto kernel = product_kernel<BN, KIND, WGRAD, FEW, BLOCKS>;
+    cudaLaunchConfig_t config = {};
+    config.blockDim = dim3(kThreads<WGRAD>);
+    config.dynamicSmemBytes = kSmem;
+    config.stream = s;
+    cudaLaunchAttribute cluster;
+    cluster.id = cudaLaunchAttributeClusterDimension;
+    cluster.val.clusterDim.x = BLOCKS, cluster.val.clusterDim.y = 1, cluster.val.clusterDim.z = 1;
+    config.attrs = &cluster;
+    config.numAttrs = BLOCKS == 2 ? 1 : 0;
+    static int resident[fg::kMaxDevices];  // blocks (pairs) that run at once; found once a device, twice does no harm
     const int slot = fg::current_device_slot();
-    if (slot < 0 || !ready[slot]) {
-        FG_CUDA_TRY(cudaFuncSetAttribute(product_kernel<BN, KIND, WGRAD>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-        if (slot >= 0) ready[slot] = true;
+    int most = slot < 0 ? 0 : resident[slot];
+    if (most == 0) {
+        FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+        most = fg::device_props().sm_count;
+        if (BLOCKS == 2) {
+            config.gridDim = dim3(most / 2 * 2);
+            FG_CUDA_TRY(cudaOccupancyMaxActiveClusters(&most, kernel, &config));
+            if (most < 1) return fg::fail(FG_ERR_CUDA, "no room for a pair of blocks");
+        }
+        if (slot >= 0) resident[slot] = most;
     }
-    const int64_t sms = fg::device_props().sm_count;
-    product_kernel<BN, KIND, WGRAD><<<(unsigned)(most_tiles < sms ? most_tiles : sms), kThreads, kSmem, s>>>(a, map_a, map_b);
-    FG_CUDA_TRY(cudaGetLastError());
+    config.gridDim = dim3((unsigned)(most_tiles < most ? most_tiles : most) * BLOCKS);
+    FG_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, a, map_a, map_b));
     fg::count_launches(1);
     return FG_OK;
 }
+// bn 512 stands for pairs of blocks: 256 x 256 tiles.
 template <Kind KIND, bool WGRAD>
 int launch(int bn, const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b, int64_t most_tiles, cudaStream_t s) {
-    if constexpr (KIND != kParts)
-        if (bn == 256) return launch_shape<256, KIND, WGRAD>(a, map_a, map_b, most_tiles, s);
-    return bn == 128 ? launch_shape<128, KIND, WGRAD>(a, map_a, map_b, most_tiles, s) : launch_shape<64, KIND, WGRAD>(a, map_a, map_b, most_tiles, s);
+    if constexpr (KIND != kParts) {
+        if constexpr (!WGRAD)
+            if (a.box_rows <= 32) return launch_shape<64, KIND, false, true, 1>(a, map_a, map_b, most_tiles, s);
+        if (bn == 512) return launch_shape<256, KIND, WGRAD, false, 2>(a, map_a, map_b, most_tiles, s);
+        if (bn == 256) return launch_shape<256, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s);
+    }
+    return bn == 128 ? launch_shape<128, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s)
+                     : launch_shape<64, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s);
 }
 
 // Columns of an output tile: the widest whose tiles still give each SM one (and of which two stages of parts fit).
@@ -633,6 +870,14 @@ int tile_width(int64_t units, int width, int32_t type) {
     for (int bn = type == FG_F32 ? 128 : 256; bn > 64; bn /= 2)
         if (width > bn / 2 && units * ((width + bn - 1) / bn) >= fg::device_props().sm_count) return bn;
     return 64;
+}
+// Pairs of blocks (256 x 256 tiles) load a third less for the same products, which is what 128 x 256 tiles wait for, but
+// leave more of the last tiles empty: taken where the tiles they add are less than a tenth of all, and give
+// each pair two.  `rows_tiles`, `row_pairs`: 128- and 256-row tiles.
+bool pairs_pay(int64_t row_tiles, int64_t row_pairs, int width, int32_t type) {
+    if (type == FG_F32 || width <= 128) return false;
+    const int64_t cols = (width + 255) / 256;
+    return row_pairs * cols >= fg::device_props().sm_count && row_pairs * 2 * 10 <= row_tiles * 11;
 }
 
 // Rows of one partial sum of dW: 0 (none) where the tiles of all groups already give each SM two, else such that they do.
@@ -674,7 +919,7 @@ int fg_grouped_matmul_status(void* stream) {
 
 int64_t fg_grouped_matmul_workspace(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,
                                     const int32_t* d_order, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
-    if (num_rows <= 0 || groups < 1 || inner < 1 || outer < 1) return 0;
+    if (num_rows <= 0 || groups < 1 || inner < 1 || outer < 1 || few_rows(num_rows, w_in, inner, type)) return 0;
     const WeightLayout w(d_w, w_group, w_out, w_in, groups, inner, outer, type);
     return (rows_need_copy(d_x, ldx ? ldx : inner, d_order, type) ? packed_bytes(num_rows, inner, type) : 0) +
            (w.copy ? packed_bytes(w.count * w.rows, w.cols, type) : 0);
@@ -697,6 +942,17 @@ int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, con
     if (!d_order && x_rows != num_rows) return fg::fail(FG_ERR_INVALID_ARGUMENT, "without an order x has a row for each slot");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
 
+    if (few_rows(num_rows, w_in, inner, type)) {
+        const int size = fg::type_size(type);
+        FewArgs f{d_x, d_w, type == FG_E4M3 ? d_x_scales : nullptr, type == FG_E4M3 ? d_w_scales : nullptr, d_offsets, d_order, d_y, ldx, w_group, w_out, x_rows,
+                  (int32_t)num_rows, choices, groups, inner, outer, out_type, (int32_t)round_up(inner, 16), false, false};
+        f.vector_rows = fg::aligned16(d_x) && ldx * size % 16 == 0;
+        f.vector = fg::aligned16(d_w) && w_out * size % 16 == 0 && w_group * size % 16 == 0;
+        return type == FG_F32   ? launch_few<float>(f, s)
+               : type == FG_F16 ? launch_few<__half>(f, s)
+               : type == FG_BF16 ? launch_few<__nv_bfloat16>(f, s)
+                                 : launch_few<__nv_fp8_e4m3>(f, s);
+    }
     const WeightLayout layout(d_w, w_group, w_out, w_in, groups, inner, outer, type);
     const int64_t need = fg_grouped_matmul_workspace(d_x, ldx, d_w, w_group, w_out, w_in, d_order, num_rows, groups, inner, outer, type);
     if (workspace_bytes < need || (need && !d_workspace)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_grouped_matmul_workspace()");
@@ -713,16 +969,20 @@ int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, con
         if (int rc = pack(d_w, w_group, step, b_mn ? w_out : w_in, layout.count, layout.rows, layout.cols, nullptr, 1, 0, type, &work, s)) return rc;
     }
     const int64_t units = num_rows / kTileRows + (groups < num_rows ? groups : num_rows);
-    const int bn = tile_width(units, outer, type), chunk = type == FG_E4M3 ? 128 : 64;
+    const int box_rows = type == FG_F32 || num_rows > 32 ? kTileRows : num_rows <= 8 ? 8 : num_rows <= 16 ? 16 : 32;
+    // half a tile of each group is empty on average
+    const int64_t expected = num_rows / kTileRows + groups / 2, expected_pairs = num_rows / (2 * kTileRows) + groups / 2;
+    const bool paired = pairs_pay(expected, expected_pairs, outer, type);
+    const int bn = box_rows <= 32 ? 64 : paired ? 512 : tile_width(units, outer, type), chunk = type == FG_E4M3 ? 128 : 64;
     CUtensorMap map_x, map_w;
-    if (int rc = make_map(&map_x, x, chunk, kTileRows)) return rc;
-    if (int rc = make_map(&map_w, w, chunk, b_mn ? 64 : bn)) return rc;
+    if (int rc = make_map(&map_x, x, chunk, box_rows)) return rc;
+    if (int rc = make_map(&map_w, w, chunk, b_mn ? 64 : paired ? 128 : bn)) return rc;
     MmaArgs a{};
     a.offsets = d_offsets, a.order = d_order, a.x_scales = d_x_scales, a.w_scales = d_w_scales, a.y = d_y;
     a.m = num_rows, a.x_rows = x_rows, a.choices = choices, a.groups = groups, a.inner = inner, a.outer = outer;
     a.type = type, a.out_type = out_type, a.format = w.type == FG_BF16 ? 1 : 0;
-    a.b_mn = b_mn, a.shared_weight = w_group == 0;
-    const int64_t tiles = units * ((outer + bn - 1) / bn);
+    a.b_mn = b_mn, a.shared_weight = w_group == 0, a.box_rows = box_rows;
+    const int64_t tiles = units * ((outer + (paired ? 256 : bn) - 1) / (paired ? 256 : bn));
     return type == FG_E4M3  ? launch<kEight, false>(bn, a, map_x, map_w, tiles, s)
            : type == FG_F32 ? launch<kParts, false>(bn, a, map_x, map_w, tiles, s)
                             : launch<kHalf, false>(bn, a, map_x, map_w, tiles, s);
@@ -765,13 +1025,16 @@ int fg_grouped_matmul_wgrad(const void* d_x, int64_t ldx, const void* d_dy, int6
     if (int rc = make_map(&map_dy, dy, 64, 64)) return rc;
     if (int rc = make_map(&map_x, x, 64, 64)) return rc;
     const int64_t units = split ? num_rows / split + groups : groups, rows_tiles = (outer + kTileRows - 1) / kTileRows;
-    const int bn = tile_width(units * rows_tiles, inner, type);
+    // in pairs, the columns' waste counts as well as the rows'
+    const int64_t singles = units * rows_tiles * ((inner + 127) / 128), doubles = units * ((outer + 255) / 256) * ((inner + 255) / 256);
+    const bool paired = pairs_pay(singles, doubles * 2, 256, type);
+    const int bn = paired ? 512 : tile_width(units * rows_tiles, inner, type);
     MmaArgs a{};
     a.offsets = d_offsets, a.order = d_order, a.y = split ? static_cast<void*>(sums) : d_dw;
     a.m = num_rows, a.x_rows = x_rows, a.choices = choices, a.groups = groups, a.inner = inner, a.outer = outer;
     a.type = type, a.out_type = split ? FG_F32 : type, a.format = dy.type == FG_BF16 ? 1 : 0;
     a.split = (int32_t)split, a.units = (int32_t)units;
-    const int64_t tiles = units * rows_tiles * ((inner + bn - 1) / bn);
+    const int64_t tiles = paired ? doubles : units * rows_tiles * ((inner + bn - 1) / bn);
     if (int rc = type == FG_F32 ? launch<kParts, true>(bn, a, map_dy, map_x, tiles, s) : launch<kHalf, true>(bn, a, map_dy, map_x, tiles, s)) return rc;
     if (split) {
         const dim3 grid((unsigned)((cells + 255) / 256 < 4096 ? (cells + 255) / 256 : 4096), (unsigned)groups);

@@ -19,23 +19,32 @@ __device__ __forceinline__ void barrier_arrive(uint32_t bar) {
 __device__ __forceinline__ void barrier_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+template <bool CLUSTER>
 __device__ __forceinline__ bool barrier_try(uint32_t bar, uint32_t parity) {
     uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
-        : "=r"(done)
-        : "r"(bar), "r"(parity)
-        : "memory");
+    if (CLUSTER)  // arrivals may come from the other block of a pair
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.b32 %0, 1, 0, p;\n}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
     return done != 0;
 }
 
 // Every wait ends: after about four seconds (at 2 GHz) it raises the block's `stop` word and gives up, and so does every
 // other wait of the block that sees the word.  `ignore_stop`: the last waits for copies in flight.
 constexpr long long kWaitClocks = 8ll << 30;
+template <bool CLUSTER = false>
 __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, volatile int* stop, bool ignore_stop = false) {
-    if (barrier_try(bar, parity)) return true;
+    if (barrier_try<CLUSTER>(bar, parity)) return true;
     const long long start = clock64();
-    while (!barrier_try(bar, parity)) {
+    while (!barrier_try<CLUSTER>(bar, parity)) {
         if ((*stop && !ignore_stop) || clock64() - start > kWaitClocks) {
             *stop = 1;
             return false;
@@ -44,26 +53,76 @@ __device__ __forceinline__ bool barrier_wait(uint32_t bar, uint32_t parity, vola
     return true;
 }
 
-__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-                 "l"(map), "r"(x), "r"(y), "r"(bar)
-                 : "memory");
+// ---- pairs of blocks (clusters of two) ----
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
 }
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Arrives at block `rank`'s barrier of the same address.  The release at cluster scope takes over a thousand cycles: once
+// an output tile, not once a stage.
+__device__ __forceinline__ void barrier_arrive_at(uint32_t bar, uint32_t rank) {
     asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}" ::"r"(bar), "r"(rank)
         : "memory");
+}
+
+// Tile loads into this block's shared memory.  In a pair both blocks' loads count on the first one's barrier (the second
+// block's bit of a cluster address cleared).
+template <int BLOCKS>
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+    if (BLOCKS == 2)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                     "l"(map), "r"(x), "r"(y), "r"(bar & 0xfeffffffu)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                     "l"(map), "r"(x), "r"(y), "r"(bar)
+                     : "memory");
+}
+template <int BLOCKS>
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
+    if (BLOCKS == 2)
+        asm volatile(
+            "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar & 0xfeffffffu)
+            : "memory");
+    else
+        asm volatile(
+            "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+            "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+            : "memory");
 }
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
-// ---- tensor memory ----
-__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t columns) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+// True in one lane of the (converged) warp, the same every time.  Copies and products are issued under it: their operands
+// sit in uniform registers, and only under elect.sync does the compiler know that one thread is left.  Under
+// `lane == 0` it wraps each of them in a loop over the active lanes.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.b32 %0, 1, 0, p;\n}" : "=r"(one));
+    return one != 0;
 }
+
+// ---- tensor memory ----
+// (a pair allocates, multiplies and frees together: cta_group::2)
+template <int BLOCKS>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t columns) {
+    if (BLOCKS == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+}
+template <int BLOCKS>
 __device__ __forceinline__ void tmem_free(uint32_t address, uint32_t columns) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
+    if (BLOCKS == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
+    else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
 }
 __device__ __forceinline__ void tcgen05_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -95,21 +154,30 @@ __device__ __forceinline__ uint64_t operand_descriptor(uint32_t address, uint32_
 __host__ __device__ constexpr uint32_t product_descriptor(uint32_t format, bool a_mn, bool b_mn, uint32_t m, uint32_t n) {
     return (1u << 4) | (format << 7) | (format << 10) | ((a_mn ? 1u : 0u) << 15) | ((b_mn ? 1u : 0u) << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
 }
-template <bool EIGHT>
+#define FG_PRODUCT(group, kind)                                                                                                       \
+    asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::" group ".kind::" kind " [%0], %1, %2, %3, p;\n}" ::"r"( \
+                     acc),                                                                                                           \
+                 "l"(a), "l"(b), "r"(descriptor), "r"((uint32_t)add)                                                                 \
+                 : "memory")
+template <int BLOCKS, bool EIGHT>
 __device__ __forceinline__ void product_step(uint32_t acc, uint64_t a, uint64_t b, uint32_t descriptor, bool add) {
-    if (EIGHT)
-        asm volatile(
-            "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}" ::"r"(acc), "l"(a), "l"(b),
-            "r"(descriptor), "r"((uint32_t)add)
-            : "memory");
-    else
-        asm volatile("{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(acc), "l"(a),
-                     "l"(b), "r"(descriptor), "r"((uint32_t)add)
-                     : "memory");
+    if (BLOCKS == 2) {
+        if (EIGHT) FG_PRODUCT("2", "f8f6f4");
+        else FG_PRODUCT("2", "f16");
+    } else {
+        if (EIGHT) FG_PRODUCT("1", "f8f6f4");
+        else FG_PRODUCT("1", "f16");
+    }
 }
-// Arrives at `bar` when all products issued so far by this thread are done.
+#undef FG_PRODUCT
+// Arrives at `bar` (of both blocks of a pair) when all products issued so far by this thread are done.
+template <int BLOCKS>
 __device__ __forceinline__ void product_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+    if (BLOCKS == 2)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 }  // namespace fg
