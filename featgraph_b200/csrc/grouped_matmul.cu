@@ -5,8 +5,8 @@
 // the device only, so a launch covers every way they can fall: persistent blocks, one an SM, scan the offsets into
 // shared memory once (a microsecond) and walk a numbering of 128-row tiles that never span two groups.
 //
-// A block is six warps.  Warp 0 loads: 128-byte wide tiles of both operands through TMA into a ring of stages.  Warp 1 issues tcgen05 products of 128 x BN x 32 bytes into one of two accumulators in tensor memory.  Warps
-// 2 to 5 take a finished accumulator to the output while the other one fills.
+// A block is ten warps.  Warp 0 loads: 128-byte wide tiles of both operands through TMA into a ring of stages.  Warp 1 issues tcgen05 products of 128 x BN x 32 bytes into one of two accumulators in tensor memory.  Warps
+// 2 to 9 take a finished accumulator to the output while the other one fills.
 //
 // Rows of a tile beyond its group's end belong to the next group (or to nothing): in y they are computed and not
 // stored.  In dW they would be terms of the sum, so they are overwritten with zeros in shared memory, in both
@@ -73,90 +73,90 @@ struct Shape {
     static constexpr int kStageBytes = kParts * (kA + kB);
     static constexpr int kStages = 196608 / kStageBytes < 16 ? 196608 / kStageBytes : 16;
     static constexpr int kColumns = 2 * BN;
-    static constexpr int kStaging = kStages * kStageBytes;  // 4 KB for each output warp
-    static constexpr int kSmem = 1024 + kStaging + 4 * 4096;
+    static constexpr int kStaging = kStages * kStageBytes;  // 2 KB for each output warp
+    static constexpr int kSmem = 1024 + kStaging + 8 * 2048;
 };
 
 struct Tables {
-    uint64_t full[16], empty[16], filled[2], drained[2], ask, tail, last;
+    uint64_t full[16], empty[16], tail[16], filled[2], drained[2], last;
     uint32_t tmem;
     int stop;
-    int warp_sums[8];
+    int warp_sums[11];
     int start[kMaxGroups + 1];  // first slot of each group
     int tiles[kMaxGroups + 1];  // row tiles (partial sums of dW) before each group
 };
 
 // Takes a warp's 32 rows of an accumulator, from `tmem` on, to the output rows from `out` on (row pitch `width`; rows >=
-// `rows` and columns >= `left` are not stored).  A thread holds a row in tensor memory's layout, so 128-byte wide pieces go
-// through the warp's 4 KB of shared memory (16-byte cells, XOR-swizzled: no bank conflicts either way) and leave as whole
-// 128-byte lines, 8 lanes a row.  Stored straight from the threads, 16 bytes in each of 32 rows at a time, the output
-// of a 65536 x 4096 product kept the products waiting.
+// `rows` and columns >= `left` are not stored): every second 64-byte wide piece of the BN columns, the warp's partner takes
+// the others.  A thread holds a row in tensor memory's layout, so the pieces go through the warp's 2 KB of shared memory
+// (16-byte cells, XOR-swizzled: no bank conflicts either way) and leave as whole sectors, 4 lanes a row.  Stored
+// straight from the threads, 16 bytes in each of 32 rows at a time, or by four warps instead of eight, the output of
+// products with a short inner axis keeps the tensor cores waiting.
 template <typename O, int BN, bool EIGHT>
 __device__ __forceinline__ void store_rows(uint32_t tmem, bool filled, O* out, int64_t width, int rows, int left, bool vector, uint32_t staging,
-                                           float scale, const float* column_scales) {
-    constexpr int kCols = 128 / sizeof(O), kCells = 16 / sizeof(O);
+                                           int half, float scale, const float* column_scales) {
+    constexpr int kCols = 64 / sizeof(O), kCells = 16 / sizeof(O);
     const int lane = threadIdx.x & 31;
-    for (int c = 0; c < BN; c += kCols, left -= kCols) {
-        if (left <= 0) break;
-        uint32_t raw[kCols / 32][32];
+    for (int c = half * kCols; c < BN; c += 2 * kCols) {
+        const int rest = left - c;
+        if (rest <= 0) break;
+        uint32_t raw[kCols];
         if (filled) {
-#pragma unroll
-            for (int h = 0; h < kCols / 32; ++h) fg::tmem_load_32(tmem + c + h * 32, raw[h]);
+            fg::tmem_load<kCols>(tmem + c, raw);
             fg::tmem_load_wait();
         } else {
 #pragma unroll
-            for (int j = 0; j < kCols; ++j) raw[j / 32][j % 32] = 0;
+            for (int j = 0; j < kCols; ++j) raw[j] = 0;
         }
 #pragma unroll
-        for (int q = 0; q < 8; ++q) {
+        for (int q = 0; q < 4; ++q) {
             Pack<O, kCells> p;
 #pragma unroll
             for (int j = 0; j < kCells; ++j) {
                 const int k = q * kCells + j;
-                float v = __uint_as_float(raw[k / 32][k % 32]);
-                if (EIGHT) v = __fmul_rn(__fmul_rn(v, scale), k < left ? column_scales[c + k] : 0.0f);
+                float v = __uint_as_float(raw[k]);
+                if (EIGHT) v = __fmul_rn(__fmul_rn(v, scale), k < rest ? column_scales[c + k] : 0.0f);
                 p.v[j] = from_f32<O>(v);
             }
             const uint32_t* word = reinterpret_cast<const uint32_t*>(&p);
-            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 128 + ((q ^ (lane & 7)) << 4)), "r"(word[0]), "r"(word[1]),
-                         "r"(word[2]), "r"(word[3])
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)), "r"(word[0]),
+                         "r"(word[1]), "r"(word[2]), "r"(word[3])
                          : "memory");
         }
         __syncwarp();
         if (vector) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = i * 4 + (lane >> 3), q = lane & 7;
+            for (int i = 0; i < 4; ++i) {
+                const int r = i * 8 + (lane >> 2), q = lane & 3;
                 Pack<uint32_t, 4> p;
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
                              : "=r"(p.v[0]), "=r"(p.v[1]), "=r"(p.v[2]), "=r"(p.v[3])
-                             : "r"(staging + r * 128 + ((q ^ (r & 7)) << 4))
+                             : "r"(staging + r * 64 + ((q ^ ((r >> 1) & 3)) << 4))
                              : "memory");
-                if (r < rows && q * kCells < left) store_pack<uint32_t, 4>(reinterpret_cast<uint32_t*>(out + r * width + c + q * kCells), p);
+                if (r < rows && q * kCells < rest) store_pack<uint32_t, 4>(reinterpret_cast<uint32_t*>(out + r * width + c + q * kCells), p);
             }
         } else {
-            for (int r = 0; r < min(rows, 32); ++r)
-#pragma unroll
-                for (int k = lane; k < kCols; k += 32) {
-                    const uint32_t at = staging + r * 128 + (((k / kCells) ^ (r & 7)) << 4) + (k % kCells) * sizeof(O);
-                    O v;
-                    if constexpr (sizeof(O) == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(*reinterpret_cast<uint32_t*>(&v)) : "r"(at) : "memory");
-                    else asm volatile("ld.shared.b16 %0, [%1];" : "=h"(*reinterpret_cast<uint16_t*>(&v)) : "r"(at) : "memory");
-                    if (k < left) out[r * width + c + k] = v;
-                }
+            constexpr int kAtOnce = 32 / kCols;  // rows side by side
+            for (int r = lane / kCols; r < min(rows, 32); r += kAtOnce) {
+                const int k = lane % kCols;
+                const uint32_t at = staging + r * 64 + (((k / kCells) ^ ((r >> 1) & 3)) << 4) + (k % kCells) * sizeof(O);
+                O v;
+                if constexpr (sizeof(O) == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(*reinterpret_cast<uint32_t*>(&v)) : "r"(at) : "memory");
+                else asm volatile("ld.shared.b16 %0, [%1];" : "=h"(*reinterpret_cast<uint16_t*>(&v)) : "r"(at) : "memory");
+                if (k < rest) out[r * width + c + k] = v;
+            }
         }
         __syncwarp();
     }
 }
 
 // A wait of all lanes, with one answer for all of them.
-template <bool CLUSTER = false>
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop) {
-    return __all_sync(0xffffffffu, fg::barrier_wait<CLUSTER>(bar, parity, stop));
+    return __all_sync(0xffffffffu, fg::barrier_wait(bar, parity, stop));
 }
 
 template <bool WGRAD>
-constexpr int kThreads = WGRAD ? 224 : 192;
+constexpr int kThreads = WGRAD ? 352 : 320;
 
 template <int BN, Kind KIND, bool WGRAD, bool FEW, int BLOCKS>
 __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
@@ -173,15 +173,14 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < S::kStages; ++s) {
-            fg::barrier_init(fg::smem_address(&t.full[s]), 1);
+            fg::barrier_init(fg::smem_address(&t.full[s]), BLOCKS);
+            fg::barrier_init(fg::smem_address(&t.tail[s]), 1);
             fg::barrier_init(fg::smem_address(&t.empty[s]), 1);
         }
         for (int s = 0; s < 2; ++s) {
             fg::barrier_init(fg::smem_address(&t.filled[s]), 1);
-            fg::barrier_init(fg::smem_address(&t.drained[s]), 4 * BLOCKS);
+            fg::barrier_init(fg::smem_address(&t.drained[s]), 8 * BLOCKS);
         }
-        fg::barrier_init(fg::smem_address(&t.ask), 1);
-        fg::barrier_init(fg::smem_address(&t.tail), BLOCKS);
         fg::barrier_init(fg::smem_address(&t.last), 1);
         fg::barrier_init_fence();
         t.stop = 0;
@@ -240,6 +239,7 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
     struct Tile {
         int group, unit, row, col;
         int begin, end, chunks;
+        __device__ bool ragged() const { return (end - begin) % 16 != 0; }
     };
     int cursor = 0;
     auto locate = [&](int64_t index) {
@@ -274,6 +274,7 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
     if (warp == 0) {
         if (fg::elect_one()) {
             int64_t step = 0;  // stages filled so far
+            uint32_t tail_now = 0, tail_parity = 0;  // a bit a stage: holds a tail; parity of its next tail
             bool live = true;
             for (int64_t i = start; live && i < total; i += stride) {
                 const Tile w = locate(i);
@@ -284,52 +285,73 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
                     return WGRAD || a.b_mn ? max(min(S::kOwnCols / 64, ((WGRAD ? a.inner : a.outer) - at + 63) / 64), 0) : S::kOwnCols / 64;
                 };
                 const int a_blocks = blocks_a(w.row), b_blocks = blocks_b(col);
-                uint32_t bytes = ((WGRAD ? a_blocks * 8192 : a.box_rows * kChunkBytes) + b_blocks * 8192) * S::kParts;
+                const uint32_t own = ((WGRAD ? a_blocks * 8192 : a.box_rows * kChunkBytes) + b_blocks * 8192) * S::kParts;
+                uint32_t bytes = own;
                 if (BLOCKS == 2)  // the first block's barrier counts the second one's loads too
                     bytes += ((WGRAD ? blocks_a(w.row + kTileRows) * 8192 : a.box_rows * kChunkBytes) + blocks_b(col + S::kOwnCols) * 8192) * S::kParts;
                 for (int c = 0; c < w.chunks; ++c, ++step) {
                     const int s = (int)(step % S::kStages);
-                    const uint32_t bar = fg::smem_address(&t.full[s]), stage = ring + s * S::kStageBytes;
+                    const uint32_t full = fg::smem_address(&t.full[s]), stage = ring + s * S::kStageBytes;
                     if (step >= S::kStages && !fg::barrier_wait(fg::smem_address(&t.empty[s]), (step / S::kStages - 1) & 1, stop)) {
                         live = false;
                         break;
                     }
-                    if (rank == 0) fg::barrier_expect(bar, bytes);
                     const int k = c * kChunk;
+                    if (WGRAD && c == w.chunks - 1 && w.ragged()) {  // goes through the warp that clears it, each block's own
+                        const uint32_t bar = fg::smem_address(&t.tail[s]);
+                        tail_now |= 1u << s;
+                        tail_parity ^= 1u << s;
+                        fg::barrier_expect(bar, own);
+#pragma unroll
+                        for (int p = 0; p < S::kParts; ++p) {
+                            const uint32_t at = stage + p * S::kA, bt = stage + S::kParts * S::kA + p * S::kB;
+                            const int slot = w.begin + k + p * (int)a.m;
+                            for (int q = 0; q < a_blocks; ++q) fg::tma_load_2d<1>(at + q * 8192, &map_a, w.row + q * 64, slot, bar);
+                            for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d<1>(bt + q * 8192, &map_b, col + q * 64, slot, bar);
+                        }
+                        continue;
+                    }
+                    tail_now &= ~(1u << s);
+                    if (rank == 0) {
+                        fg::barrier_expect(full, bytes);
+                        if (BLOCKS == 2) fg::barrier_arrive(full);  // two arrivals: those of the clearing warps, for a tail
+                    }
 #pragma unroll
                     for (int p = 0; p < S::kParts; ++p) {
                         const uint32_t at = stage + p * S::kA, bt = stage + S::kParts * S::kA + p * S::kB;
                         if (WGRAD) {  // 64 slots by 64 columns a block
                             const int slot = w.begin + k + p * (int)a.m;
-                            for (int q = 0; q < a_blocks; ++q) fg::tma_load_2d<BLOCKS>(at + q * 8192, &map_a, w.row + q * 64, slot, bar);
-                            for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d<BLOCKS>(bt + q * 8192, &map_b, col + q * 64, slot, bar);
+                            for (int q = 0; q < a_blocks; ++q) fg::tma_load_2d<BLOCKS>(at + q * 8192, &map_a, w.row + q * 64, slot, full);
+                            for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d<BLOCKS>(bt + q * 8192, &map_b, col + q * 64, slot, full);
                         } else {
                             const int g = a.shared_weight ? p : w.group + p * a.groups;
-                            fg::tma_load_2d<BLOCKS>(at, &map_a, k, w.begin + p * (int)a.m, bar);
+                            fg::tma_load_2d<BLOCKS>(at, &map_a, k, w.begin + p * (int)a.m, full);
                             if (!a.b_mn) {
-                                fg::tma_load_3d<BLOCKS>(bt, &map_b, k, col, g, bar);
+                                fg::tma_load_3d<BLOCKS>(bt, &map_b, k, col, g, full);
                             } else {
-                                for (int q = 0; q < b_blocks; ++q) fg::tma_load_3d<BLOCKS>(bt + q * 8192, &map_b, col + q * 64, k, g, bar);
+                                for (int q = 0; q < b_blocks; ++q) fg::tma_load_3d<BLOCKS>(bt + q * 8192, &map_b, col + q * 64, k, g, full);
                             }
                         }
                     }
                 }
             }
-            if (*stop && rank == 0)  // no copy may be in flight when the block (or its pair) ends
-                for (int64_t q = max(step - S::kStages, (int64_t)0); q < step; ++q)
-                    fg::barrier_wait(fg::smem_address(&t.full[q % S::kStages]), (q / S::kStages) & 1, stop, true);
+            if (*stop)  // no copy may be in flight when the block (or its pair) ends
+                for (int64_t q = max(step - S::kStages, (int64_t)0); q < step; ++q) {
+                    const int s = (int)(q % S::kStages);
+                    if (tail_now >> s & 1) fg::barrier_wait(fg::smem_address(&t.tail[s]), ~tail_parity >> s & 1, stop, true);
+                    else if (rank == 0) fg::barrier_wait(fg::smem_address(&t.full[s]), (q / S::kStages) & 1, stop, true);
+                }
         }
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0 && fg::elect_one()) {
-            int64_t step = 0, turn = 0, tails = 0;
+            int64_t step = 0, turn = 0;
             const uint32_t descriptor = fg::product_descriptor(a.format, WGRAD, WGRAD || a.b_mn, kRows, BN);
             const bool b_mn = WGRAD || a.b_mn;
             bool live = true;
             for (int64_t i = start; live && i < total; i += stride) {
                 const Tile w = locate(i);
                 if (w.chunks == 0) continue;  // an empty group's dW: nothing to add up
-                const bool tail = WGRAD && (w.end - w.begin) % kChunk != 0;
                 const int buffer = (int)(turn & 1);
                 const uint32_t acc = tmem + buffer * BN;
                 if (turn >= 2 && !fg::barrier_wait<BLOCKS == 2>(fg::smem_address(&t.drained[buffer]), (turn / 2 - 1) & 1, stop)) break;
@@ -337,14 +359,11 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
                 for (int c = 0; c < w.chunks; ++c, ++step) {
                     const int s = (int)(step % S::kStages);
                     const uint32_t stage = ring + s * S::kStageBytes, parity = (step / S::kStages) & 1;
-                    live = fg::barrier_wait(fg::smem_address(&t.full[s]), parity, stop);
-                    if (live && tail && c == w.chunks - 1) {
-                        fg::barrier_arrive(fg::smem_address(&t.ask));
-                        if (BLOCKS == 2) fg::barrier_arrive_at(fg::smem_address(&t.ask), 1);
-                        live = fg::barrier_wait<BLOCKS == 2>(fg::smem_address(&t.tail), tails++ & 1, stop);
-                    }
+                    live = fg::barrier_wait<BLOCKS == 2 && WGRAD>(fg::smem_address(&t.full[s]), parity, stop);
                     if (!live) break;
                     fg::tcgen05_after_sync();
+                    // of a group's last chunk only the steps that have rows of it
+                    const int steps = WGRAD && c == w.chunks - 1 ? (w.end - w.begin - c * kChunk + 15) / 16 : 4;
 #pragma unroll
                     for (int pair = S::kParts == 3 ? 0 : 5; pair < 6; ++pair) {
                         const uint32_t at = stage + part_a(pair) * S::kA, bt = stage + S::kParts * S::kA + part_b(pair) * S::kB;
@@ -352,7 +371,7 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
                         for (int k = 0; k < 4; ++k) {
                             const uint64_t da = WGRAD ? fg::operand_descriptor(at + k * 2048, 8192, 1024) : fg::operand_descriptor(at + k * 32, 16, 1024);
                             const uint64_t db = b_mn ? fg::operand_descriptor(bt + k * 2048, 8192, 1024) : fg::operand_descriptor(bt + k * 32, 16, 1024);
-                            fg::product_step<BLOCKS, EIGHT>(acc, da, db, descriptor, c > 0 || pair > (S::kParts == 3 ? 0 : 5) || k > 0);
+                            if (!WGRAD || k < steps) fg::product_step<BLOCKS, EIGHT>(acc, da, db, descriptor, c > 0 || pair > (S::kParts == 3 ? 0 : 5) || k > 0);
                         }
                     }
                     fg::product_commit<BLOCKS>(fg::smem_address(&t.empty[s]));
@@ -367,32 +386,35 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
             }
         }
         __syncwarp();
-    } else if (WGRAD && warp == 6) {
-        // The rows of a group's last chunk that are not its own become zeros, on being asked once the chunk is there: 128
+    } else if (WGRAD && warp == 10) {
+        // In a group's last chunk, the rows that are not its own become zeros, as far as the last step of 16 reaches: 128
         // bytes a row, 64 rows a column block.
-        int64_t step = 0, tails = 0;
+        int64_t step = 0;
+        uint32_t tail_parity = 0;
         for (int64_t i = start; i < total; i += stride) {
             const Tile w = locate(i);
             step += w.chunks;
-            const int keep = (w.end - w.begin) % kChunk;
-            if (w.chunks == 0 || keep == 0) continue;
-            const int s = (int)((step - 1) % S::kStages);
+            if (w.chunks == 0 || !w.ragged()) continue;
+            const int s = (int)((step - 1) % S::kStages), keep = (w.end - w.begin - 1) % kChunk + 1, upto = (keep + 15) / 16 * 16;
             const uint32_t stage = ring + s * S::kStageBytes;
-            if (!warp_wait<BLOCKS == 2>(fg::smem_address(&t.ask), tails++ & 1, stop)) break;
-            for (int q = 0; q < S::kStageBytes / 8192; ++q)
-                for (int z = keep * 8 + lane; z < 64 * 8; z += 32)
+            if (!warp_wait(fg::smem_address(&t.tail[s]), tail_parity >> s & 1, stop)) break;
+            tail_parity ^= 1u << s;
+            for (int z = keep * 8 + lane; z < upto * 8; z += 32)
+#pragma unroll
+                for (int q = 0; q < S::kStageBytes / 8192; ++q)
                     asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(stage + q * 8192 + z * 16), "r"(0) : "memory");
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                if (BLOCKS == 2) fg::barrier_arrive_at(fg::smem_address(&t.tail), 0);
-                else fg::barrier_arrive(fg::smem_address(&t.tail));
+                if (BLOCKS == 2) fg::barrier_arrive_at(fg::smem_address(&t.full[s]), 0);
+                else fg::barrier_arrive(fg::smem_address(&t.full[s]));
             }
             __syncwarp();
         }
     } else {
         const int quarter = warp & 3;  // the lanes of tensor memory this warp can read
-        const uint32_t staging = ring + S::kStaging + quarter * 4096;
+        const int half = (warp - 2) >> 2;
+        const uint32_t staging = ring + S::kStaging + (warp - 2) * 2048;
         const int width = WGRAD ? a.inner : a.outer;
         const int size = a.out_type == FG_F32 ? 4 : 2;
         const bool vector = (int64_t)width * size % 16 == 0 && ((uintptr_t)a.y & 15) == 0;
@@ -420,11 +442,11 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
             const uint32_t acc = tmem + ((uint32_t)above << 16) + buffer * BN;
             const int64_t at = first * width + w.col;
             if (a.out_type == FG_F32)
-                store_rows<float, BN, EIGHT>(acc, w.chunks > 0, static_cast<float*>(a.y) + at, width, rows, width - w.col, vector, staging, scale, column_scales);
+                store_rows<float, BN, EIGHT>(acc, w.chunks > 0, static_cast<float*>(a.y) + at, width, rows, width - w.col, vector, staging, half, scale, column_scales);
             else if (a.out_type == FG_F16)
-                store_rows<__half, BN, EIGHT>(acc, w.chunks > 0, static_cast<__half*>(a.y) + at, width, rows, width - w.col, vector, staging, scale, column_scales);
+                store_rows<__half, BN, EIGHT>(acc, w.chunks > 0, static_cast<__half*>(a.y) + at, width, rows, width - w.col, vector, staging, half, scale, column_scales);
             else
-                store_rows<__nv_bfloat16, BN, EIGHT>(acc, w.chunks > 0, static_cast<__nv_bfloat16*>(a.y) + at, width, rows, width - w.col, vector, staging, scale,
+                store_rows<__nv_bfloat16, BN, EIGHT>(acc, w.chunks > 0, static_cast<__nv_bfloat16*>(a.y) + at, width, rows, width - w.col, vector, staging, half, scale,
                                                      column_scales);
             if (w.chunks) {
                 fg::tcgen05_before_sync();
@@ -438,7 +460,7 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
         }
         if (!WGRAD) {  // rows in no group
             const int64_t from = (int64_t)t.start[a.groups] * a.outer, values = a.m * a.outer;
-            for (int64_t i = from + (int64_t)blockIdx.x * 128 + (threadIdx.x - 64); i < values; i += (int64_t)gridDim.x * 128) {
+            for (int64_t i = from + (int64_t)blockIdx.x * 256 + (threadIdx.x - 64); i < values; i += (int64_t)gridDim.x * 256) {
                 if (a.out_type == FG_F32) static_cast<float*>(a.y)[i] = 0.0f;
                 else static_cast<uint16_t*>(a.y)[i] = 0;
             }
@@ -738,8 +760,17 @@ int make_map(CUtensorMap* map, const Matrix& m, int box_cols, int box_rows) {
     const cuuint64_t strides[2] = {(cuuint64_t)(m.pitch * size), (cuuint64_t)(m.group_stride * size)};
     const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
     const CUtensorMapDataType type = m.type == FG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : m.type == FG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    const CUresult rc = encode(map, type, m.groups ? 3 : 2, const_cast<void*>(m.data), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    auto run = [&] {
+        return encode(map, type, m.groups ? 3 : 2, const_cast<void*>(m.data), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    };
+    CUresult rc = run();
+    if (rc == CUDA_ERROR_INVALID_CONTEXT) {  // a host thread's first CUDA call (an autograd thread's): bind the device's context
+        int device = 0;
+        FG_CUDA_TRY(cudaGetDevice(&device));
+        FG_CUDA_TRY(cudaSetDevice(device));
+        rc = run();
+    }
     if (rc != CUDA_SUCCESS) return fg::fail(FG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)rc);
     return FG_OK;
 }

@@ -127,8 +127,20 @@ __device__ __forceinline__ void tmem_free(uint32_t address, uint32_t columns) {
 __device__ __forceinline__ void tcgen05_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tcgen05_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
-// 32 lanes (this warp's quarter) x 32 columns: thread = lane, register = column.
-__device__ __forceinline__ void tmem_load_32(uint32_t address, uint32_t (&r)[32]) {
+// 32 lanes (this warp's quarter) x 16 or 32 columns: thread = lane, register = column.
+template <int N>
+__device__ __forceinline__ void tmem_load(uint32_t address, uint32_t (&r)[N]);
+template <>
+__device__ __forceinline__ void tmem_load<16>(uint32_t address, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(address));
+}
+template <>
+__device__ __forceinline__ void tmem_load<32>(uint32_t address, uint32_t (&r)[32]) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
         "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "

@@ -427,6 +427,21 @@ def test_product_of_8_bit_rows(n, k, count, inner, outer, out):
     assert torch.equal(grouped_matmul(x, w, groups, gather=True).double(), grouped_matmul(x, odd, groups, gather=True).double())
 
 
+def test_product_from_a_thread_that_made_no_cuda_call_yet():
+    """A host thread has no CUDA context until its first runtime call; the tensor maps need one."""
+    import threading
+
+    from featgraph.module import grouped_matmul
+    groups = make_groups(200, 1, 2, 5)
+    x, w = normal((200, 64), 1, torch.bfloat16), normal((2, 64, 64), 2, torch.bfloat16)
+    want, got = grouped_matmul(x, w, groups), []
+    torch.cuda.synchronize()
+    thread = threading.Thread(target=lambda: got.append(grouped_matmul(x, w, groups)))
+    thread.start()
+    thread.join()
+    assert got and torch.equal(got[0], want)
+
+
 def test_product_has_the_same_bits_again():
     from featgraph.module import grouped_matmul
     for t in sorted(TYPES):
