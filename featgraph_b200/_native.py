@@ -56,7 +56,7 @@ SIGNATURES = {
     "fg_route_backward": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _vp]),
     "fg_group_rows_workspace": (_i64, [_i64, _i32]),
     "fg_group_rows": (ctypes.c_int, [_vp, _i64, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
-    "fg_grouped_matmul_status": (ctypes.c_int, [_vp]),
+    "fg_wait_status": (ctypes.c_int, [_vp]),
     "fg_grouped_matmul_workspace": (_i64, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i32, _i32, _i32, _i32]),
     "fg_grouped_matmul": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i64, _vp, _i64, _i32, _i32, _i32,
                                          _i32, _i32, _vp, _i64, _vp]),

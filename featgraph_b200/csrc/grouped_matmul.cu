@@ -36,7 +36,7 @@ using fg::to_f32;
 
 constexpr int kTileRows = 128, kChunkBytes = 128, kMaxGroups = 1024, kSuperRows = 16;
 
-__device__ int g_stuck;  // set when a wait ran out; fg_grouped_matmul_status reads it
+__device__ int g_stuck;  // set when a wait ran out; fg_wait_status reads it
 
 struct MmaArgs {
     const int32_t *offsets, *order;
@@ -940,12 +940,13 @@ int check_product(int64_t m, int64_t x_rows, int32_t choices, int32_t groups, in
 
 extern "C" {
 
-int fg_grouped_matmul_status(void* stream) {
-    int v = 0;
+int fg_wait_status(void* stream) {
+    int product = 0, norm = 0;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    FG_CUDA_TRY(cudaMemcpyFromSymbolAsync(&v, g_stuck, sizeof(v), 0, cudaMemcpyDeviceToHost, s));
+    FG_CUDA_TRY(cudaMemcpyFromSymbolAsync(&product, g_stuck, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
+    if (int rc = fg::norm_stuck(s, &norm)) return rc;
     FG_CUDA_TRY(cudaStreamSynchronize(s));
-    return v ? fg::fail(FG_ERR_CUDA, "a grouped product gave up waiting for its own copies") : FG_OK;
+    return product || norm ? fg::fail(FG_ERR_CUDA, "%s gave up waiting for its own copies", product ? "a grouped product" : "a norm's gradient") : FG_OK;
 }
 
 int64_t fg_grouped_matmul_workspace(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,

@@ -16,6 +16,7 @@
 #include <climits>
 
 #include "rows.cuh"
+#include "tcgen05.cuh"
 
 namespace {
 
@@ -25,7 +26,9 @@ using fg::Pack;
 using fg::store_pack;
 using fg::to_f32;
 
-constexpr int kE4M3Max = 448;
+constexpr int kE4M3Max = 448, kMaxStages = 8;
+
+__device__ int g_stuck;  // set when a wait for a copy ran out
 
 // Sum / maximum over the TPR threads of a row; `slot` picks a buffer so that two reductions in a row need no
 // barrier between them.
@@ -168,14 +171,22 @@ struct NormGradArgs {
     void* dx;
     float* partial;  // [gridDim.x, d], or NULL where the weight's gradient is not wanted
     int64_t ldh, lddy, lddh, n;
-    int32_t d;
+    int32_t d, stages, slot;  // slot: bytes of one array's row in shared memory
     float eps;
     bool weight_f32;
 };
 
+// Waits for the other threads of the row (named barriers where a block holds several rows of several warps).
+template <int TPR, int THREADS>
+__device__ __forceinline__ void row_sync(int sub) {
+    if (TPR == 32) __syncwarp();
+    else if (TPR == THREADS) __syncthreads();
+    else asm volatile("bar.sync %0, %1;" ::"r"(sub + 1), "n"(TPR) : "memory");
+}
+
 // Two sums over the TPR threads of a row, through one of two buffers in turn, so that a row needs one barrier.
-template <int TPR>
-__device__ __forceinline__ void row_sums(float& x, float& y, float2* buffer) {
+template <int TPR, int THREADS>
+__device__ __forceinline__ void row_sums(float& x, float& y, float2* buffer, int sub) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) {
         x = __fadd_rn(x, __shfl_xor_sync(0xffffffffu, x, o));
@@ -183,95 +194,135 @@ __device__ __forceinline__ void row_sums(float& x, float& y, float2* buffer) {
     }
     if (TPR == 32) return;
     constexpr int kWarps = TPR / 32;
-    const int first = (threadIdx.x / TPR) * kWarps;
     if ((threadIdx.x & 31) == 0) buffer[threadIdx.x >> 5] = make_float2(x, y);
-    __syncthreads();
-    const float2 v = buffer[first];
+    row_sync<TPR, THREADS>(sub);
+    const float2 v = buffer[sub * kWarps];
     x = v.x, y = v.y;
 #pragma unroll
     for (int i = 1; i < kWarps; ++i) {
-        const float2 w = buffer[first + i];
+        const float2 w = buffer[sub * kWarps + i];
         x = __fadd_rn(x, w.x), y = __fadd_rn(y, w.y);
     }
 }
 
-// Where a row is shared by several warps, the next row's values are requested before the current one's sums, so that loads
-// are in flight across the barrier (32768 x 4096 bf16 with dh: 325 -> 253 us).  A row of one warp meets no barrier, and
-// there the registers are worth more as warps (100003 x 331 fp32: 122 us without, 211 us with); rows of 1024 threads
-// have 64 registers a thread and no room.
-template <typename T, int VEC, int TPR, int E>
-__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(const NormGradArgs a) {
+// The TPR threads of a row walk the rows with a ring of `stages` rows in shared memory ahead of them, filled by bulk copies:
+// what is in flight does not take registers (with the next row in registers 16 warps an SM were left, and 32768 x
+// 4096 bf16 with dh took 253 us), and a row that starts off the 16-byte grid is copied from the grid point before it
+// on, up to 15 bytes more on either side in the 16-byte units that hold the row's first and last values.
+// A stage is free again as soon as its values are in registers, which the barrier of the sums shows.
+template <typename T, int VEC, int TPR, int E, bool DH>
+__global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR <= 256 ? 2 : 1) norm_grad_kernel(const NormGradArgs a) {
     constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR, NV = E / VEC;
+    extern __shared__ __align__(16) uint8_t ring[];
+    __shared__ uint64_t full[kRows][kMaxStages];
     __shared__ float2 buffer[2][kThreads / 32];
     __shared__ float across[kRows > 1 ? kRows * TPR * E : 1];
+    __shared__ int stop;
+    constexpr int arrays = DH ? 3 : 2;
     const int t = threadIdx.x % TPR, sub = threadIdx.x / TPR;
-    const int64_t step = (int64_t)gridDim.x * kRows;
-    float acc[E];
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-    struct Row {
-        Pack<T, VEC> h[NV], g[NV], d[NV];
+    const float over_d = __fdiv_rn(1.0f, (float)a.d);
+    const int64_t first = (int64_t)blockIdx.x * kRows + sub, step = (int64_t)gridDim.x * kRows;
+    const uint8_t* mine = ring + sub * a.stages * arrays * a.slot;
+    const uint32_t base = fg::smem_address(mine);
+    if (t == 0)
+        for (int s = 0; s < a.stages; ++s) fg::barrier_init(fg::smem_address(&full[sub][s]), 1);
+    if (threadIdx.x == 0) stop = 0;
+    fg::barrier_init_fence();
+    __syncthreads();
+    auto address = [&](int array, int64_t row) {
+        return array == 0   ? reinterpret_cast<uint64_t>(static_cast<const T*>(a.h) + row * a.ldh)
+               : array == 1 ? reinterpret_cast<uint64_t>(static_cast<const T*>(a.dy) + row * a.lddy)
+                            : reinterpret_cast<uint64_t>(static_cast<const T*>(a.dh) + row * a.lddh);
     };
-    auto request = [&](Row& r, int64_t row) {
-        const bool live = row < a.n;
-        const T* h = static_cast<const T*>(a.h) + (live ? row : 0) * a.ldh;
-        const T* dy = static_cast<const T*>(a.dy) + (live ? row : 0) * a.lddy;
-        const T* dh = static_cast<const T*>(a.dh) + (live ? row : 0) * a.lddh;
+    auto request = [&](int s, int64_t row) {  // one thread of the row
+        const uint32_t bar = fg::smem_address(&full[sub][s]);
+        uint32_t bytes = 0;
+        for (int q = 0; q < arrays; ++q) {
+            const uint64_t from = address(q, row), lo = from & ~15ull;
+            bytes += (uint32_t)(((from + (uint64_t)a.d * sizeof(T) + 15) & ~15ull) - lo);
+        }
+        fg::barrier_expect(bar, bytes);
+        for (int q = 0; q < arrays; ++q) {
+            const uint64_t from = address(q, row), lo = from & ~15ull;
+            fg::bulk_load(base + (s * arrays + q) * a.slot, lo, (uint32_t)(((from + (uint64_t)a.d * sizeof(T) + 15) & ~15ull) - lo), bar);
+        }
+    };
+    if (t == 0)
+        for (int s = 0; s < a.stages; ++s)
+            if (first + s * step < a.n) request(s, first + s * step);
+    float acc[E], weight[E];  // the thread's columns: the same for all rows
+#pragma unroll
+    for (int c = 0; c < NV; ++c)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            const int i = (c * TPR + t) * VEC + j;
+            acc[c * VEC + j] = 0.0f;
+            weight[c * VEC + j] = i < a.d ? weight_at(a.weight, a.weight_f32, i, T()) : 0.0f;
+        }
+    int s = 0, parity = 0, turn = 0;
+    for (int64_t row = first; row < a.n; row += step, turn ^= 1) {
+        fg::barrier_wait(fg::smem_address(&full[sub][s]), parity, &stop);  // without the copy: wrong values, and the flag
+        Pack<T, VEC> h[NV], g[NV], d[NV];
+        // where a row starts in its 16-byte unit; rows that are read in vectors start on the grid
+        const uint8_t* stage = mine + s * arrays * a.slot;
+        const T* hs = reinterpret_cast<const T*>(stage + (VEC == 1 ? (uint32_t)address(0, row) & 15 : 0));
+        const T* gs = reinterpret_cast<const T*>(stage + a.slot + (VEC == 1 ? (uint32_t)address(1, row) & 15 : 0));
+        const T* ds = reinterpret_cast<const T*>(stage + 2 * a.slot + (VEC == 1 && DH ? (uint32_t)address(2, row) & 15 : 0));
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
             const int i = (c * TPR + t) * VEC;
-            if (live && i < a.d) {
-                r.h[c] = load_pack<T, VEC>(h + i);
-                r.g[c] = load_pack<T, VEC>(dy + i);
-                if (a.dh != nullptr) r.d[c] = load_pack<T, VEC>(dh + i);
+            if (i < a.d) {
+                h[c] = load_pack<T, VEC>(hs + i);
+                g[c] = load_pack<T, VEC>(gs + i);
+                if (DH) d[c] = load_pack<T, VEC>(ds + i);
             }
         }
-    };
-    constexpr bool kAhead = VEC > 1 && TPR >= 64 && TPR <= 512;
-    Row now, next;
-    int turn = 0;
-    if (kAhead) request(now, (int64_t)blockIdx.x * kRows + sub);
-    for (int64_t base = (int64_t)blockIdx.x * kRows; base < a.n; base += step, turn ^= 1) {
-        const int64_t row = base + sub;
-        const bool live = row < a.n;
-        if (kAhead) request(next, row + step);
-        else request(now, row);
         float ss = 0.0f, sg = 0.0f;
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
             const int i = (c * TPR + t) * VEC;
-            if (live && i < a.d) {
+            if (i < a.d) {
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float u = to_f32<T>(now.h[c].v[j]);
-                    const float g = __fmul_rn(to_f32<T>(now.g[c].v[j]), weight_at(a.weight, a.weight_f32, i + j, T()));
+                    const float u = to_f32<T>(h[c].v[j]);
+                    const float v = __fmul_rn(to_f32<T>(g[c].v[j]), weight[c * VEC + j]);
                     ss = __fmaf_rn(u, u, ss);
-                    sg = __fmaf_rn(u, g, sg);
+                    sg = __fmaf_rn(u, v, sg);
                 }
             }
         }
-        row_sums<TPR>(ss, sg, buffer[turn]);
-        const float r = __frsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)a.d), a.eps));
-        const float along = __fmul_rn(__fmul_rn(r, r), __fmul_rn(r, __fdiv_rn(sg, (float)a.d)));
+        row_sums<TPR, kThreads>(ss, sg, buffer[turn], sub);
+        if (TPR == 32) __syncwarp();
+        if (t == 0 && row + a.stages * step < a.n) request(s, row + a.stages * step);
+        if (++s == a.stages) s = 0, parity ^= 1;
+        const float r = __frsqrt_rn(__fmaf_rn(ss, over_d, a.eps));
+        const float along = __fmul_rn(__fmul_rn(r, r), __fmul_rn(r, __fmul_rn(sg, over_d)));
         T* dx = static_cast<T*>(a.dx) + row * a.d;
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
             const int i = (c * TPR + t) * VEC;
-            if (live && i < a.d) {
+            if (i < a.d) {
                 Pack<T, VEC> o;
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
-                    const float u = to_f32<T>(now.h[c].v[j]), dyj = to_f32<T>(now.g[c].v[j]);
-                    const float g = __fmul_rn(dyj, weight_at(a.weight, a.weight_f32, i + j, T()));
-                    float v = __fmaf_rn(-u, along, __fmul_rn(r, g));
-                    if (a.dh != nullptr) v = __fadd_rn(v, to_f32<T>(now.d[c].v[j]));
-                    o.v[j] = from_f32<T>(v);
+                    const float u = to_f32<T>(h[c].v[j]), dyj = to_f32<T>(g[c].v[j]);
+                    const float v = __fmul_rn(dyj, weight[c * VEC + j]);
+                    float w = __fmaf_rn(-u, along, __fmul_rn(r, v));
+                    if (DH) w = __fadd_rn(w, to_f32<T>(d[c].v[j]));
+                    o.v[j] = from_f32<T>(w);
                     acc[c * VEC + j] = __fmaf_rn(dyj, __fmul_rn(u, r), acc[c * VEC + j]);
                 }
                 store_pack<T, VEC>(dx + i, o);
             }
         }
-        if (kAhead) now = next;
+    }
+    if (stop) {  // a wait ran out: the copies that are left end before the block does
+        if (t == 0)
+            for (int q = 0; q < a.stages; ++q) {
+                fg::barrier_wait(fg::smem_address(&full[sub][q]), 0, &stop, true);
+                fg::barrier_wait(fg::smem_address(&full[sub][q]), 1, &stop, true);
+            }
+        if (threadIdx.x == 0) atomicExch(&g_stuck, 1);
     }
     if (a.partial == nullptr) return;
     float* out = a.partial + (int64_t)blockIdx.x * a.d;
@@ -280,9 +331,9 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR) norm_grad_kernel(const 
         for (int e = 0; e < E; ++e) across[(sub * E + e) * TPR + t] = acc[e];
         __syncthreads();
         if (sub != 0) return;
-        for (int s = 1; s < kRows; ++s)
+        for (int q = 1; q < kRows; ++q)
 #pragma unroll
-            for (int e = 0; e < E; ++e) acc[e] = __fadd_rn(acc[e], across[(s * E + e) * TPR + t]);
+            for (int e = 0; e < E; ++e) acc[e] = __fadd_rn(acc[e], across[(q * E + e) * TPR + t]);
     }
 #pragma unroll
     for (int c = 0; c < NV; ++c) {
@@ -314,12 +365,11 @@ __global__ void __launch_bounds__(1024) weight_grad_kernel(const float* __restri
 
 constexpr int kMaxWidth = 16384;
 
-// Calls f.template operator()<T, VEC, TPR, E>() with the smallest TPR * E that covers d.  Single-value accesses cost an
-// address and a register each, so there a thread holds 8 values rather than 16 (100003 x 331 fp32, backward: 16 values a
-// thread leave 16 warps an SM, 122 us).
-template <typename T, int VEC, typename F>
+// Calls f.template operator()<T, VEC, TPR, E>() with the smallest TPR * E that covers d.  Single values straight from memory
+// cost an address and a register each, so there (SLIM) a thread holds 8 values rather than 16.
+template <typename T, int VEC, bool SLIM, typename F>
 void by_width(int d, F&& f) {
-    if constexpr (VEC == 1) {
+    if constexpr (SLIM) {
         if (d <= 256) f.template operator()<T, VEC, 32, 8>();
         else if (d <= 512) f.template operator()<T, VEC, 64, 8>();
         else if (d <= 1024) f.template operator()<T, VEC, 128, 8>();
@@ -337,15 +387,16 @@ void by_width(int d, F&& f) {
         else f.template operator()<T, VEC, 1024, 16>();
     }
 }
-template <typename F>
+template <bool SLIM, typename F>
 void by_type(int32_t type, bool vec, int d, F&& f) {
-    if (type == FG_F32) vec ? by_width<float, 4>(d, f) : by_width<float, 1>(d, f);
-    else if (type == FG_F16) vec ? by_width<__half, 8>(d, f) : by_width<__half, 1>(d, f);
-    else vec ? by_width<__nv_bfloat16, 8>(d, f) : by_width<__nv_bfloat16, 1>(d, f);
+    if (type == FG_F32) vec ? by_width<float, 4, false>(d, f) : by_width<float, 1, SLIM>(d, f);
+    else if (type == FG_F16) vec ? by_width<__half, 8, false>(d, f) : by_width<__half, 1, SLIM>(d, f);
+    else vec ? by_width<__nv_bfloat16, 8, false>(d, f) : by_width<__nv_bfloat16, 1, SLIM>(d, f);
 }
 
-// Rows that a block of the backward pass walks at a time, at most.
+// Rows that a block of the backward pass walks at a time, and blocks an SM.
 int rows_per_block(int d) { return d <= 512 ? 8 : d <= 1024 ? 4 : d <= 2048 ? 2 : 1; }
+int blocks_per_sm(int d) { return d <= 4096 ? 2 : 1; }
 
 // 128-bit accesses need every row to start on a 16-byte boundary.
 bool vector_rows(const void* p, int64_t ld, int32_t type) {
@@ -362,19 +413,27 @@ struct LaunchNorm {
     }
 };
 struct LaunchNormGrad {
-    const NormGradArgs& a;
+    NormGradArgs& a;
     unsigned blocks;
     cudaStream_t s;
     template <typename T, int VEC, int TPR, int E>
     void operator()() const {
-        norm_grad_kernel<T, VEC, TPR, E><<<blocks, TPR < 256 ? 256 : TPR, 0, s>>>(a);
+        constexpr int kThreads = TPR < 256 ? 256 : TPR, kRows = kThreads / TPR;
+        // rows ahead: some 180 KB of them an SM; a very wide row takes what it takes
+        a.slot = (a.d * (int)sizeof(T) + 15) / 16 * 16 + 16;
+        const int row = kRows * (a.dh != nullptr ? 3 : 2) * a.slot, room = 180 * 1024 / blocks_per_sm(a.d), most = room / row;
+        a.stages = most < 1 ? 1 : most < kMaxStages ? most : kMaxStages;
+        const int smem = a.stages * row;
+        const auto kernel = a.dh ? norm_grad_kernel<T, VEC, TPR, E, true> : norm_grad_kernel<T, VEC, TPR, E, false>;
+        if (smem > 30 * 1024) (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem < room ? room : smem);
+        kernel<<<blocks, kThreads, smem, s>>>(a);
     }
 };
 
 int launch_norm(NormArgs& a, int32_t type, void* stream) {
     const bool vec = a.d % (16 / fg::type_size(type)) == 0 && vector_rows(a.x, a.ldx, type) &&
                      vector_rows(a.residual, a.ldr, type) && vector_rows(a.h, a.d, type) && fg::aligned16(a.y);
-    by_type(type, vec, a.d, LaunchNorm{a, static_cast<cudaStream_t>(stream)});
+    by_type<true>(type, vec, a.d, LaunchNorm{a, static_cast<cudaStream_t>(stream)});
     FG_CUDA_TRY(cudaGetLastError());
     fg::count_launches(1);
     return FG_OK;
@@ -388,6 +447,13 @@ int check_rows(int64_t n, int32_t d, int32_t type) {
 }
 
 }  // namespace
+
+namespace fg {
+int norm_stuck(cudaStream_t s, int* out) {
+    FG_CUDA_TRY(cudaMemcpyFromSymbolAsync(out, g_stuck, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
+    return FG_OK;
+}
+}  // namespace fg
 
 extern "C" {
 
@@ -422,7 +488,7 @@ int fg_quantize_rows(const void* d_x, int64_t ldx, void* d_y, float* d_scales, i
 int64_t fg_rms_norm_backward_blocks(int64_t n, int32_t d) {
     if (n < 1 || d < 1) return 0;
     const int rows = rows_per_block(d);
-    const int64_t want = (n + rows - 1) / rows, most = (int64_t)fg::device_props().sm_count * (d <= 4096 ? 4 : d <= 8192 ? 2 : 1);
+    const int64_t want = (n + rows - 1) / rows, most = (int64_t)fg::device_props().sm_count * blocks_per_sm(d);
     return want < most ? want : most;
 }
 
@@ -444,10 +510,10 @@ int fg_rms_norm_backward(const void* d_h, int64_t ldh, const void* d_weight, con
     if (!d_h || !d_dy || !d_dx || (d_dweight && !d_partial)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
     if (blocks < 1 || blocks > INT_MAX) return fg::fail(FG_ERR_INVALID_ARGUMENT, "blocks must come from fg_rms_norm_backward_blocks");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    NormGradArgs a{d_h, d_weight, d_dy, d_dh, d_dx, d_dweight ? d_partial : nullptr, ldh, lddy, lddh, n, d, eps, weight_type == FG_F32};
+    NormGradArgs a{d_h, d_weight, d_dy, d_dh, d_dx, d_dweight ? d_partial : nullptr, ldh, lddy, lddh, n, d, 0, 0, eps, weight_type == FG_F32};
     const bool vec = d % (16 / fg::type_size(type)) == 0 && vector_rows(d_h, ldh, type) && vector_rows(d_dy, lddy, type) &&
                      vector_rows(d_dh, lddh, type) && fg::aligned16(d_dx);
-    by_type(type, vec, d, LaunchNormGrad{a, (unsigned)blocks, s});
+    by_type<false>(type, vec, d, LaunchNormGrad{a, (unsigned)blocks, s});
     FG_CUDA_TRY(cudaGetLastError());
     fg::count_launches(1);
     if (d_dweight) {

@@ -56,6 +56,9 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
+// Whether a wait of the norm's gradient ever ran out on the current device (row_norm.cu), copied to *out on `s`.
+int norm_stuck(cudaStream_t s, int* out);
+
 inline int type_size(int32_t t) { return t == FG_F32 ? 4 : t == FG_E4M3 ? 1 : 2; }
 inline bool float_type(int32_t t) { return t == FG_F32 || t == FG_F16 || t == FG_BF16; }
 

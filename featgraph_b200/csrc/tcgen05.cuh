@@ -96,6 +96,11 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
             "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
             : "memory");
 }
+// Consecutive bytes (addresses and size on the 16-byte grid).
+__device__ __forceinline__ void bulk_load(uint32_t dst, uint64_t src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar)
+                 : "memory");
+}
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* map) { asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory"); }
 
 // True in one lane of the (converged) warp, the same every time.  Copies and products are issued under it: their operands

@@ -345,6 +345,10 @@ int fg_coo_validate(const int32_t* d_row, const int32_t* d_col, int64_t n_rows, 
 #define FG_BF16 2
 #define FG_E4M3 3
 
+/* Kernels wait for their own copies with a limit (seconds).  Synchronises `stream` and returns FG_ERR_CUDA if such a
+ * wait ever ran out on the current device; the output of that call was wrong. */
+int fg_wait_status(void* stream);
+
 /* Root-mean-square norm: h = x + residual (rounded to `type`; h = x and d_h unused where d_residual is NULL),
  * y = h * r * weight with r = 1 / sqrt(mean(h^2) + eps).  d_weight may be NULL (ones), else of `type` or fp32.
  * out_type FG_E4M3: d_scales[row] = max|y| / 448 (1 for a row of zeros) and the 8-bit values y / scale.
@@ -386,10 +390,7 @@ int fg_group_rows(const int32_t* d_keys, int64_t num_entries, int32_t num_groups
  * y[p, o] = sum over i of x[row(p), i] * w[g, o, i] for the rows p of each group g; rows in no group are 0.
  * row(p) = p where d_order is NULL, else d_order[p] / choices.  w[g, o, i] is d_w[g w_group + o w_out + i w_in].
  * FG_E4M3: times d_x_scales[row(p)] * d_w_scales[g * outer + o], output of out_type.  y dense, [num_rows, outer].
- * The products wait for their own copies with a limit: fg_grouped_matmul_status synchronises `stream` and returns
- * FG_ERR_CUDA if one ever ran out on this device (its output is then wrong).
  * fg_grouped_matmul_wgrad: d_dw[g, o, i] = sum over the rows p of g of dy[p, o] * x[row(p), i], dense. */
-int fg_grouped_matmul_status(void* stream);
 int64_t fg_grouped_matmul_workspace(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,
                                     const int32_t* d_order, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type);
 int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, const void* d_w, int64_t w_group, int64_t w_out,

@@ -631,4 +631,4 @@ def test_refusals_that_need_a_device():
 def test_no_wait_ever_ran_out():
     """Runs last: the products' bounded waits (for their own copies) all ended in time in this process."""
     from featgraph_b200 import _native
-    assert _native.lib().fg_grouped_matmul_status(torch.cuda.current_stream().cuda_stream) == 0
+    assert _native.lib().fg_wait_status(torch.cuda.current_stream().cuda_stream) == 0
