@@ -60,9 +60,10 @@ SIGNATURES = {
     "fg_grouped_matmul_workspace": (_i64, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _i64, _i32, _i32, _i32, _i32]),
     "fg_grouped_matmul": (ctypes.c_int, [_vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i64, _vp, _i64, _i32, _i32, _i32,
                                          _i32, _i32, _vp, _i64, _vp]),
-    "fg_grouped_matmul_wgrad_workspace": (_i64, [_vp, _i64, _vp, _i64, _vp, _i64, _i32, _i32, _i32, _i32]),
-    "fg_grouped_matmul_wgrad": (ctypes.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _i32, _i64, _vp, _i64, _i32, _i32, _i32, _i32, _vp, _i64,
-                                               _vp]),
+    "fg_grouped_matmul_backward_workspace": (_i64, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _i64, _i32, _i32, _i64, _i32, _i32, _i32,
+                                                    _i32]),
+    "fg_grouped_matmul_backward": (ctypes.c_int, [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i32, _i64, _vp, _i64, _vp, _vp, _i64,
+                                                  _i32, _i32, _i32, _i32, _vp, _i64, _vp]),
     "fg_combine_rows": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _vp]),
     "fg_combine_rows_backward": (ctypes.c_int, [_vp, _i64, _vp, _vp, _vp, _i32, _vp, _i64, _vp, _vp, _i64, _i32, _i32, _i32, _vp]),
 }

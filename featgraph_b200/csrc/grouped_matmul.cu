@@ -23,6 +23,7 @@
 // row pitch or a start off the 16-byte grid, two strides above 1) and cuts fp32 into parts.
 #include <climits>
 #include <mutex>
+#include <type_traits>
 
 #include "rows.cuh"
 #include "tcgen05.cuh"
@@ -44,11 +45,15 @@ struct MmaArgs {
     void* y;              // output rows, dW, or partial sums of dW
     int64_t m, x_rows;    // slots; rows of x
     int32_t choices, groups, inner, outer;  // inner: the summed axis (y) or x's width (dW); outer: width of y
-    int32_t type, out_type, format;
+    int32_t out_type, format;
     bool b_mn, shared_weight;
     int32_t split;        // dW: rows of one partial sum (0: a group's rows in one)
     int32_t units;        // dW: partial sums that there is room for
-    int32_t box_rows;     // y: rows of a tile that are loaded (all that a group can have, where that is fewer than a tile's)
+    // few rows
+    const void* x;
+    int64_t ldx;
+    int32_t stages, held;  // stages of weights; bytes of the rows
+    bool vector_rows;      // rows on the 16-byte grid
 };
 
 enum Kind { kHalf, kEight, kParts };  // 16-bit values, e4m3, fp32 in three bf16 parts
@@ -60,8 +65,10 @@ __host__ __device__ constexpr int part_b(int pair) { return (0x010120 >> (4 * pa
 // A stage holds 128 bytes of the summed axis of both operands, of all parts: each is loaded once for its three, two
 // or one products (loaded for each product anew, 100003 x 256 x 128 took 66 us against the copy engines' rate).
 //
-// FEW: at most 32 slots in all.  Only 4 KB of a stage hold rows; the products read 16 KB from there on, which for the rows
-// that are not stored is whatever lies in the stages behind.
+// FEW: at most 32 slots in all.  Their rows, gathered as the block starts, stay in shared memory for all of its tiles (row =
+// slot; the products read 128 rows from there on, of which those that are not stored are whatever lies behind), and the
+// stages hold weights alone, 256 bytes of the summed axis each: a stage costs the thread that issues its products some 400
+// cycles, in which 64 columns x 128 bytes from each of the SMs are less than the memory delivers.
 //
 // BLOCKS = 2: a pair of blocks computes 256 x BN; each loads 128 rows of the one operand and half the columns of the other,
 // and the first one's products read both shared memories (cta_group::2).
@@ -69,31 +76,33 @@ template <int BN, Kind KIND, bool FEW, int BLOCKS>
 struct Shape {
     static constexpr int kParts = KIND == Kind::kParts ? 3 : 1;
     static constexpr int kOwnCols = BN / BLOCKS;
-    static constexpr int kA = (FEW ? 32 : kTileRows) * kChunkBytes, kB = kOwnCols * kChunkBytes;  // bytes of one part
-    static constexpr int kStageBytes = kParts * (kA + kB);
-    static constexpr int kStages = 196608 / kStageBytes < 16 ? 196608 / kStageBytes : 16;
+    static constexpr int kA = FEW ? 0 : kTileRows * kChunkBytes, kB = kOwnCols * kChunkBytes;  // bytes of one part
+    static constexpr int kDeep = FEW ? 2 : 1;  // 128-byte chunks a stage
+    static constexpr int kStageBytes = kParts * (kA + kB) * kDeep;
+    static constexpr int kStages = 196608 / kStageBytes < 16 ? 196608 / kStageBytes : 16;  // at most
     static constexpr int kColumns = 2 * BN;
-    static constexpr int kStaging = kStages * kStageBytes;  // 2 KB for each output warp
-    static constexpr int kSmem = 1024 + kStaging + 8 * 2048;
+    static constexpr int kOutput = 8 * 2048;  // 2 KB for each output warp
+    static constexpr int kSmem = 1024 + kOutput + (FEW ? 196608 : kStages * kStageBytes);
 };
 
 struct Tables {
-    uint64_t full[16], empty[16], tail[16], filled[2], drained[2], last;
+    uint64_t full[16], empty[16], tail[16], filled[2], drained[2], rows, last;
     uint32_t tmem;
     int stop;
     int warp_sums[11];
+    int sources[32];            // few rows: the row of x behind each slot, or -1
     int start[kMaxGroups + 1];  // first slot of each group
     int tiles[kMaxGroups + 1];  // row tiles (partial sums of dW) before each group
 };
 
-// Takes a warp's 32 rows of an accumulator, from `tmem` on, to the output rows from `out` on (row pitch `width`; rows >=
-// `rows` and columns >= `left` are not stored): every second 64-byte wide piece of the BN columns, the warp's partner takes
+// Takes a warp's 32 rows of an accumulator, from `tmem` on, to the output rows from `out` on (row pitch `width`; rows
+// outside [from, rows) and columns >= `left` are not stored): every second 64-byte wide piece of the BN columns, the warp's partner takes
 // the others.  A thread holds a row in tensor memory's layout, so the pieces go through the warp's 2 KB of shared memory
 // (16-byte cells, XOR-swizzled: no bank conflicts either way) and leave as whole sectors, 4 lanes a row.  Stored
 // straight from the threads, 16 bytes in each of 32 rows at a time, or by four warps instead of eight, the output of
 // products with a short inner axis keeps the tensor cores waiting.
 template <typename O, int BN, bool EIGHT>
-__device__ __forceinline__ void store_rows(uint32_t tmem, bool filled, O* out, int64_t width, int rows, int left, bool vector, uint32_t staging,
+__device__ __forceinline__ void store_rows(uint32_t tmem, bool filled, O* out, int64_t width, int from, int rows, int left, bool vector, uint32_t staging,
                                            int half, float scale, const float* column_scales) {
     constexpr int kCols = 64 / sizeof(O), kCells = 16 / sizeof(O);
     const int lane = threadIdx.x & 31;
@@ -133,7 +142,7 @@ __device__ __forceinline__ void store_rows(uint32_t tmem, bool filled, O* out, i
                              : "=r"(p.v[0]), "=r"(p.v[1]), "=r"(p.v[2]), "=r"(p.v[3])
                              : "r"(staging + r * 64 + ((q ^ ((r >> 1) & 3)) << 4))
                              : "memory");
-                if (r < rows && q * kCells < rest) store_pack<uint32_t, 4>(reinterpret_cast<uint32_t*>(out + r * width + c + q * kCells), p);
+                if (r >= from && r < rows && q * kCells < rest) store_pack<uint32_t, 4>(reinterpret_cast<uint32_t*>(out + r * width + c + q * kCells), p);
             }
         } else {
             constexpr int kAtOnce = 32 / kCols;  // rows side by side
@@ -143,10 +152,43 @@ __device__ __forceinline__ void store_rows(uint32_t tmem, bool filled, O* out, i
                 O v;
                 if constexpr (sizeof(O) == 4) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(*reinterpret_cast<uint32_t*>(&v)) : "r"(at) : "memory");
                 else asm volatile("ld.shared.b16 %0, [%1];" : "=h"(*reinterpret_cast<uint16_t*>(&v)) : "r"(at) : "memory");
-                if (k < rest) out[r * width + c + k] = v;
+                if (r >= from && k < rest) out[r * width + c + k] = v;
             }
         }
         __syncwarp();
+    }
+}
+
+// Few rows: 256 threads gather the slots' rows into shared memory, as a TMA load would lay them: 128-byte chunks of each
+// row, `chunk` bytes a chunk of all, 16-byte cells XOR-swizzled, zeros beyond the inner axis and for a slot without a row.
+template <bool EIGHT>
+__device__ __forceinline__ void hold_rows(const MmaArgs& a, uint32_t held, int chunk, const int* sources, int thread) {
+    using V = typename std::conditional<EIGHT, uint8_t, uint16_t>::type;
+    constexpr int kPer = 16 / sizeof(V), kAhead = 8;
+    const int pieces = (a.inner + kPer * 16 - 1) / (kPer * 16) * 16, all = (int)a.m * pieces;
+    for (int first = thread; first < all; first += 256 * kAhead) {
+        Pack<V, kPer> p[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = first + u * 256, r = min(i, all - 1) / pieces, k = (i - r * pieces) * kPer, source = sources[r];
+            const V* x = static_cast<const V*>(a.x) + (int64_t)max(source, 0) * a.ldx + k;
+            const bool in = i < all && source >= 0;
+            if (in && a.vector_rows && k + kPer <= a.inner) {
+                p[u] = fg::load_pack<V, kPer>(x);
+            } else {
+#pragma unroll
+                for (int j = 0; j < kPer; ++j) p[u].v[j] = in && k + j < a.inner ? x[j] : V(0);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+            const int i = first + u * 256, r = min(i, all - 1) / pieces, piece = i - r * pieces;
+            if (i >= all) break;
+            const uint32_t* word = reinterpret_cast<const uint32_t*>(&p[u]);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(held + (piece >> 3) * chunk + r * 128 + (((piece & 7) ^ (r & 7)) << 4)),
+                         "r"(word[0]), "r"(word[1]), "r"(word[2]), "r"(word[3])
+                         : "memory");
+        }
     }
 }
 
@@ -163,16 +205,19 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
     product_kernel(const MmaArgs a, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
     using S = Shape<BN, KIND, FEW, BLOCKS>;
     constexpr bool EIGHT = KIND == kEight;
-    constexpr int kChunk = EIGHT ? 128 : 64;  // values of the summed axis a stage holds
+    constexpr int kChunk = (EIGHT ? 128 : 64) * S::kDeep;  // values of the summed axis a stage holds
     constexpr int kRows = kTileRows * BLOCKS;
     extern __shared__ uint8_t dynamic[];
     __shared__ Tables t;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = BLOCKS == 2 ? (int)fg::cluster_rank() : 0;
-    const uint32_t ring = (fg::smem_address(dynamic) + 1023u) & ~1023u;
+    const uint32_t held = (fg::smem_address(dynamic) + 1023u) & ~1023u;  // few rows: they come first
+    const uint32_t ring = held + (FEW ? a.held : 0);
+    const int stages = FEW ? a.stages : S::kStages;
+    const int held_chunk = (int)(a.m + 7) / 8 * 1024;  // few rows: bytes of 128 bytes of each
 
     if (threadIdx.x == 0) {
-        for (int s = 0; s < S::kStages; ++s) {
+        for (int s = 0; s < stages; ++s) {
             fg::barrier_init(fg::smem_address(&t.full[s]), BLOCKS);
             fg::barrier_init(fg::smem_address(&t.tail[s]), 1);
             fg::barrier_init(fg::smem_address(&t.empty[s]), 1);
@@ -181,13 +226,23 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
             fg::barrier_init(fg::smem_address(&t.filled[s]), 1);
             fg::barrier_init(fg::smem_address(&t.drained[s]), 8 * BLOCKS);
         }
+        fg::barrier_init(fg::smem_address(&t.rows), 8);
         fg::barrier_init(fg::smem_address(&t.last), 1);
         fg::barrier_init_fence();
         t.stop = 0;
-        fg::prefetch_map(&map_a);
+        if (!FEW) fg::prefetch_map(&map_a);
         fg::prefetch_map(&map_b);
     }
     if (warp == 1) fg::tmem_alloc<BLOCKS>(fg::smem_address(&t.tmem), S::kColumns);
+
+    if (FEW && threadIdx.x < 32 && threadIdx.x < a.m) {
+        int r = threadIdx.x;
+        if (a.order) {
+            const int e = a.order[r];
+            r = e >= 0 ? e / a.choices : -1;
+        }
+        t.sources[threadIdx.x] = r < a.x_rows ? r : -1;
+    }
 
     // groups' first slots and tile counts, scanned: thread i takes groups [i * each, (i + 1) * each)
     {
@@ -273,7 +328,8 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
 
     if (warp == 0) {
         if (fg::elect_one()) {
-            int64_t step = 0;  // stages filled so far
+            int s = 0, parity = 1;  // next stage, and the parity that its emptying will have had (a fresh barrier passes for 1)
+            int64_t step = 0;       // stages filled so far
             uint32_t tail_now = 0, tail_parity = 0;  // a bit a stage: holds a tail; parity of its next tail
             bool live = true;
             for (int64_t i = start; live && i < total; i += stride) {
@@ -285,22 +341,23 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
                     return WGRAD || a.b_mn ? max(min(S::kOwnCols / 64, ((WGRAD ? a.inner : a.outer) - at + 63) / 64), 0) : S::kOwnCols / 64;
                 };
                 const int a_blocks = blocks_a(w.row), b_blocks = blocks_b(col);
-                const uint32_t own = ((WGRAD ? a_blocks * 8192 : a.box_rows * kChunkBytes) + b_blocks * 8192) * S::kParts;
+                const uint32_t own = ((WGRAD ? a_blocks * 8192 : S::kA) + b_blocks * 8192) * S::kParts * S::kDeep;
                 uint32_t bytes = own;
                 if (BLOCKS == 2)  // the first block's barrier counts the second one's loads too
-                    bytes += ((WGRAD ? blocks_a(w.row + kTileRows) * 8192 : a.box_rows * kChunkBytes) + blocks_b(col + S::kOwnCols) * 8192) * S::kParts;
+                    bytes += ((WGRAD ? blocks_a(w.row + kTileRows) * 8192 : S::kA) + blocks_b(col + S::kOwnCols) * 8192) * S::kParts;
                 for (int c = 0; c < w.chunks; ++c, ++step) {
-                    const int s = (int)(step % S::kStages);
+                    const int at_stage = s;
                     const uint32_t full = fg::smem_address(&t.full[s]), stage = ring + s * S::kStageBytes;
-                    if (step >= S::kStages && !fg::barrier_wait(fg::smem_address(&t.empty[s]), (step / S::kStages - 1) & 1, stop)) {
+                    if (!fg::barrier_wait(fg::smem_address(&t.empty[s]), parity, stop)) {
                         live = false;
                         break;
                     }
+                    if (++s == stages) s = 0, parity ^= 1;
                     const int k = c * kChunk;
                     if (WGRAD && c == w.chunks - 1 && w.ragged()) {  // goes through the warp that clears it, each block's own
-                        const uint32_t bar = fg::smem_address(&t.tail[s]);
-                        tail_now |= 1u << s;
-                        tail_parity ^= 1u << s;
+                        const uint32_t bar = fg::smem_address(&t.tail[at_stage]);
+                        tail_now |= 1u << at_stage;
+                        tail_parity ^= 1u << at_stage;
                         fg::barrier_expect(bar, own);
 #pragma unroll
                         for (int p = 0; p < S::kParts; ++p) {
@@ -311,7 +368,7 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
                         }
                         continue;
                     }
-                    tail_now &= ~(1u << s);
+                    tail_now &= ~(1u << at_stage);
                     if (rank == 0) {
                         fg::barrier_expect(full, bytes);
                         if (BLOCKS == 2) fg::barrier_arrive(full);  // two arrivals: those of the clearing warps, for a tail
@@ -325,30 +382,36 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
                             for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d<BLOCKS>(bt + q * 8192, &map_b, col + q * 64, slot, full);
                         } else {
                             const int g = a.shared_weight ? p : w.group + p * a.groups;
-                            fg::tma_load_2d<BLOCKS>(at, &map_a, k, w.begin + p * (int)a.m, full);
-                            if (!a.b_mn) {
-                                fg::tma_load_3d<BLOCKS>(bt, &map_b, k, col, g, full);
-                            } else {
-                                for (int q = 0; q < b_blocks; ++q) fg::tma_load_3d<BLOCKS>(bt + q * 8192, &map_b, col + q * 64, k, g, full);
+                            if (!FEW) fg::tma_load_2d<BLOCKS>(at, &map_a, k, w.begin + p * (int)a.m, full);
+#pragma unroll
+                            for (int h = 0; h < S::kDeep; ++h) {
+                                const int kh = k + h * (kChunk / S::kDeep);
+                                const uint32_t to = bt + h * S::kB;
+                                if (!a.b_mn) {
+                                    fg::tma_load_3d<BLOCKS>(to, &map_b, kh, col, g, full);
+                                } else {
+                                    for (int q = 0; q < b_blocks; ++q) fg::tma_load_3d<BLOCKS>(to + q * 8192, &map_b, col + q * 64, kh, g, full);
+                                }
                             }
                         }
                     }
                 }
             }
             if (*stop)  // no copy may be in flight when the block (or its pair) ends
-                for (int64_t q = max(step - S::kStages, (int64_t)0); q < step; ++q) {
-                    const int s = (int)(q % S::kStages);
-                    if (tail_now >> s & 1) fg::barrier_wait(fg::smem_address(&t.tail[s]), ~tail_parity >> s & 1, stop, true);
-                    else if (rank == 0) fg::barrier_wait(fg::smem_address(&t.full[s]), (q / S::kStages) & 1, stop, true);
+                for (int64_t q = max(step - stages, (int64_t)0); q < step; ++q) {
+                    const int at = (int)(q % stages);
+                    if (tail_now >> at & 1) fg::barrier_wait(fg::smem_address(&t.tail[at]), ~tail_parity >> at & 1, stop, true);
+                    else if (rank == 0) fg::barrier_wait(fg::smem_address(&t.full[at]), (q / stages) & 1, stop, true);
                 }
         }
         __syncwarp();
     } else if (warp == 1) {
         if (rank == 0 && fg::elect_one()) {
-            int64_t step = 0, turn = 0;
+            int s = 0, parity = 0;
+            int64_t turn = 0;
             const uint32_t descriptor = fg::product_descriptor(a.format, WGRAD, WGRAD || a.b_mn, kRows, BN);
             const bool b_mn = WGRAD || a.b_mn;
-            bool live = true;
+            bool live = !FEW || start >= total || fg::barrier_wait(fg::smem_address(&t.rows), 0, stop);
             for (int64_t i = start; live && i < total; i += stride) {
                 const Tile w = locate(i);
                 if (w.chunks == 0) continue;  // an empty group's dW: nothing to add up
@@ -356,25 +419,26 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
                 const uint32_t acc = tmem + buffer * BN;
                 if (turn >= 2 && !fg::barrier_wait<BLOCKS == 2>(fg::smem_address(&t.drained[buffer]), (turn / 2 - 1) & 1, stop)) break;
                 fg::tcgen05_after_sync();
-                for (int c = 0; c < w.chunks; ++c, ++step) {
-                    const int s = (int)(step % S::kStages);
-                    const uint32_t stage = ring + s * S::kStageBytes, parity = (step / S::kStages) & 1;
+                for (int c = 0; c < w.chunks; ++c) {
+                    const uint32_t stage = ring + s * S::kStageBytes, empty = fg::smem_address(&t.empty[s]);
                     live = fg::barrier_wait<BLOCKS == 2 && WGRAD>(fg::smem_address(&t.full[s]), parity, stop);
+                    if (++s == stages) s = 0, parity ^= 1;
                     if (!live) break;
                     fg::tcgen05_after_sync();
                     // of a group's last chunk only the steps that have rows of it
                     const int steps = WGRAD && c == w.chunks - 1 ? (w.end - w.begin - c * kChunk + 15) / 16 : 4;
 #pragma unroll
                     for (int pair = S::kParts == 3 ? 0 : 5; pair < 6; ++pair) {
-                        const uint32_t at = stage + part_a(pair) * S::kA, bt = stage + S::kParts * S::kA + part_b(pair) * S::kB;
+                        const uint32_t at = FEW ? held + c * 2 * held_chunk : stage + part_a(pair) * S::kA, bt = stage + S::kParts * S::kA + part_b(pair) * S::kB;
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            const uint64_t da = WGRAD ? fg::operand_descriptor(at + k * 2048, 8192, 1024) : fg::operand_descriptor(at + k * 32, 16, 1024);
-                            const uint64_t db = b_mn ? fg::operand_descriptor(bt + k * 2048, 8192, 1024) : fg::operand_descriptor(bt + k * 32, 16, 1024);
+                        for (int k = 0; k < 4 * S::kDeep; ++k) {
+                            const uint32_t ah = at + k / 4 * held_chunk, bh = bt + k / 4 * S::kB;  // a chunk further from the fifth step on
+                            const uint64_t da = WGRAD ? fg::operand_descriptor(at + k * 2048, 8192, 1024) : fg::operand_descriptor(ah + k % 4 * 32, 16, 1024);
+                            const uint64_t db = b_mn ? fg::operand_descriptor(bh + k % 4 * 2048, 8192, 1024) : fg::operand_descriptor(bh + k % 4 * 32, 16, 1024);
                             if (!WGRAD || k < steps) fg::product_step<BLOCKS, EIGHT>(acc, da, db, descriptor, c > 0 || pair > (S::kParts == 3 ? 0 : 5) || k > 0);
                         }
                     }
-                    fg::product_commit<BLOCKS>(fg::smem_address(&t.empty[s]));
+                    fg::product_commit<BLOCKS>(empty);
                 }
                 if (!live) break;
                 fg::product_commit<BLOCKS>(fg::smem_address(&t.filled[buffer]));
@@ -395,7 +459,7 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
             const Tile w = locate(i);
             step += w.chunks;
             if (w.chunks == 0 || !w.ragged()) continue;
-            const int s = (int)((step - 1) % S::kStages), keep = (w.end - w.begin - 1) % kChunk + 1, upto = (keep + 15) / 16 * 16;
+            const int s = (int)((step - 1) % stages), keep = (w.end - w.begin - 1) % kChunk + 1, upto = (keep + 15) / 16 * 16;
             const uint32_t stage = ring + s * S::kStageBytes;
             if (!warp_wait(fg::smem_address(&t.tail[s]), tail_parity >> s & 1, stop)) break;
             tail_parity ^= 1u << s;
@@ -414,7 +478,13 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
     } else {
         const int quarter = warp & 3;  // the lanes of tensor memory this warp can read
         const int half = (warp - 2) >> 2;
-        const uint32_t staging = ring + S::kStaging + (warp - 2) * 2048;
+        const uint32_t staging = ring + stages * S::kStageBytes + (warp - 2) * 2048;
+        if (FEW && start < total) {
+            hold_rows<EIGHT>(a, held, held_chunk, t.sources, threadIdx.x - 64);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) fg::barrier_arrive(fg::smem_address(&t.rows));
+        }
         const int width = WGRAD ? a.inner : a.outer;
         const int size = a.out_type == FG_F32 ? 4 : 2;
         const bool vector = (int64_t)width * size % 16 == 0 && ((uintptr_t)a.y & 15) == 0;
@@ -422,13 +492,15 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
         for (int64_t i = start; i < total; i += stride) {
             const Tile w = locate(i);
             const int above = quarter * 32;
-            const int rows = (WGRAD ? a.outer - w.row : w.end - w.begin) - above;
-            const int64_t first = (WGRAD ? (int64_t)(a.split ? w.unit : w.group) * a.outer + w.row : w.begin) + above;
+            // a tile's rows start with its first slot, held ones with slot 0: there, rows of [begin, end) are stored
+            const int slot0 = FEW ? 0 : w.begin, from = FEW ? w.begin - above : 0;
+            const int rows = (WGRAD ? a.outer - w.row : w.end - slot0) - above;
+            const int64_t first = (WGRAD ? (int64_t)(a.split ? w.unit : w.group) * a.outer + w.row : slot0) + above;
             float scale = 0.0f;
             const float* column_scales = nullptr;
             if (EIGHT) {
-                const int slot = w.begin + above + lane;
-                if (slot < w.end) {
+                const int slot = slot0 + above + lane;
+                if (slot >= w.begin && slot < w.end) {
                     const int e = a.order ? a.order[slot] : 0, r = a.order ? e / a.choices : slot;
                     if (e >= 0 && r < a.x_rows) scale = a.x_scales[r];
                 }
@@ -442,11 +514,11 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
             const uint32_t acc = tmem + ((uint32_t)above << 16) + buffer * BN;
             const int64_t at = first * width + w.col;
             if (a.out_type == FG_F32)
-                store_rows<float, BN, EIGHT>(acc, w.chunks > 0, static_cast<float*>(a.y) + at, width, rows, width - w.col, vector, staging, half, scale, column_scales);
+                store_rows<float, BN, EIGHT>(acc, w.chunks > 0, static_cast<float*>(a.y) + at, width, from, rows, width - w.col, vector, staging, half, scale, column_scales);
             else if (a.out_type == FG_F16)
-                store_rows<__half, BN, EIGHT>(acc, w.chunks > 0, static_cast<__half*>(a.y) + at, width, rows, width - w.col, vector, staging, half, scale, column_scales);
+                store_rows<__half, BN, EIGHT>(acc, w.chunks > 0, static_cast<__half*>(a.y) + at, width, from, rows, width - w.col, vector, staging, half, scale, column_scales);
             else
-                store_rows<__nv_bfloat16, BN, EIGHT>(acc, w.chunks > 0, static_cast<__nv_bfloat16*>(a.y) + at, width, rows, width - w.col, vector, staging, half, scale,
+                store_rows<__nv_bfloat16, BN, EIGHT>(acc, w.chunks > 0, static_cast<__nv_bfloat16*>(a.y) + at, width, from, rows, width - w.col, vector, staging, half, scale,
                                                      column_scales);
             if (w.chunks) {
                 fg::tcgen05_before_sync();
@@ -820,9 +892,17 @@ int rows_matrix(Matrix* out, const void* p, int64_t ld, int64_t source_rows, con
     return pack(p, 0, ld, 1, 1, m, cols, order, choices, source_rows, type, work, s);
 }
 
-// Few rows, a dense inner axis and 8 rows of it in shared memory: the form without tiles.
-bool few_rows(int64_t num_rows, int64_t w_in, int32_t inner, int32_t type) {
-    return type == FG_F32 && num_rows <= kFewRows && (w_in == 1 || inner == 1) && round_up(inner, 16) * 8 * fg::type_size(type) <= 192 * 1024;
+// Few fp32 rows (or a weight off the 16-byte grid), a dense inner axis and 8 rows of it in shared memory: the form without
+// tiles, which reads the weights as they are.
+bool few_rows(int64_t num_rows, const void* w, int64_t w_group, int64_t w_out, int64_t w_in, int32_t inner, int32_t type) {
+    return num_rows <= kFewRows && (w_in == 1 || inner == 1) && round_up(inner, 16) * 8 * fg::type_size(type) <= 192 * 1024 &&
+           !loadable(w, w_out, w_group, type);
+}
+// Few rows that stay in shared memory beside 8 stages of weights: their bytes there; 0 where they do not.
+int64_t held_bytes(int64_t num_rows, int32_t inner, int32_t type) {
+    if (num_rows > kFewRows || type == FG_F32) return 0;
+    const int64_t bytes = round_up((int64_t)inner * fg::type_size(type), 2 * kChunkBytes) * round_up(num_rows, 8);
+    return bytes <= 64 * 1024 ? bytes : 0;
 }
 template <typename T>
 int launch_few(const FewArgs& a, cudaStream_t s) {
@@ -888,7 +968,7 @@ template <Kind KIND, bool WGRAD>
 int launch(int bn, const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b, int64_t most_tiles, cudaStream_t s) {
     if constexpr (KIND != kParts) {
         if constexpr (!WGRAD)
-            if (a.box_rows <= 32) return launch_shape<64, KIND, false, true, 1>(a, map_a, map_b, most_tiles, s);
+            if (a.held) return launch_shape<64, KIND, false, true, 1>(a, map_a, map_b, most_tiles, s);
         if (bn == 512) return launch_shape<256, KIND, WGRAD, false, 2>(a, map_a, map_b, most_tiles, s);
         if (bn == 256) return launch_shape<256, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s);
     }
@@ -936,6 +1016,90 @@ int check_product(int64_t m, int64_t x_rows, int32_t choices, int32_t groups, in
     return FG_OK;
 }
 
+// A launch's sizes and lists, as the entry points get them.
+struct Problem {
+    const int32_t *offsets, *order;
+    int64_t m, x_rows;
+    int32_t choices, groups, inner, outer, type;
+};
+
+int64_t weight_bytes(const Problem& p, const void* w, int64_t w_group, int64_t w_out, int64_t w_in) {
+    const WeightLayout layout(w, w_group, w_out, w_in, p.groups, p.inner, p.outer, p.type);
+    return layout.copy ? packed_bytes(layout.count * layout.rows, layout.cols, p.type) : 0;
+}
+
+// y = products of the slots' rows; `x` as loads see them, or, where `held`, as they lie (d_x, ldx, by the order).
+int run_product(const Problem& p, const Matrix& x, const void* d_x, int64_t ldx, const float* x_scales, const void* d_w, int64_t w_group,
+                int64_t w_out, int64_t w_in, const float* w_scales, int64_t held, void* d_y, int32_t out_type, uint8_t** work, cudaStream_t s) {
+    const WeightLayout layout(d_w, w_group, w_out, w_in, p.groups, p.inner, p.outer, p.type);
+    const bool b_mn = layout.b_mn;
+    const int64_t step = b_mn ? w_in : w_out;  // of the weight's rows as stored
+    Matrix w;
+    if (!layout.copy) {
+        w = Matrix{d_w, layout.cols, layout.rows, layout.count, step, w_group ? w_group : layout.rows * step, p.type};
+    } else {
+        const int64_t pitch = pitch_of(layout.cols, p.type);
+        w = Matrix{*work, layout.cols, layout.rows, layout.count * (p.type == FG_F32 ? 3 : 1), pitch, layout.rows * pitch, p.type == FG_F32 ? FG_BF16 : p.type};
+        if (int rc = pack(d_w, w_group, step, b_mn ? w_out : w_in, layout.count, layout.rows, layout.cols, nullptr, 1, 0, p.type, work, s)) return rc;
+    }
+    const int64_t units = p.m / kTileRows + (p.groups < p.m ? p.groups : p.m);
+    // half a tile of each group is empty on average
+    const int64_t expected = p.m / kTileRows + p.groups / 2, expected_pairs = p.m / (2 * kTileRows) + p.groups / 2;
+    const bool paired = !held && pairs_pay(expected, expected_pairs, p.outer, p.type);
+    const int bn = held ? 64 : paired ? 512 : tile_width(units, p.outer, p.type), chunk = p.type == FG_E4M3 ? 128 : 64;
+    CUtensorMap map_x = {}, map_w;
+    if (!held)
+        if (int rc = make_map(&map_x, x, chunk, kTileRows)) return rc;
+    if (int rc = make_map(&map_w, w, chunk, b_mn ? 64 : paired ? 128 : bn)) return rc;
+    MmaArgs a{};
+    a.offsets = p.offsets, a.order = p.order, a.x_scales = x_scales, a.w_scales = w_scales, a.y = d_y;
+    a.m = p.m, a.x_rows = p.x_rows, a.choices = p.choices, a.groups = p.groups, a.inner = p.inner, a.outer = p.outer;
+    a.out_type = out_type, a.format = w.type == FG_BF16 ? 1 : 0;
+    a.b_mn = b_mn, a.shared_weight = w_group == 0;
+    a.x = d_x, a.ldx = ldx, a.held = (int32_t)held, a.vector_rows = fg::aligned16(d_x) && ldx * fg::type_size(p.type) % 16 == 0;
+    a.stages = (int32_t)((196608 - held) / 16384);
+    const int64_t tiles = units * ((p.outer + (paired ? 256 : bn) - 1) / (paired ? 256 : bn));
+    return p.type == FG_E4M3  ? launch<kEight, false>(bn, a, map_x, map_w, tiles, s)
+           : p.type == FG_F32 ? launch<kParts, false>(bn, a, map_x, map_w, tiles, s)
+                              : launch<kHalf, false>(bn, a, map_x, map_w, tiles, s);
+}
+
+// dW = sums over each group's rows of dy x^T; `sums`: partial_bytes() of workspace.
+int run_weight_gradient(const Problem& p, const Matrix& x, const Matrix& dy, void* d_dw, float* sums, cudaStream_t s) {
+    const int64_t cells = (int64_t)p.inner * p.outer, split = split_rows(p.m, p.groups, wgrad_tiles(p.inner, p.outer));
+    CUtensorMap map_x, map_dy;
+    if (int rc = make_map(&map_dy, dy, 64, 64)) return rc;
+    if (int rc = make_map(&map_x, x, 64, 64)) return rc;
+    const int64_t units = split ? p.m / split + p.groups : p.groups, rows_tiles = (p.outer + kTileRows - 1) / kTileRows;
+    // in pairs, the columns' waste counts as well as the rows', and a short sum is mostly output: 256 rows a group, 128
+    // groups of 2048 x 1408 took 325 us in pairs and 292 without, 1024 rows and more are faster in pairs
+    const int64_t singles = units * rows_tiles * ((p.inner + 127) / 128), doubles = units * ((p.outer + 255) / 256) * ((p.inner + 255) / 256);
+    const bool paired = p.m >= 768 * units && pairs_pay(singles, doubles * 2, 256, p.type);
+    const int bn = paired ? 512 : tile_width(units * rows_tiles, p.inner, p.type);
+    MmaArgs a{};
+    a.offsets = p.offsets, a.y = split ? static_cast<void*>(sums) : d_dw;
+    a.m = p.m, a.x_rows = p.x_rows, a.choices = p.choices, a.groups = p.groups, a.inner = p.inner, a.outer = p.outer;
+    a.out_type = split ? FG_F32 : p.type, a.format = dy.type == FG_BF16 ? 1 : 0;
+    a.split = (int32_t)split, a.units = (int32_t)units;
+    const int64_t tiles = paired ? doubles : units * rows_tiles * ((p.inner + bn - 1) / bn);
+    if (int rc = p.type == FG_F32 ? launch<kParts, true>(bn, a, map_dy, map_x, tiles, s) : launch<kHalf, true>(bn, a, map_dy, map_x, tiles, s)) return rc;
+    if (!split) return FG_OK;
+    const dim3 grid((unsigned)((cells + 255) / 256 < 4096 ? (cells + 255) / 256 : 4096), (unsigned)p.groups);
+    if (p.type == FG_F32) join_kernel<float><<<grid, 256, 0, s>>>(sums, p.offsets, p.groups, p.m, (int)split, a.units, cells, static_cast<float*>(d_dw));
+    else if (p.type == FG_F16) join_kernel<__half><<<grid, 256, 0, s>>>(sums, p.offsets, p.groups, p.m, (int)split, a.units, cells, static_cast<__half*>(d_dw));
+    else join_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(sums, p.offsets, p.groups, p.m, (int)split, a.units, cells, static_cast<__nv_bfloat16*>(d_dw));
+    FG_CUDA_TRY(cudaGetLastError());
+    fg::count_launches(1);
+    return FG_OK;
+}
+
+// The gradient of x, slot by slot, is a product with the weight read the other way.
+Problem other_way(const Problem& p) {
+    Problem q = p;
+    q.order = nullptr, q.choices = 1, q.x_rows = p.m, q.inner = p.outer, q.outer = p.inner;
+    return q;
+}
+
 }  // namespace
 
 extern "C" {
@@ -951,9 +1115,9 @@ int fg_wait_status(void* stream) {
 
 int64_t fg_grouped_matmul_workspace(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,
                                     const int32_t* d_order, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
-    if (num_rows <= 0 || groups < 1 || inner < 1 || outer < 1 || few_rows(num_rows, w_in, inner, type)) return 0;
+    if (num_rows <= 0 || groups < 1 || inner < 1 || outer < 1 || few_rows(num_rows, d_w, w_group, w_out, w_in, inner, type)) return 0;
     const WeightLayout w(d_w, w_group, w_out, w_in, groups, inner, outer, type);
-    return (rows_need_copy(d_x, ldx ? ldx : inner, d_order, type) ? packed_bytes(num_rows, inner, type) : 0) +
+    return (!held_bytes(num_rows, inner, type) && rows_need_copy(d_x, ldx ? ldx : inner, d_order, type) ? packed_bytes(num_rows, inner, type) : 0) +
            (w.copy ? packed_bytes(w.count * w.rows, w.cols, type) : 0);
 }
 
@@ -974,7 +1138,7 @@ int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, con
     if (!d_order && x_rows != num_rows) return fg::fail(FG_ERR_INVALID_ARGUMENT, "without an order x has a row for each slot");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
 
-    if (few_rows(num_rows, w_in, inner, type)) {
+    if (few_rows(num_rows, d_w, w_group, w_out, w_in, inner, type)) {
         const int size = fg::type_size(type);
         FewArgs f{d_x, d_w, type == FG_E4M3 ? d_x_scales : nullptr, type == FG_E4M3 ? d_w_scales : nullptr, d_offsets, d_order, d_y, ldx, w_group, w_out, x_rows,
                   (int32_t)num_rows, choices, groups, inner, outer, out_type, (int32_t)round_up(inner, 16), false, false};
@@ -985,98 +1149,75 @@ int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, con
                : type == FG_BF16 ? launch_few<__nv_bfloat16>(f, s)
                                  : launch_few<__nv_fp8_e4m3>(f, s);
     }
-    const WeightLayout layout(d_w, w_group, w_out, w_in, groups, inner, outer, type);
     const int64_t need = fg_grouped_matmul_workspace(d_x, ldx, d_w, w_group, w_out, w_in, d_order, num_rows, groups, inner, outer, type);
     if (workspace_bytes < need || (need && !d_workspace)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_grouped_matmul_workspace()");
     uint8_t* work = static_cast<uint8_t*>(d_workspace);
-    Matrix x, w;
-    if (int rc = rows_matrix(&x, d_x, ldx, x_rows, d_order, choices, num_rows, inner, type, &work, s)) return rc;
-    const bool b_mn = layout.b_mn;
-    const int64_t step = b_mn ? w_in : w_out;  // of the weight's rows as stored
-    if (!layout.copy) {
-        w = Matrix{d_w, layout.cols, layout.rows, layout.count, step, w_group ? w_group : layout.rows * step, type};
-    } else {
-        const int64_t pitch = pitch_of(layout.cols, type);
-        w = Matrix{work, layout.cols, layout.rows, layout.count * (type == FG_F32 ? 3 : 1), pitch, layout.rows * pitch, type == FG_F32 ? FG_BF16 : type};
-        if (int rc = pack(d_w, w_group, step, b_mn ? w_out : w_in, layout.count, layout.rows, layout.cols, nullptr, 1, 0, type, &work, s)) return rc;
-    }
-    const int64_t units = num_rows / kTileRows + (groups < num_rows ? groups : num_rows);
-    const int box_rows = type == FG_F32 || num_rows > 32 ? kTileRows : num_rows <= 8 ? 8 : num_rows <= 16 ? 16 : 32;
-    // half a tile of each group is empty on average
-    const int64_t expected = num_rows / kTileRows + groups / 2, expected_pairs = num_rows / (2 * kTileRows) + groups / 2;
-    const bool paired = pairs_pay(expected, expected_pairs, outer, type);
-    const int bn = box_rows <= 32 ? 64 : paired ? 512 : tile_width(units, outer, type), chunk = type == FG_E4M3 ? 128 : 64;
-    CUtensorMap map_x, map_w;
-    if (int rc = make_map(&map_x, x, chunk, box_rows)) return rc;
-    if (int rc = make_map(&map_w, w, chunk, b_mn ? 64 : paired ? 128 : bn)) return rc;
-    MmaArgs a{};
-    a.offsets = d_offsets, a.order = d_order, a.x_scales = d_x_scales, a.w_scales = d_w_scales, a.y = d_y;
-    a.m = num_rows, a.x_rows = x_rows, a.choices = choices, a.groups = groups, a.inner = inner, a.outer = outer;
-    a.type = type, a.out_type = out_type, a.format = w.type == FG_BF16 ? 1 : 0;
-    a.b_mn = b_mn, a.shared_weight = w_group == 0, a.box_rows = box_rows;
-    const int64_t tiles = units * ((outer + (paired ? 256 : bn) - 1) / (paired ? 256 : bn));
-    return type == FG_E4M3  ? launch<kEight, false>(bn, a, map_x, map_w, tiles, s)
-           : type == FG_F32 ? launch<kParts, false>(bn, a, map_x, map_w, tiles, s)
-                            : launch<kHalf, false>(bn, a, map_x, map_w, tiles, s);
+    const Problem p{d_offsets, d_order, num_rows, x_rows, choices, groups, inner, outer, type};
+    Matrix x{};
+    const int64_t held = held_bytes(num_rows, inner, type);
+    if (!held)
+        if (int rc = rows_matrix(&x, d_x, ldx, x_rows, d_order, choices, num_rows, inner, type, &work, s)) return rc;
+    return run_product(p, x, d_x, ldx, d_x_scales, d_w, w_group, w_out, w_in, d_w_scales, held, d_y, out_type, &work, s);
 }
 
-int64_t fg_grouped_matmul_wgrad_workspace(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const int32_t* d_order,
-                                          int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
+int64_t fg_grouped_matmul_backward_workspace(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,
+                                             const int32_t* d_order, const void* d_dy, int64_t lddy, int32_t want_dx, int32_t want_dw,
+                                             int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
     if (num_rows <= 0 || groups < 1 || inner < 1 || outer < 1) return 0;
-    return partial_bytes(num_rows, groups, inner, outer) +
-           (rows_need_copy(d_x, ldx ? ldx : inner, d_order, type) ? packed_bytes(num_rows, inner, type) : 0) +
-           (rows_need_copy(d_dy, lddy ? lddy : outer, nullptr, type) ? packed_bytes(num_rows, outer, type) : 0);
+    const Problem p{nullptr, d_order, num_rows, 0, 1, groups, inner, outer, type};
+    return (rows_need_copy(d_dy, lddy ? lddy : outer, nullptr, type) ? packed_bytes(num_rows, outer, type) : 0) +
+           (want_dx ? weight_bytes(other_way(p), d_w, w_group, w_in, w_out) : 0) +
+           (want_dx && d_order ? round_up(num_rows * (int64_t)inner * fg::type_size(type), 256) : 0) +
+           (want_dw ? partial_bytes(num_rows, groups, inner, outer) : 0) +
+           (want_dw && rows_need_copy(d_x, ldx ? ldx : inner, d_order, type) ? packed_bytes(num_rows, inner, type) : 0);
 }
 
-int fg_grouped_matmul_wgrad(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const int32_t* d_offsets,
-                            const int32_t* d_order, int32_t choices, int64_t x_rows, void* d_dw, int64_t num_rows, int32_t groups,
-                            int32_t inner, int32_t outer, int32_t type, void* d_workspace, int64_t workspace_bytes, void* stream) {
+int fg_grouped_matmul_backward(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,
+                               const int32_t* d_offsets, const int32_t* d_order, const int32_t* d_position, int32_t choices, int64_t x_rows,
+                               const void* d_dy, int64_t lddy, void* d_dx, void* d_dw, int64_t num_rows, int32_t groups, int32_t inner,
+                               int32_t outer, int32_t type, void* d_workspace, int64_t workspace_bytes, void* stream) {
     if (int rc = check_product(num_rows, x_rows, choices, groups, inner, outer, type)) return rc;
     if (!fg::float_type(type)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "unknown value type %d", type);
     if (ldx == 0) ldx = inner;
     if (lddy == 0) lddy = outer;
     if (ldx < inner || lddy < outer) return fg::fail(FG_ERR_INVALID_ARGUMENT, "row strides must be 0 or >= the width");
-    if (!d_dw || !d_offsets || (num_rows && (!d_x || !d_dy))) return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
-    if (!d_order && x_rows != num_rows) return fg::fail(FG_ERR_INVALID_ARGUMENT, "without an order x has a row for each slot");
+    if (w_group < 0 || w_out < 0 || w_in < 0) return fg::fail(FG_ERR_INVALID_ARGUMENT, "the weight's strides must be >= 0");
+    if (!d_dx && !d_dw) return FG_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const int64_t cells = (int64_t)inner * outer;
-    if (num_rows == 0) {
-        FG_CUDA_TRY(cudaMemsetAsync(d_dw, 0, (size_t)(groups * cells * fg::type_size(type)), s));
+    if (num_rows == 0) {  // no slots: no rows of x either
+        if (d_dw) FG_CUDA_TRY(cudaMemsetAsync(d_dw, 0, (size_t)groups * inner * outer * fg::type_size(type), s));
         return FG_OK;
     }
-    const int64_t split = split_rows(num_rows, groups, wgrad_tiles(inner, outer));
-    const int64_t need = fg_grouped_matmul_wgrad_workspace(d_x, ldx, d_dy, lddy, d_order, num_rows, groups, inner, outer, type);
-    if (workspace_bytes < need || (need && !d_workspace)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_grouped_matmul_wgrad_workspace()");
+    if (!d_offsets || !d_dy || (d_dw && !d_x) || (d_dx && !d_w) || (d_order && !d_position))
+        return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
+    if (!d_order && x_rows != num_rows) return fg::fail(FG_ERR_INVALID_ARGUMENT, "without an order x has a row for each slot");
+    if (d_order && x_rows * choices != num_rows) return fg::fail(FG_ERR_INVALID_ARGUMENT, "the order lists `choices` slots a row of x");
+    const int64_t need = fg_grouped_matmul_backward_workspace(d_x, ldx, d_w, w_group, w_out, w_in, d_order, d_dy, lddy, d_dx != nullptr, d_dw != nullptr,
+                                                              num_rows, groups, inner, outer, type);
+    if (workspace_bytes < need || (need && !d_workspace))
+        return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_grouped_matmul_backward_workspace()");
     uint8_t* work = static_cast<uint8_t*>(d_workspace);
+    const Problem p{d_offsets, d_order, num_rows, x_rows, choices, groups, inner, outer, type};
+    Matrix dy;
+    if (int rc = rows_matrix(&dy, d_dy, lddy, num_rows, nullptr, 1, num_rows, outer, type, &work, s)) return rc;
+    if (d_dx) {
+        // A gathered row's gradient is the sum over its slots: each slot's part in x's type (one more rounding than the sum
+        // itself has, half the bytes of 32-bit parts), their sum in 32 bits.
+        void* parts = d_dx;
+        if (d_order) {
+            parts = work;
+            work += round_up(num_rows * (int64_t)inner * fg::type_size(type), 256);
+        }
+        if (int rc = run_product(other_way(p), dy, nullptr, 0, nullptr, d_w, w_group, w_in, w_out, nullptr, 0, parts, type, &work, s)) return rc;
+        if (d_order)
+            if (int rc = fg_combine_rows(parts, 0, nullptr, d_position, d_dx, x_rows, choices, inner, type, stream)) return rc;
+    }
+    if (!d_dw) return FG_OK;
     float* sums = reinterpret_cast<float*>(work);
     work += partial_bytes(num_rows, groups, inner, outer);
-    Matrix x, dy;
+    Matrix x;
     if (int rc = rows_matrix(&x, d_x, ldx, x_rows, d_order, choices, num_rows, inner, type, &work, s)) return rc;
-    if (int rc = rows_matrix(&dy, d_dy, lddy, num_rows, nullptr, 1, num_rows, outer, type, &work, s)) return rc;
-    CUtensorMap map_x, map_dy;
-    if (int rc = make_map(&map_dy, dy, 64, 64)) return rc;
-    if (int rc = make_map(&map_x, x, 64, 64)) return rc;
-    const int64_t units = split ? num_rows / split + groups : groups, rows_tiles = (outer + kTileRows - 1) / kTileRows;
-    // in pairs, the columns' waste counts as well as the rows'
-    const int64_t singles = units * rows_tiles * ((inner + 127) / 128), doubles = units * ((outer + 255) / 256) * ((inner + 255) / 256);
-    const bool paired = pairs_pay(singles, doubles * 2, 256, type);
-    const int bn = paired ? 512 : tile_width(units * rows_tiles, inner, type);
-    MmaArgs a{};
-    a.offsets = d_offsets, a.order = d_order, a.y = split ? static_cast<void*>(sums) : d_dw;
-    a.m = num_rows, a.x_rows = x_rows, a.choices = choices, a.groups = groups, a.inner = inner, a.outer = outer;
-    a.type = type, a.out_type = split ? FG_F32 : type, a.format = dy.type == FG_BF16 ? 1 : 0;
-    a.split = (int32_t)split, a.units = (int32_t)units;
-    const int64_t tiles = paired ? doubles : units * rows_tiles * ((inner + bn - 1) / bn);
-    if (int rc = type == FG_F32 ? launch<kParts, true>(bn, a, map_dy, map_x, tiles, s) : launch<kHalf, true>(bn, a, map_dy, map_x, tiles, s)) return rc;
-    if (split) {
-        const dim3 grid((unsigned)((cells + 255) / 256 < 4096 ? (cells + 255) / 256 : 4096), (unsigned)groups);
-        if (type == FG_F32) join_kernel<float><<<grid, 256, 0, s>>>(sums, d_offsets, groups, num_rows, (int)split, a.units, cells, static_cast<float*>(d_dw));
-        else if (type == FG_F16) join_kernel<__half><<<grid, 256, 0, s>>>(sums, d_offsets, groups, num_rows, (int)split, a.units, cells, static_cast<__half*>(d_dw));
-        else join_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(sums, d_offsets, groups, num_rows, (int)split, a.units, cells, static_cast<__nv_bfloat16*>(d_dw));
-        FG_CUDA_TRY(cudaGetLastError());
-        fg::count_launches(1);
-    }
-    return FG_OK;
+    return run_weight_gradient(p, x, dy, d_dw, sums, s);
 }
 
 }  // extern "C"

@@ -387,22 +387,18 @@ class _Product(torch.autograd.Function):
         x, w = ctx.saved_tensors
         groups, gather = ctx.groups, ctx.gather
         outer, inner = w.shape[1], w.shape[2]
+        want_dx, want_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         dyr, ldy = _as_rows(dy)
-        dx = dw = None
-        if ctx.needs_input_grad[0]:
-            # per slot first, in x's type; with k slots a row their sum is then taken in 32 bits
-            dx = _product(dyr, ldy, None, w, (w.stride(0), w.stride(2), w.stride(1)), None, groups, False, dyr.shape[0], outer, inner, x.dtype)
-            if gather:
-                dx = _combine(dx, groups, None)
-        if ctx.needs_input_grad[1]:
-            xr, ldx = _as_rows(x)
-            kind = _TYPES[x.dtype]
-            dw = torch.empty(w.shape, dtype=w.dtype, device=w.device)
-            order, m = (groups.order.data_ptr() if gather else None), groups.num_entries
-            size = _size("fg_grouped_matmul_wgrad_workspace", xr.data_ptr(), ldx, dyr.data_ptr(), ldy, order, m, groups.num_groups, inner, outer, kind)
-            work = torch.empty(size, dtype=torch.uint8, device=w.device) if size else None
-            _call("fg_grouped_matmul_wgrad", x.get_device(), xr.data_ptr(), ldx, dyr.data_ptr(), ldy, groups.offsets.data_ptr(),
-                  order, groups.choices, x.shape[0], dw.data_ptr(), m, groups.num_groups, inner, outer, kind, _ptr(work), size)
+        xr, ldx = _as_rows(x)
+        device, kind, m, g = x.device, _TYPES[x.dtype], groups.order.numel(), groups.offsets.numel() - 1
+        dx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_dx else None
+        dw = torch.empty(w.shape, dtype=w.dtype, device=device) if want_dw else None
+        order, position = (groups.order.data_ptr(), groups.position.data_ptr()) if gather else (None, None)
+        operands = (xr.data_ptr(), ldx, w.data_ptr(), *w.stride())
+        size = _size("fg_grouped_matmul_backward_workspace", *operands, order, dyr.data_ptr(), ldy, want_dx, want_dw, m, g, inner, outer, kind)
+        work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
+        _call("fg_grouped_matmul_backward", x.get_device(), *operands, groups.offsets.data_ptr(), order, position, groups.position.shape[1],
+              x.shape[0], dyr.data_ptr(), ldy, _ptr(dx), _ptr(dw), m, g, inner, outer, kind, _ptr(work), size)
         return dx, dw, None, None
 
 

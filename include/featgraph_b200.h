@@ -390,18 +390,24 @@ int fg_group_rows(const int32_t* d_keys, int64_t num_entries, int32_t num_groups
  * y[p, o] = sum over i of x[row(p), i] * w[g, o, i] for the rows p of each group g; rows in no group are 0.
  * row(p) = p where d_order is NULL, else d_order[p] / choices.  w[g, o, i] is d_w[g w_group + o w_out + i w_in].
  * FG_E4M3: times d_x_scales[row(p)] * d_w_scales[g * outer + o], output of out_type.  y dense, [num_rows, outer].
- * fg_grouped_matmul_wgrad: d_dw[g, o, i] = sum over the rows p of g of dy[p, o] * x[row(p), i], dense. */
+ * fg_grouped_matmul_backward, either output NULL where it is not wanted: d_dx[t, i] = sum over the slots p of row t of
+ * sum over o of w[g, o, i] * dy[p, o] (rows without a slot are 0), d_dw[g, o, i] = sum over the rows p of g of
+ * dy[p, o] * x[row(p), i]; both dense.  d_position: the inverse of d_order, where that is given.
+ * fp32 products: sums of six bf16 products of three parts of each operand, 2^-24 of the terms off; an infinity among
+ * the operands gives NaN. */
 int64_t fg_grouped_matmul_workspace(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,
                                     const int32_t* d_order, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type);
 int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, const void* d_w, int64_t w_group, int64_t w_out,
                       int64_t w_in, const float* d_w_scales, const int32_t* d_offsets, const int32_t* d_order, int32_t choices,
                       int64_t x_rows, void* d_y, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type,
                       int32_t out_type, void* d_workspace, int64_t workspace_bytes, void* stream);
-int64_t fg_grouped_matmul_wgrad_workspace(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const int32_t* d_order,
-                                          int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type);
-int fg_grouped_matmul_wgrad(const void* d_x, int64_t ldx, const void* d_dy, int64_t lddy, const int32_t* d_offsets,
-                            const int32_t* d_order, int32_t choices, int64_t x_rows, void* d_dw, int64_t num_rows, int32_t groups,
-                            int32_t inner, int32_t outer, int32_t type, void* d_workspace, int64_t workspace_bytes, void* stream);
+int64_t fg_grouped_matmul_backward_workspace(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,
+                                             const int32_t* d_order, const void* d_dy, int64_t lddy, int32_t want_dx, int32_t want_dw,
+                                             int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type);
+int fg_grouped_matmul_backward(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,
+                               const int32_t* d_offsets, const int32_t* d_order, const int32_t* d_position, int32_t choices, int64_t x_rows,
+                               const void* d_dy, int64_t lddy, void* d_dx, void* d_dw, int64_t num_rows, int32_t groups, int32_t inner,
+                               int32_t outer, int32_t type, void* d_workspace, int64_t workspace_bytes, void* stream);
 
 /* out[t] = sum over j of weights[t, j] * y[position[t * k + j]] (entries with position -1 are left out; d_weights may
  * be NULL: ones), and its gradients: d_dy [n k, d] (rows from d_offsets[num_groups] on are 0) and d_dweights [n, k],

@@ -101,7 +101,11 @@ def test_c_entries_report_bad_arguments():
     refused("fg_grouped_matmul", 1, 0, None, 1, 40, 8, 1, None, 1, None, 0, 4, 1, 4, 2, 8, 5, 0, 0, None, 0, None, text=b"bad sizes")
     refused("fg_grouped_matmul", 1, 0, None, 1, 40, 8, 1, None, 1, None, 1, 4, 1, 4, 2, 8, 5, 3, 2, None, 0, None, text=b"NULL")
     refused("fg_grouped_matmul", 1, 0, None, 1, 40, 8, 1, None, 1, None, 1, 4, 1, 4, 2, 8, 5, 0, 2, None, 0, None, text=b"inputs' type")
-    refused("fg_grouped_matmul_wgrad", 1, 0, 1, 4, 1, None, 1, 4, 1, 4, 2, 8, 5, 0, None, 0, None, text=b"row strides")
+    refused("fg_grouped_matmul_backward", 1, 0, 1, 40, 8, 1, 1, None, None, 1, 4, 1, 4, 1, 1, 4, 2, 8, 5, 0, None, 0, None, text=b"row strides")
+    refused("fg_grouped_matmul_backward", 1, 0, 1, 40, 8, 1, 1, 1, None, 1, 4, 1, 0, 1, 1, 4, 2, 8, 5, 2, None, 0, None, text=b"NULL")
+    refused("fg_grouped_matmul_backward", 1, 0, 1, 40, 8, 1, 1, 1, 1, 2, 4, 1, 0, 1, 1, 4, 2, 8, 5, 2, None, 0, None, text=b"choices")
+    refused("fg_grouped_matmul_backward", 1, 0, 1, 40, 8, 1, 1, None, None, 1, 4, 1, 0, 1, 1, 4, 2, 8, 5, 0, None, 0, None, text=b"workspace")
+    refused("fg_grouped_matmul_backward", 1, 0, 1, 40, 8, 1, 1, None, None, 1, 4, 1, 0, 1, 1, 4, 2, 8, 5, 3, None, 0, None, text=b"value type")
     refused("fg_combine_rows", 1, 0, None, 1, 1, 4, 33, 8, 0, None, text=b"bad sizes")
     refused("fg_combine_rows_backward", 1, 0, None, None, 1, 2, 1, 0, 1, None, 4, 2, 8, 0, None, text=b"NULL")
     # nothing to do is no error
