@@ -21,6 +21,7 @@
 // tile loads' rate.  Measured at 65536 x 2048 x 4096 in bf16: 2767 us with gather loads in the ring, 922 us for rows in
 // slot order, the copy about 70 us; dW 8512 against 1241 us.  The same kernel copies an operand that TMA cannot read (a
 // row pitch or a start off the 16-byte grid, two strides above 1) and cuts fp32 into parts.
+#include <atomic>
 #include <climits>
 #include <mutex>
 #include <type_traits>
@@ -945,9 +946,9 @@ int launch_shape(const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& 
     cluster.val.clusterDim.x = BLOCKS, cluster.val.clusterDim.y = 1, cluster.val.clusterDim.z = 1;
     config.attrs = &cluster;
     config.numAttrs = BLOCKS == 2 ? 1 : 0;
-    static int resident[fg::kMaxDevices];  // blocks (pairs) that run at once; found once a device, twice does no harm
+    static std::atomic<int> resident[fg::kMaxDevices];  // blocks (pairs) that run at once; found once a device, twice does no harm
     const int slot = fg::current_device_slot();
-    int most = slot < 0 ? 0 : resident[slot];
+    int most = slot < 0 ? 0 : resident[slot].load();
     if (most == 0) {
         FG_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
         most = fg::device_props().sm_count;
@@ -956,7 +957,7 @@ int launch_shape(const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& 
             FG_CUDA_TRY(cudaOccupancyMaxActiveClusters(&most, kernel, &config));
             if (most < 1) return fg::fail(FG_ERR_CUDA, "no room for a pair of blocks");
         }
-        if (slot >= 0) resident[slot] = most;
+        if (slot >= 0) resident[slot].store(most);
     }
     config.gridDim = dim3((unsigned)(most_tiles < most ? most_tiles : most) * BLOCKS);
     FG_CUDA_TRY(cudaLaunchKernelEx(&config, kernel, a, map_a, map_b));

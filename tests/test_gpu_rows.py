@@ -427,6 +427,49 @@ def test_product_of_8_bit_rows(n, k, count, inner, outer, out):
     assert torch.equal(grouped_matmul(x, w, groups, gather=True).double(), grouped_matmul(x, odd, groups, gather=True).double())
 
 
+def test_gradients_are_not_differentiable_again():
+    from featgraph.module import combine_rows, grouped_matmul, rms_norm, route
+    x = normal((6, 8), 1).requires_grad_(True)
+    groups = make_groups(6, 1, 2, 5)
+    w = normal((2, 8, 8), 2).requires_grad_(True)
+    for out in (rms_norm(x), route(x, 2).weights, grouped_matmul(x, w, groups), combine_rows(x, groups)):
+        grad, = torch.autograd.grad(out.square().sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            grad.sum().backward()
+
+
+def test_expanded_gradients_and_repeated_choices():
+    """A sum's gradient arrives as an expanded tensor; a row may name the same group twice."""
+    from featgraph.module import combine_rows, group_rows, grouped_matmul, rms_norm
+    keys = torch.tensor([[0, 0], [1, 0], [2, 2], [-1, 1]], dtype=torch.int32, device="cuda")
+    groups = group_rows(keys, 3)
+    for t in sorted(TYPES):
+        dt = TYPES[t]
+        x, w = normal((4, 16), 1, dt).requires_grad_(True), normal((3, 8, 16), 2, dt).requires_grad_(True)
+        weights = normal((4, 2), 3).requires_grad_(True)
+        out = combine_rows(grouped_matmul(x, w, groups, gather=True), groups, weights)
+        got = torch.autograd.grad(out.sum(), (x, w, weights))
+        xd, wd, sd = (v.detach().double().requires_grad_(True) for v in (x, w, weights))
+        want = sum(torch.where(keys[:, j:j + 1] >= 0, sd[:, j:j + 1] * torch.einsum("ni,noi->no", xd, wd[keys[:, j].clamp(min=0).long()]), torch.zeros((), dtype=torch.float64, device="cuda"))
+                   for j in range(2))
+        # three roundings to the type on each way (slot, sum, gradient) of values below 8
+        close(out.detach(), want.detach(), 24 * half_step(dt) * (1 + want.detach().abs()), "out")
+        for a, b in zip(got, torch.autograd.grad(want.sum(), (xd, wd, sd))):
+            close(a, b, 24 * half_step(dt) * (1 + b.abs().max()), "gradients")
+        y = normal((5, 24), 4, dt).requires_grad_(True)
+        g = normal((24,), 5).requires_grad_(True)  # a 32-bit weight beside rows of fewer bits
+        dy, dg = torch.autograd.grad(rms_norm(y, g).sum(), (y, g))
+        assert dg.dtype == torch.float32
+        yd, gd = y.detach().double().requires_grad_(True), g.detach().double().requires_grad_(True)
+        by, bg = torch.autograd.grad(norm_reference_graph(yd, gd).sum(), (yd, gd))
+        close(dy, by, half_step(dt) * by.abs() + 200 * U * (1 + by.abs().max()), "dx")
+        close(dg, bg, 200 * U * (1 + bg.abs().max()), "dweight")
+
+
+def norm_reference_graph(h, w, eps=1e-6):
+    return h / torch.sqrt(h.pow(2).mean(-1, keepdim=True) + eps) * w
+
+
 def test_product_from_a_thread_that_made_no_cuda_call_yet():
     """A host thread has no CUDA context until its first runtime call; the tensor maps need one."""
     import threading
