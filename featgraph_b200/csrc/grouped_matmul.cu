@@ -12,9 +12,9 @@
 // stored.  In dW they would be terms of the sum, so they are overwritten with zeros in shared memory, in both
 // operands - a zero times their infinities or NaN would still be NaN - before the last products of the group.
 //
-// fp32: no tensor-core type holds it, so x and w are each cut into three bf16 parts of 8 bits (x = a + b + c exactly up to
-// 2^-24) and six products of parts are summed, smallest first: a c', b b', c a', a b', b a', a a'; the parts left out are
-// below 2^-24 of the result's terms.  Six bf16 products against one fp32 product on the scalar units.
+// fp32: no tensor-core type holds it, so x and w are each cut into three bf16 parts of 8 bits (x = a + b + c exactly) and six
+// products of parts are summed, smallest first: a c', b b', c a', a b', b a', a a'; the parts left out, b c', c b' and
+// c c', are below 2^-23 of a term.  Six bf16 products against one fp32 product on the scalar units.
 //
 // Rows that are gathered (slot p reads row order[p] / choices) are first copied into slot order: every column tile reads
 // them again, and row-gather TMA loads (tile::gather4, four rows an instruction) move a 128-row tile at a fraction of the
@@ -57,7 +57,8 @@ struct MmaArgs {
     bool vector_rows;      // rows on the 16-byte grid
 };
 
-enum Kind { kHalf, kEight, kParts };  // 16-bit values, e4m3, fp32 in three bf16 parts
+// 16-bit values, e4m3, fp32 in three bf16 parts; kCut: the weight in parts, the rows as they are, cut on their way
+enum Kind { kHalf, kEight, kParts, kCut };
 
 // Parts multiplied in each of the six products, smallest first.
 __host__ __device__ constexpr int part_a(int pair) { return (0x001102 >> (4 * pair)) & 3; }
@@ -75,7 +76,7 @@ __host__ __device__ constexpr int part_b(int pair) { return (0x010120 >> (4 * pa
 // and the first one's products read both shared memories (cta_group::2).
 template <int BN, Kind KIND, bool FEW, int BLOCKS>
 struct Shape {
-    static constexpr int kParts = KIND == Kind::kParts ? 3 : 1;
+    static constexpr int kParts = KIND == Kind::kParts || KIND == kCut ? 3 : 1;
     static constexpr int kOwnCols = BN / BLOCKS;
     static constexpr int kA = FEW ? 0 : kTileRows * kChunkBytes, kB = kOwnCols * kChunkBytes;  // bytes of one part
     static constexpr int kDeep = FEW ? 2 : 1;  // 128-byte chunks a stage
@@ -83,14 +84,15 @@ struct Shape {
     static constexpr int kStages = 196608 / kStageBytes < 16 ? 196608 / kStageBytes : 16;  // at most
     static constexpr int kColumns = 2 * BN;
     static constexpr int kOutput = 8 * 2048;  // 2 KB for each output warp
-    static constexpr int kSmem = 1024 + kOutput + (FEW ? 196608 : kStages * kStageBytes);
+    static constexpr int kRaw = KIND == kCut ? 3 : 0, kRawBytes = kTileRows * 128;  // 32 fp32 values of each row
+    static constexpr int kSmem = 1024 + kOutput + kRaw * kRawBytes + (FEW ? 196608 : kStages * kStageBytes);
 };
 
 struct Tables {
-    uint64_t full[16], empty[16], tail[16], filled[2], drained[2], rows, last;
+    uint64_t full[16], empty[16], tail[16], filled[2], drained[2], raw[3], spent[3], rows, last;
     uint32_t tmem;
     int stop;
-    int warp_sums[11];
+    int warp_sums[19];
     int sources[32];            // few rows: the row of x behind each slot, or -1
     int start[kMaxGroups + 1];  // first slot of each group
     int tiles[kMaxGroups + 1];  // row tiles (partial sums of dW) before each group
@@ -193,16 +195,58 @@ __device__ __forceinline__ void hold_rows(const MmaArgs& a, uint32_t held, int c
     }
 }
 
+// Eight fp32 values in three bf16 parts each, by cutting 16 bits off: x = a + b + c exactly (8 bits of its 24 each), and no
+// conversion, which rounding to bf16 would take (at a fraction of the multiply-adds' rate).
+__device__ __forceinline__ void cut_values(const float (&v)[8], Pack<__nv_bfloat16, 8> (&p)[3]) {
+    uint32_t part[3][8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        part[0][j] = __float_as_uint(v[j]);
+        const float rest = __fsub_rn(v[j], __uint_as_float(part[0][j] & 0xffff0000u));
+        part[1][j] = __float_as_uint(rest);
+        part[2][j] = __float_as_uint(__fsub_rn(rest, __uint_as_float(part[1][j] & 0xffff0000u)));
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(&p[k])[j] = __byte_perm(part[k][2 * j], part[k][2 * j + 1], 0x7632);
+}
+
+// Half `h` of a chunk: 32 fp32 values of 128 rows at `raw` (128 bytes a row, 16-byte cells XOR-swizzled) to that half of the
+// three parts' tiles at `stage`, 16 KB each, laid the same way.  256 threads, 8 values each, twice.
+__device__ __forceinline__ void cut_rows(uint32_t raw, uint32_t stage, int h, int thread) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int unit = thread + u * 256, r = unit >> 2, q = unit & 3, x = r & 7;
+        float v[8];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+            asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];"
+                         : "=f"(v[4 * e]), "=f"(v[4 * e + 1]), "=f"(v[4 * e + 2]), "=f"(v[4 * e + 3])
+                         : "r"(raw + r * 128 + (((2 * q + e) ^ x) << 4))
+                         : "memory");
+        Pack<__nv_bfloat16, 8> p[3];
+        cut_values(v, p);
+#pragma unroll
+        for (int k = 0; k < 3; ++k) {
+            const uint32_t* word = reinterpret_cast<const uint32_t*>(&p[k]);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + k * kTileRows * kChunkBytes + r * 128 + (((h * 4 + q) ^ x) << 4)),
+                         "r"(word[0]), "r"(word[1]), "r"(word[2]), "r"(word[3])
+                         : "memory");
+        }
+    }
+}
+
 // A wait of all lanes, with one answer for all of them.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* stop) {
     return __all_sync(0xffffffffu, fg::barrier_wait(bar, parity, stop));
 }
 
-template <bool WGRAD>
-constexpr int kThreads = WGRAD ? 352 : 320;
+template <Kind KIND, bool WGRAD>
+constexpr int kThreads = KIND == kCut ? 608 : WGRAD ? 352 : 320;
 
 template <int BN, Kind KIND, bool WGRAD, bool FEW, int BLOCKS>
-__global__ void __launch_bounds__(kThreads<WGRAD>, 1)
+__global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
     product_kernel(const MmaArgs a, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
     using S = Shape<BN, KIND, FEW, BLOCKS>;
     constexpr bool EIGHT = KIND == kEight;
@@ -219,13 +263,17 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
-            fg::barrier_init(fg::smem_address(&t.full[s]), BLOCKS);
+            fg::barrier_init(fg::smem_address(&t.full[s]), KIND == kCut ? 8 : BLOCKS);
             fg::barrier_init(fg::smem_address(&t.tail[s]), 1);
             fg::barrier_init(fg::smem_address(&t.empty[s]), 1);
         }
         for (int s = 0; s < 2; ++s) {
             fg::barrier_init(fg::smem_address(&t.filled[s]), 1);
             fg::barrier_init(fg::smem_address(&t.drained[s]), 8 * BLOCKS);
+        }
+        for (int s = 0; s < S::kRaw; ++s) {
+            fg::barrier_init(fg::smem_address(&t.raw[s]), 1);
+            fg::barrier_init(fg::smem_address(&t.spent[s]), 8);
         }
         fg::barrier_init(fg::smem_address(&t.rows), 8);
         fg::barrier_init(fg::smem_address(&t.last), 1);
@@ -247,7 +295,7 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
 
     // groups' first slots and tile counts, scanned: thread i takes groups [i * each, (i + 1) * each)
     {
-        constexpr int kAll = kThreads<WGRAD>;
+        constexpr int kAll = kThreads<KIND, WGRAD>;
         const int each = (a.groups + kAll - 1) / kAll, from = min((int)threadIdx.x * each, a.groups), to = min(from + each, a.groups);
         const int64_t unit = WGRAD ? (a.split ? a.split : (int64_t)INT_MAX) : kRows;
         int own = 0;
@@ -342,13 +390,14 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
                     return WGRAD || a.b_mn ? max(min(S::kOwnCols / 64, ((WGRAD ? a.inner : a.outer) - at + 63) / 64), 0) : S::kOwnCols / 64;
                 };
                 const int a_blocks = blocks_a(w.row), b_blocks = blocks_b(col);
-                const uint32_t own = ((WGRAD ? a_blocks * 8192 : S::kA) + b_blocks * 8192) * S::kParts * S::kDeep;
+                const uint32_t own = ((WGRAD ? a_blocks * 8192 : KIND == kCut ? 0 : S::kA) + b_blocks * 8192) * S::kParts * S::kDeep;
                 uint32_t bytes = own;
                 if (BLOCKS == 2)  // the first block's barrier counts the second one's loads too
                     bytes += ((WGRAD ? blocks_a(w.row + kTileRows) * 8192 : S::kA) + blocks_b(col + S::kOwnCols) * 8192) * S::kParts;
                 for (int c = 0; c < w.chunks; ++c, ++step) {
                     const int at_stage = s;
-                    const uint32_t full = fg::smem_address(&t.full[s]), stage = ring + s * S::kStageBytes;
+                    // (cut rows: the weights have a barrier of their own, the stage's counts the cutting warps)
+                    const uint32_t full = fg::smem_address(KIND == kCut ? &t.tail[s] : &t.full[s]), stage = ring + s * S::kStageBytes;
                     if (!fg::barrier_wait(fg::smem_address(&t.empty[s]), parity, stop)) {
                         live = false;
                         break;
@@ -383,7 +432,7 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
                             for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d<BLOCKS>(bt + q * 8192, &map_b, col + q * 64, slot, full);
                         } else {
                             const int g = a.shared_weight ? p : w.group + p * a.groups;
-                            if (!FEW) fg::tma_load_2d<BLOCKS>(at, &map_a, k, w.begin + p * (int)a.m, full);
+                            if (!FEW && KIND != kCut) fg::tma_load_2d<BLOCKS>(at, &map_a, k, w.begin + p * (int)a.m, full);
 #pragma unroll
                             for (int h = 0; h < S::kDeep; ++h) {
                                 const int kh = k + h * (kChunk / S::kDeep);
@@ -398,12 +447,14 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
                     }
                 }
             }
-            if (*stop)  // no copy may be in flight when the block (or its pair) ends
+            if (*stop) {  // no copy may be in flight when the block (or its pair) ends
                 for (int64_t q = max(step - stages, (int64_t)0); q < step; ++q) {
                     const int at = (int)(q % stages);
-                    if (tail_now >> at & 1) fg::barrier_wait(fg::smem_address(&t.tail[at]), ~tail_parity >> at & 1, stop, true);
+                    if (KIND == kCut) fg::barrier_wait(fg::smem_address(&t.tail[at]), (q / stages) & 1, stop, true);
+                    else if (tail_now >> at & 1) fg::barrier_wait(fg::smem_address(&t.tail[at]), ~tail_parity >> at & 1, stop, true);
                     else if (rank == 0) fg::barrier_wait(fg::smem_address(&t.full[at]), (q / stages) & 1, stop, true);
                 }
+            }
         }
         __syncwarp();
     } else if (warp == 1) {
@@ -423,6 +474,7 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
                 for (int c = 0; c < w.chunks; ++c) {
                     const uint32_t stage = ring + s * S::kStageBytes, empty = fg::smem_address(&t.empty[s]);
                     live = fg::barrier_wait<BLOCKS == 2 && WGRAD>(fg::smem_address(&t.full[s]), parity, stop);
+                    if (KIND == kCut) live = live && fg::barrier_wait(fg::smem_address(&t.tail[s]), parity, stop);
                     if (++s == stages) s = 0, parity ^= 1;
                     if (!live) break;
                     fg::tcgen05_after_sync();
@@ -451,6 +503,51 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
             }
         }
         __syncwarp();
+    } else if (KIND == kCut && warp == 18) {
+        if (fg::elect_one()) {  // the rows, half a chunk a load, ahead of the weights' stages
+            int raw = 0, parity = 1;
+            int64_t loads = 0;
+            bool live = true;
+            for (int64_t i = start; live && i < total; i += stride) {
+                const Tile w = locate(i);
+                for (int h = 0; h < 2 * w.chunks; ++h, ++loads) {
+                    live = fg::barrier_wait(fg::smem_address(&t.spent[raw]), parity, stop);
+                    if (!live) break;
+                    const uint32_t bar = fg::smem_address(&t.raw[raw]);
+                    fg::barrier_expect(bar, S::kRawBytes);
+                    fg::tma_load_2d<1>(ring + S::kStages * S::kStageBytes + raw * S::kRawBytes, &map_a, h * 32, w.begin, bar);
+                    if (++raw == S::kRaw) raw = 0, parity ^= 1;
+                }
+            }
+            if (*stop)
+                for (int64_t q = max(loads - S::kRaw, (int64_t)0); q < loads; ++q)
+                    fg::barrier_wait(fg::smem_address(&t.raw[q % 3]), (q / 3) & 1, stop, true);
+        }
+        __syncwarp();
+    } else if (KIND == kCut && warp >= 10) {
+        // x = a + b + c: 8 values a thread and step, from 32 bytes of a raw row to 16 bytes of each part's row
+        int s = 0, parity = 1, raw = 0, raw_parity = 0;
+        bool live = true;
+        for (int64_t i = start; live && i < total; i += stride) {
+            const Tile w = locate(i);
+            for (int c = 0; live && c < w.chunks; ++c) {
+                const uint32_t stage = ring + s * S::kStageBytes;
+                live = warp_wait(fg::smem_address(&t.empty[s]), parity, stop);
+                for (int h = 0; live && h < 2; ++h) {
+                    live = warp_wait(fg::smem_address(&t.raw[raw]), raw_parity, stop);
+                    if (!live) break;
+                    cut_rows(ring + S::kStages * S::kStageBytes + raw * S::kRawBytes, stage, h, threadIdx.x - 320);
+                    __syncwarp();
+                    if (lane == 0) fg::barrier_arrive(fg::smem_address(&t.spent[raw]));
+                    if (++raw == S::kRaw) raw = 0, raw_parity ^= 1;
+                }
+                if (!live) break;
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) fg::barrier_arrive(fg::smem_address(&t.full[s]));
+                if (++s == stages) s = 0, parity ^= 1;
+            }
+        }
     } else if (WGRAD && warp == 10) {
         // In a group's last chunk, the rows that are not its own become zeros, as far as the last step of 16 reaches: 128
         // bytes a row, 64 rows a column block.
@@ -479,7 +576,7 @@ __global__ void __launch_bounds__(kThreads<WGRAD>, 1)
     } else {
         const int quarter = warp & 3;  // the lanes of tensor memory this warp can read
         const int half = (warp - 2) >> 2;
-        const uint32_t staging = ring + stages * S::kStageBytes + (warp - 2) * 2048;
+        const uint32_t staging = ring + stages * S::kStageBytes + S::kRaw * S::kRawBytes + (warp - 2) * 2048;
         if (FEW && start < total) {
             hold_rows<EIGHT>(a, held, held_chunk, t.sources, threadIdx.x - 64);
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -775,19 +872,7 @@ __global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
             const int64_t at = line * a.pitch + c;
             if constexpr (sizeof(T) == 4) {
                 Pack<__nv_bfloat16, 8> p[3];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const float x = v[j];
-                    // a finite value that would round to infinity is cut instead; of an infinity or NaN the other parts are 0
-                    const bool finite = isfinite(x);
-                    __nv_bfloat16 hi = __float2bfloat16_rn(x);
-                    if (finite && isinf(__bfloat162float(hi))) hi = __float2bfloat16_rz(x);
-                    const float rest = finite ? __fsub_rn(x, __bfloat162float(hi)) : 0.0f;
-                    const __nv_bfloat16 mid = __float2bfloat16_rn(rest);
-                    p[0].v[j] = hi;
-                    p[1].v[j] = mid;
-                    p[2].v[j] = __float2bfloat16_rn(__fsub_rn(rest, __bfloat162float(mid)));
-                }
+                cut_values(v, p);
                 for (int k = 0; k < 3; ++k) store_pack<__nv_bfloat16, 8>(static_cast<__nv_bfloat16*>(a.dst) + k * plane + at, p[k]);
             } else {
                 Pack<T, kPer> p;
@@ -832,7 +917,7 @@ int make_map(CUtensorMap* map, const Matrix& m, int box_cols, int box_rows) {
     const cuuint64_t dims[3] = {(cuuint64_t)m.cols, (cuuint64_t)m.rows, (cuuint64_t)(m.groups ? m.groups : 1)};
     const cuuint64_t strides[2] = {(cuuint64_t)(m.pitch * size), (cuuint64_t)(m.group_stride * size)};
     const cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1}, ones[3] = {1, 1, 1};
-    const CUtensorMapDataType type = m.type == FG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : m.type == FG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+    const CUtensorMapDataType type = m.type == FG_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : m.type == FG_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : m.type == FG_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
     auto run = [&] {
         return encode(map, type, m.groups ? 3 : 2, const_cast<void*>(m.data), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE,
                       CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -882,6 +967,12 @@ int pack(const void* src, int64_t s0, int64_t s1, int64_t s2, int64_t groups, in
 
 // The slots' rows [m, cols] as a loadable matrix: where they lie, or copied.
 bool rows_need_copy(const void* p, int64_t ld, const int32_t* order, int32_t type) { return order || !loadable(p, ld, 0, type); }
+// fp32 rows that a product takes as they are (kCut): on the 16-byte grid, in slot order, and at most two column tiles, each of
+// which cuts them again.  100003 rows, 7 groups: 256 to 128 columns 70 us, in parts beforehand 89; 64 to 64: 20 and 26; but 128
+// to 256 79 and 68.
+bool rows_cut_on_the_way(const void* p, int64_t ld, const int32_t* order, int32_t outer, int32_t type) {
+    return type == FG_F32 && !order && outer <= 128 && fg::aligned16(p) && ld % 4 == 0 && ld < (1ll << 38);
+}
 int rows_matrix(Matrix* out, const void* p, int64_t ld, int64_t source_rows, const int32_t* order, int32_t choices, int64_t m, int64_t cols,
                 int32_t type, uint8_t** work, cudaStream_t s) {
     if (!rows_need_copy(p, ld, order, type)) {
@@ -938,7 +1029,7 @@ int launch_shape(const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& 
     constexpr int kSmem = Shape<BN, KIND, FEW, BLOCKS>::kSmem;
     const auto kernel = product_kernel<BN, KIND, WGRAD, FEW, BLOCKS>;
     cudaLaunchConfig_t config = {};
-    config.blockDim = dim3(kThreads<WGRAD>);
+    config.blockDim = dim3(kThreads<KIND, WGRAD>);
     config.dynamicSmemBytes = kSmem;
     config.stream = s;
     cudaLaunchAttribute cluster;
@@ -967,14 +1058,17 @@ int launch_shape(const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& 
 // bn 512 stands for pairs of blocks: 256 x 256 tiles.
 template <Kind KIND, bool WGRAD>
 int launch(int bn, const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b, int64_t most_tiles, cudaStream_t s) {
-    if constexpr (KIND != kParts) {
+    if constexpr (KIND == kCut) return launch_shape<64, kCut, false, false, 1>(a, map_a, map_b, most_tiles, s);
+    if constexpr (KIND != kParts && KIND != kCut) {
         if constexpr (!WGRAD)
             if (a.held) return launch_shape<64, KIND, false, true, 1>(a, map_a, map_b, most_tiles, s);
-        if (bn == 512) return launch_shape<256, KIND, WGRAD, false, 2>(a, map_a, map_b, most_tiles, s);
         if (bn == 256) return launch_shape<256, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s);
     }
-    return bn == 128 ? launch_shape<128, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s)
-                     : launch_shape<64, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s);
+    if constexpr (KIND != kCut)
+        if (bn == 512) return launch_shape<256, KIND, WGRAD, false, 2>(a, map_a, map_b, most_tiles, s);
+    if constexpr (KIND != kCut)
+        return bn == 128 ? launch_shape<128, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s)
+                         : launch_shape<64, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s);
 }
 
 // Columns of an output tile: the widest whose tiles still give each SM one (and of which two stages of parts fit).
@@ -986,8 +1080,8 @@ int tile_width(int64_t units, int width, int32_t type) {
 // Pairs of blocks (256 x 256 tiles) load a third less for the same products, which is what 128 x 256 tiles wait for, but
 // leave more of the last tiles empty: taken where the tiles they add are less than a tenth of all, and give
 // each pair two.  `rows_tiles`, `row_pairs`: 128- and 256-row tiles.
-bool pairs_pay(int64_t row_tiles, int64_t row_pairs, int width, int32_t type) {
-    if (type == FG_F32 || width <= 128) return false;
+bool pairs_pay(int64_t row_tiles, int64_t row_pairs, int width) {
+    if (width <= 128) return false;
     const int64_t cols = (width + 255) / 256;
     return row_pairs * cols >= fg::device_props().sm_count && row_pairs * 2 * 10 <= row_tiles * 11;
 }
@@ -1046,11 +1140,12 @@ int run_product(const Problem& p, const Matrix& x, const void* d_x, int64_t ldx,
     const int64_t units = p.m / kTileRows + (p.groups < p.m ? p.groups : p.m);
     // half a tile of each group is empty on average
     const int64_t expected = p.m / kTileRows + p.groups / 2, expected_pairs = p.m / (2 * kTileRows) + p.groups / 2;
-    const bool paired = !held && pairs_pay(expected, expected_pairs, p.outer, p.type);
-    const int bn = held ? 64 : paired ? 512 : tile_width(units, p.outer, p.type), chunk = p.type == FG_E4M3 ? 128 : 64;
+    const bool cut = p.type == FG_F32 && x.type == FG_F32;  // rows as they are
+    const bool paired = !held && !cut && pairs_pay(expected, expected_pairs, p.outer);
+    const int bn = held || cut ? 64 : paired ? 512 : tile_width(units, p.outer, p.type), chunk = p.type == FG_E4M3 ? 128 : 64;
     CUtensorMap map_x = {}, map_w;
     if (!held)
-        if (int rc = make_map(&map_x, x, chunk, kTileRows)) return rc;
+        if (int rc = make_map(&map_x, x, cut ? 32 : chunk, kTileRows)) return rc;
     if (int rc = make_map(&map_w, w, chunk, b_mn ? 64 : paired ? 128 : bn)) return rc;
     MmaArgs a{};
     a.offsets = p.offsets, a.order = p.order, a.x_scales = x_scales, a.w_scales = w_scales, a.y = d_y;
@@ -1061,6 +1156,7 @@ int run_product(const Problem& p, const Matrix& x, const void* d_x, int64_t ldx,
     a.stages = (int32_t)((196608 - held) / 16384);
     const int64_t tiles = units * ((p.outer + (paired ? 256 : bn) - 1) / (paired ? 256 : bn));
     return p.type == FG_E4M3  ? launch<kEight, false>(bn, a, map_x, map_w, tiles, s)
+           : cut              ? launch<kCut, false>(bn, a, map_x, map_w, tiles, s)
            : p.type == FG_F32 ? launch<kParts, false>(bn, a, map_x, map_w, tiles, s)
                               : launch<kHalf, false>(bn, a, map_x, map_w, tiles, s);
 }
@@ -1075,7 +1171,7 @@ int run_weight_gradient(const Problem& p, const Matrix& x, const Matrix& dy, voi
     // in pairs, the columns' waste counts as well as the rows', and a short sum is mostly output: 256 rows a group, 128
     // groups of 2048 x 1408 took 325 us in pairs and 292 without, 1024 rows and more are faster in pairs
     const int64_t singles = units * rows_tiles * ((p.inner + 127) / 128), doubles = units * ((p.outer + 255) / 256) * ((p.inner + 255) / 256);
-    const bool paired = p.m >= 768 * units && pairs_pay(singles, doubles * 2, 256, p.type);
+    const bool paired = p.m >= 768 * units && pairs_pay(singles, doubles * 2, 256);
     const int bn = paired ? 512 : tile_width(units * rows_tiles, p.inner, p.type);
     MmaArgs a{};
     a.offsets = p.offsets, a.y = split ? static_cast<void*>(sums) : d_dw;
@@ -1118,7 +1214,8 @@ int64_t fg_grouped_matmul_workspace(const void* d_x, int64_t ldx, const void* d_
                                     const int32_t* d_order, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
     if (num_rows <= 0 || groups < 1 || inner < 1 || outer < 1 || few_rows(num_rows, d_w, w_group, w_out, w_in, inner, type)) return 0;
     const WeightLayout w(d_w, w_group, w_out, w_in, groups, inner, outer, type);
-    return (!held_bytes(num_rows, inner, type) && rows_need_copy(d_x, ldx ? ldx : inner, d_order, type) ? packed_bytes(num_rows, inner, type) : 0) +
+    const bool as_is = held_bytes(num_rows, inner, type) || rows_cut_on_the_way(d_x, ldx ? ldx : inner, d_order, outer, type);
+    return (!as_is && rows_need_copy(d_x, ldx ? ldx : inner, d_order, type) ? packed_bytes(num_rows, inner, type) : 0) +
            (w.copy ? packed_bytes(w.count * w.rows, w.cols, type) : 0);
 }
 
@@ -1156,7 +1253,8 @@ int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, con
     const Problem p{d_offsets, d_order, num_rows, x_rows, choices, groups, inner, outer, type};
     Matrix x{};
     const int64_t held = held_bytes(num_rows, inner, type);
-    if (!held)
+    if (rows_cut_on_the_way(d_x, ldx, d_order, outer, type)) x = Matrix{d_x, inner, num_rows, 0, ldx, 0, type};
+    else if (!held)
         if (int rc = rows_matrix(&x, d_x, ldx, x_rows, d_order, choices, num_rows, inner, type, &work, s)) return rc;
     return run_product(p, x, d_x, ldx, d_x_scales, d_w, w_group, w_out, w_in, d_w_scales, held, d_y, out_type, &work, s);
 }
@@ -1199,8 +1297,10 @@ int fg_grouped_matmul_backward(const void* d_x, int64_t ldx, const void* d_w, in
         return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_grouped_matmul_backward_workspace()");
     uint8_t* work = static_cast<uint8_t*>(d_workspace);
     const Problem p{d_offsets, d_order, num_rows, x_rows, choices, groups, inner, outer, type};
+    // dW needs dy in parts; alone, dx may take it as it is
     Matrix dy;
-    if (int rc = rows_matrix(&dy, d_dy, lddy, num_rows, nullptr, 1, num_rows, outer, type, &work, s)) return rc;
+    if (!d_dw && rows_cut_on_the_way(d_dy, lddy, nullptr, inner, type)) dy = Matrix{d_dy, outer, num_rows, 0, lddy, 0, type};
+    else if (int rc = rows_matrix(&dy, d_dy, lddy, num_rows, nullptr, 1, num_rows, outer, type, &work, s)) return rc;
     if (d_dx) {
         // A gathered row's gradient is the sum over its slots: each slot's part in x's type (one more rounding than the sum
         // itself has, half the bytes of 32-bit parts), their sum in 32 bits.
