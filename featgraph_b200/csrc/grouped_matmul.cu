@@ -14,7 +14,11 @@
 //
 // fp32: no tensor-core type holds it, so x and w are each cut into three bf16 parts of 8 bits (x = a + b + c exactly) and six
 // products of parts are summed, smallest first: a c', b b', c a', a b', b a', a a'; the parts left out, b c', c b' and
-// c c', are below 2^-23 of a term.  Six bf16 products against one fp32 product on the scalar units.
+// c c', are below 2^-23 of a term.  Six bf16 products against one fp32 product on the scalar units.  The tensor cores cut the
+// sum off at 24 bits at each step, always towards zero, which adds up: summed through a whole inner axis, 704 x 6
+// / 16 steps left dW 5e-6 off, against 1e-6 for a library's fp32 product.  So an accumulator holds the products of one
+// chunk of 64 - the five small ones first, then four steps at full size - and the output warps add the chunks in
+// registers, rounding to nearest.
 //
 // Rows that are gathered (slot p reads row order[p] / choices) are first copied into slot order: every column tile reads
 // them again, and row-gather TMA loads (tile::gather4, four rows an instruction) move a 128-row tile at a fraction of the
@@ -98,22 +102,43 @@ struct Tables {
     int tiles[kMaxGroups + 1];  // row tiles (partial sums of dW) before each group
 };
 
+// Adds this warp's share of an accumulator - every second 16 of the BN columns - to its sums.
+template <int BN>
+__device__ __forceinline__ void add_chunk(uint32_t tmem, float (&sums)[BN / 2], int half) {
+#pragma unroll
+    for (int n = 0; n < BN / 32; n += 2) {
+        uint32_t raw[2][16];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) fg::tmem_load<16>(tmem + (2 * (n + u) + half) * 16, raw[u]);
+        fg::tmem_load_wait();
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[(n + u) * 16 + j] = __fadd_rn(sums[(n + u) * 16 + j], __uint_as_float(raw[u][j]));
+    }
+}
+
 // Takes a warp's 32 rows of an accumulator, from `tmem` on, to the output rows from `out` on (row pitch `width`; rows
 // outside [from, rows) and columns >= `left` are not stored): every second 64-byte wide piece of the BN columns, the warp's partner takes
 // the others.  A thread holds a row in tensor memory's layout, so the pieces go through the warp's 2 KB of shared memory
 // (16-byte cells, XOR-swizzled: no bank conflicts either way) and leave as whole sectors, 4 lanes a row.  Stored
 // straight from the threads, 16 bytes in each of 32 rows at a time, or by four warps instead of eight, the output of
 // products with a short inner axis keeps the tensor cores waiting.
-template <typename O, int BN, bool EIGHT>
-__device__ __forceinline__ void store_rows(uint32_t tmem, bool filled, O* out, int64_t width, int from, int rows, int left, bool vector, uint32_t staging,
-                                           int half, float scale, const float* column_scales) {
+// `sums` (SUMS): the values are there instead, in the order that add_chunk leaves them.
+template <typename O, int BN, bool EIGHT, bool SUMS>
+__device__ __forceinline__ void store_rows(uint32_t tmem, bool filled, const float (&sums)[BN / 2], O* out, int64_t width, int from, int rows, int left,
+                                           bool vector, uint32_t staging, int half, float scale, const float* column_scales) {
     constexpr int kCols = 64 / sizeof(O), kCells = 16 / sizeof(O);
     const int lane = threadIdx.x & 31;
-    for (int c = half * kCols; c < BN; c += 2 * kCols) {
-        const int rest = left - c;
-        if (rest <= 0) break;
+#pragma unroll (SUMS ? 16 : 1)
+    for (int n = 0; n < BN / (2 * kCols); ++n) {
+        const int c = (2 * n + half) * kCols, rest = left - c;
+        if (rest <= 0) continue;
         uint32_t raw[kCols];
-        if (filled) {
+        if (SUMS) {
+#pragma unroll
+            for (int j = 0; j < kCols; ++j) raw[j] = __float_as_uint(sums[n * kCols + j]);
+        } else if (filled) {
             fg::tmem_load<kCols>(tmem + c, raw);
             fg::tmem_load_wait();
         } else {
@@ -467,11 +492,14 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
             for (int64_t i = start; live && i < total; i += stride) {
                 const Tile w = locate(i);
                 if (w.chunks == 0) continue;  // an empty group's dW: nothing to add up
-                const int buffer = (int)(turn & 1);
-                const uint32_t acc = tmem + buffer * BN;
-                if (turn >= 2 && !fg::barrier_wait<BLOCKS == 2>(fg::smem_address(&t.drained[buffer]), (turn / 2 - 1) & 1, stop)) break;
-                fg::tcgen05_after_sync();
                 for (int c = 0; c < w.chunks; ++c) {
+                    const int buffer = (int)(turn & 1);
+                    const uint32_t acc = tmem + buffer * BN;
+                    if (c == 0 || S::kParts == 3) {  // a fresh accumulator
+                        live = turn < 2 || fg::barrier_wait<BLOCKS == 2>(fg::smem_address(&t.drained[buffer]), (turn / 2 - 1) & 1, stop);
+                        if (!live) break;
+                        fg::tcgen05_after_sync();
+                    }
                     const uint32_t stage = ring + s * S::kStageBytes, empty = fg::smem_address(&t.empty[s]);
                     live = fg::barrier_wait<BLOCKS == 2 && WGRAD>(fg::smem_address(&t.full[s]), parity, stop);
                     if (KIND == kCut) live = live && fg::barrier_wait(fg::smem_address(&t.tail[s]), parity, stop);
@@ -488,14 +516,15 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
                             const uint32_t ah = at + k / 4 * held_chunk, bh = bt + k / 4 * S::kB;  // a chunk further from the fifth step on
                             const uint64_t da = WGRAD ? fg::operand_descriptor(at + k * 2048, 8192, 1024) : fg::operand_descriptor(ah + k % 4 * 32, 16, 1024);
                             const uint64_t db = b_mn ? fg::operand_descriptor(bh + k % 4 * 2048, 8192, 1024) : fg::operand_descriptor(bh + k % 4 * 32, 16, 1024);
-                            if (!WGRAD || k < steps) fg::product_step<BLOCKS, EIGHT>(acc, da, db, descriptor, c > 0 || pair > (S::kParts == 3 ? 0 : 5) || k > 0);
+                            if (!WGRAD || k < steps) fg::product_step<BLOCKS, EIGHT>(acc, da, db, descriptor, (S::kParts == 1 && c > 0) || pair > (S::kParts == 3 ? 0 : 5) || k > 0);
                         }
                     }
                     fg::product_commit<BLOCKS>(empty);
+                    if (c == w.chunks - 1 || S::kParts == 3) {
+                        fg::product_commit<BLOCKS>(fg::smem_address(&t.filled[buffer]));
+                        ++turn;
+                    }
                 }
-                if (!live) break;
-                fg::product_commit<BLOCKS>(fg::smem_address(&t.filled[buffer]));
-                ++turn;
             }
             if (*stop) {  // products in flight end before the accumulators are freed
                 fg::product_commit<BLOCKS>(fg::smem_address(&t.last));
@@ -568,7 +597,7 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) {
-                if (BLOCKS == 2) fg::barrier_arrive_at(fg::smem_address(&t.full[s]), 0);
+                if (BLOCKS == 2) fg::barrier_arrive_at<true>(fg::smem_address(&t.full[s]), 0);
                 else fg::barrier_arrive(fg::smem_address(&t.full[s]));
             }
             __syncwarp();
@@ -604,28 +633,50 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
                 }
                 column_scales = a.w_scales + (int64_t)w.group * a.outer + w.col;
             }
-            const int buffer = (int)(turn & 1);
-            if (w.chunks) {
-                if (!warp_wait(fg::smem_address(&t.filled[buffer]), (turn / 2) & 1, stop)) break;
-                fg::tcgen05_after_sync();
-            }
-            const uint32_t acc = tmem + ((uint32_t)above << 16) + buffer * BN;
             const int64_t at = first * width + w.col;
-            if (a.out_type == FG_F32)
-                store_rows<float, BN, EIGHT>(acc, w.chunks > 0, static_cast<float*>(a.y) + at, width, from, rows, width - w.col, vector, staging, half, scale, column_scales);
-            else if (a.out_type == FG_F16)
-                store_rows<__half, BN, EIGHT>(acc, w.chunks > 0, static_cast<__half*>(a.y) + at, width, from, rows, width - w.col, vector, staging, half, scale, column_scales);
-            else
-                store_rows<__nv_bfloat16, BN, EIGHT>(acc, w.chunks > 0, static_cast<__nv_bfloat16*>(a.y) + at, width, from, rows, width - w.col, vector, staging, half, scale,
-                                                     column_scales);
-            if (w.chunks) {
+            auto drained = [&](int buffer) {
                 fg::tcgen05_before_sync();
                 __syncwarp();
                 if (lane == 0) {
-                    if (BLOCKS == 2) fg::barrier_arrive_at(fg::smem_address(&t.drained[buffer]), 0);
+                    if (BLOCKS == 2) fg::barrier_arrive_at<false>(fg::smem_address(&t.drained[buffer]), 0);
                     else fg::barrier_arrive(fg::smem_address(&t.drained[buffer]));
                 }
                 ++turn;
+            };
+            float sums[BN / 2];  // fp32: over the chunks
+            if constexpr (S::kParts == 3) {
+#pragma unroll
+                for (int j = 0; j < BN / 2; ++j) sums[j] = 0.0f;
+                bool live = true;
+                for (int c = 0; c < w.chunks; ++c) {
+                    const int buffer = (int)(turn & 1);
+                    live = warp_wait(fg::smem_address(&t.filled[buffer]), (turn / 2) & 1, stop);
+                    if (!live) break;
+                    fg::tcgen05_after_sync();
+                    add_chunk<BN>(tmem + ((uint32_t)above << 16) + buffer * BN, sums, half);
+                    drained(buffer);
+                }
+                if (!live) break;
+                store_rows<float, BN, false, true>(0, true, sums, static_cast<float*>(a.y) + at, width, from, rows, width - w.col, vector, staging, half, scale,
+                                                   column_scales);
+            } else {
+                const int buffer = (int)(turn & 1);
+                if (w.chunks) {
+                    if (!warp_wait(fg::smem_address(&t.filled[buffer]), (turn / 2) & 1, stop)) break;
+                    fg::tcgen05_after_sync();
+                }
+                const uint32_t acc = tmem + ((uint32_t)above << 16) + buffer * BN;
+                const int left = width - w.col;
+                if (a.out_type == FG_F32)
+                    store_rows<float, BN, EIGHT, false>(acc, w.chunks > 0, sums, static_cast<float*>(a.y) + at, width, from, rows, left, vector, staging, half,
+                                                        scale, column_scales);
+                else if (a.out_type == FG_F16)
+                    store_rows<__half, BN, EIGHT, false>(acc, w.chunks > 0, sums, static_cast<__half*>(a.y) + at, width, from, rows, left, vector, staging,
+                                                         half, scale, column_scales);
+                else
+                    store_rows<__nv_bfloat16, BN, EIGHT, false>(acc, w.chunks > 0, sums, static_cast<__nv_bfloat16*>(a.y) + at, width, from, rows, left, vector,
+                                                                staging, half, scale, column_scales);
+                if (w.chunks) drained(buffer);
             }
         }
         if (!WGRAD) {  // rows in no group
@@ -968,8 +1019,8 @@ int pack(const void* src, int64_t s0, int64_t s1, int64_t s2, int64_t groups, in
 // The slots' rows [m, cols] as a loadable matrix: where they lie, or copied.
 bool rows_need_copy(const void* p, int64_t ld, const int32_t* order, int32_t type) { return order || !loadable(p, ld, 0, type); }
 // fp32 rows that a product takes as they are (kCut): on the 16-byte grid, in slot order, and at most two column tiles, each of
-// which cuts them again.  100003 rows, 7 groups: 256 to 128 columns 70 us, in parts beforehand 89; 64 to 64: 20 and 26; but 128
-// to 256 79 and 68.
+// which cuts them again.  100003 rows, 7 groups: 256 to 128 columns 72 us, in parts beforehand 90; 64 to 64: 20 and 26; but 128
+// to 256 79 and 72.
 bool rows_cut_on_the_way(const void* p, int64_t ld, const int32_t* order, int32_t outer, int32_t type) {
     return type == FG_F32 && !order && outer <= 128 && fg::aligned16(p) && ld % 4 == 0 && ld < (1ll << 38);
 }
@@ -1062,10 +1113,9 @@ int launch(int bn, const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap
     if constexpr (KIND != kParts && KIND != kCut) {
         if constexpr (!WGRAD)
             if (a.held) return launch_shape<64, KIND, false, true, 1>(a, map_a, map_b, most_tiles, s);
+        if (bn == 512) return launch_shape<256, KIND, WGRAD, false, 2>(a, map_a, map_b, most_tiles, s);
         if (bn == 256) return launch_shape<256, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s);
     }
-    if constexpr (KIND != kCut)
-        if (bn == 512) return launch_shape<256, KIND, WGRAD, false, 2>(a, map_a, map_b, most_tiles, s);
     if constexpr (KIND != kCut)
         return bn == 128 ? launch_shape<128, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s)
                          : launch_shape<64, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s);
@@ -1079,9 +1129,11 @@ int tile_width(int64_t units, int width, int32_t type) {
 }
 // Pairs of blocks (256 x 256 tiles) load a third less for the same products, which is what 128 x 256 tiles wait for, but
 // leave more of the last tiles empty: taken where the tiles they add are less than a tenth of all, and give
-// each pair two.  `rows_tiles`, `row_pairs`: 128- and 256-row tiles.
-bool pairs_pay(int64_t row_tiles, int64_t row_pairs, int width) {
-    if (width <= 128) return false;
+// each pair two.  20000 x 1024 x 1024 over 5 groups in bf16: 43 us, in pairs 37; 32768 x 4096 x 4096 over 8: 783 and 736.
+// Not for fp32, whose accumulators are handed over with every chunk: 100003 x 256 x 128, gradient of x, 71 us, in pairs 97.
+// `row_tiles`, `row_pairs`: 128- and 256-row tiles.
+bool pairs_pay(int64_t row_tiles, int64_t row_pairs, int width, int32_t type) {
+    if (type == FG_F32 || width <= 128) return false;
     const int64_t cols = (width + 255) / 256;
     return row_pairs * cols >= fg::device_props().sm_count && row_pairs * 2 * 10 <= row_tiles * 11;
 }
@@ -1141,7 +1193,7 @@ int run_product(const Problem& p, const Matrix& x, const void* d_x, int64_t ldx,
     // half a tile of each group is empty on average
     const int64_t expected = p.m / kTileRows + p.groups / 2, expected_pairs = p.m / (2 * kTileRows) + p.groups / 2;
     const bool cut = p.type == FG_F32 && x.type == FG_F32;  // rows as they are
-    const bool paired = !held && !cut && pairs_pay(expected, expected_pairs, p.outer);
+    const bool paired = !held && pairs_pay(expected, expected_pairs, p.outer, p.type);
     const int bn = held || cut ? 64 : paired ? 512 : tile_width(units, p.outer, p.type), chunk = p.type == FG_E4M3 ? 128 : 64;
     CUtensorMap map_x = {}, map_w;
     if (!held)
@@ -1171,7 +1223,7 @@ int run_weight_gradient(const Problem& p, const Matrix& x, const Matrix& dy, voi
     // in pairs, the columns' waste counts as well as the rows', and a short sum is mostly output: 256 rows a group, 128
     // groups of 2048 x 1408 took 325 us in pairs and 292 without, 1024 rows and more are faster in pairs
     const int64_t singles = units * rows_tiles * ((p.inner + 127) / 128), doubles = units * ((p.outer + 255) / 256) * ((p.inner + 255) / 256);
-    const bool paired = p.m >= 768 * units && pairs_pay(singles, doubles * 2, 256);
+    const bool paired = p.m >= 768 * units && pairs_pay(singles, doubles * 2, 256, p.type);
     const int bn = paired ? 512 : tile_width(units * rows_tiles, p.inner, p.type);
     MmaArgs a{};
     a.offsets = p.offsets, a.y = split ? static_cast<void*>(sums) : d_dw;

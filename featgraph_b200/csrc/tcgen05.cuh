@@ -62,12 +62,18 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// Arrives at block `rank`'s barrier of the same address.  The release at cluster scope takes over a thousand cycles: once
-// an output tile, not once a stage.
+// Arrives at block `rank`'s barrier of the same address.  With RELEASE, what this thread wrote before is seen by who waits
+// there, which takes over a thousand cycles; without, the arrival alone is (tensor memory has been read).
+template <bool RELEASE>
 __device__ __forceinline__ void barrier_arrive_at(uint32_t bar, uint32_t rank) {
-    asm volatile(
-        "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}" ::"r"(bar), "r"(rank)
-        : "memory");
+    if (RELEASE)
+        asm volatile(
+            "{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n mbarrier.arrive.release.cluster.shared::cluster.b64 _, [r];\n}" ::"r"(bar),
+            "r"(rank)
+            : "memory");
+    else
+        asm volatile("{\n .reg .b32 r;\n mapa.shared::cluster.u32 r, %0, %1;\n mbarrier.arrive.shared::cluster.b64 _, [r];\n}" ::"r"(bar), "r"(rank)
+                     : "memory");
 }
 
 // Tile loads into this block's shared memory.  In a pair both blocks' loads count on the first one's barrier (the second
