@@ -5,12 +5,15 @@
 // the device only, so a launch covers every way they can fall: persistent blocks, one an SM, scan the offsets into
 // shared memory once (a microsecond) and walk a numbering of 128-row tiles that never span two groups.
 //
-// A block is ten warps.  Warp 0 loads: 128-byte wide tiles of both operands through TMA into a ring of stages.  Warp 1 issues tcgen05 products of 128 x BN x 32 bytes into one of two accumulators in tensor memory.  Warps
-// 2 to 9 take a finished accumulator to the output while the other one fills.
+// Warp 0 of a block loads: 128-byte wide tiles of both operands through TMA into a ring of stages.  Warp 1 issues tcgen05
+// products of 128 x BN x 32 bytes into one of two accumulators in tensor memory; both through one thread that elect.sync
+// picks (under `lane == 0` a stage cost the issuing thread 570 cycles instead of 400).  Warps 2 to 9 take a finished
+// accumulator to the output while the other one fills.
 //
 // Rows of a tile beyond its group's end belong to the next group (or to nothing): in y they are computed and not
 // stored.  In dW they would be terms of the sum, so they are overwritten with zeros in shared memory, in both
-// operands - a zero times their infinities or NaN would still be NaN - before the last products of the group.
+// operands - a zero times their infinities or NaN would still be NaN - by a warp of its own as the group's last chunk
+// lands (by the warp that issues the products it took them 3000 cycles a tile).
 //
 // fp32: no tensor-core type holds it, so x and w are each cut into three bf16 parts of 8 bits (x = a + b + c exactly) and six
 // products of parts are summed, smallest first: a c', b b', c a', a b', b a', a a'; the parts left out, b c', c b' and
@@ -119,8 +122,8 @@ __device__ __forceinline__ void add_chunk(uint32_t tmem, float (&sums)[BN / 2], 
 }
 
 // Takes a warp's 32 rows of an accumulator, from `tmem` on, to the output rows from `out` on (row pitch `width`; rows
-// outside [from, rows) and columns >= `left` are not stored): every second 64-byte wide piece of the BN columns, the warp's partner takes
-// the others.  A thread holds a row in tensor memory's layout, so the pieces go through the warp's 2 KB of shared memory
+// outside [from, rows) and columns >= `left` are not stored): every second 64-byte wide piece of the BN columns, the warp's
+// partner takes the others.  A thread holds a row in tensor memory's layout, so the pieces go through the warp's 2 KB of shared memory
 // (16-byte cells, XOR-swizzled: no bank conflicts either way) and leave as whole sectors, 4 lanes a row.  Stored
 // straight from the threads, 16 bytes in each of 32 rows at a time, or by four warps instead of eight, the output of
 // products with a short inner axis keeps the tensor cores waiting.
@@ -696,12 +699,13 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
 
 // ---- few rows ----
 
-// The form for single tokens: at most kFewRows slots in all.  Bound: the touched weights' bytes, read once for the rows of
-// a group (up to 8 at a time).  A tile of the tensor cores would be nearly empty and its column tiles too few for the
-// SMs: 4 rows x 2 of 16 experts x 2048 x 4096 in bf16 took 34 us there after a 4 us copy of the gathered rows.  Here a
-// block takes 64 columns of the j-th group that has rows, holds up to 8 of its rows in shared memory, and a warp computes
-// four columns at a time, its lanes side by side along the dense inner axis: 16-byte loads, four in flight a lane, each
-// row's values fetched from shared memory once for the four columns; 32-bit multiply-adds and a sum across the warp.
+// The form for single tokens whose weights the loads cannot take as they are: fp32, or off the 16-byte grid.  At most kFewRows
+// slots in all.  Bound: the touched weights' bytes, read once for the rows of a group (up to 8 at a time); the other way
+// would be to cut or copy all groups' weights first.  A block takes 64 columns of the j-th group that has rows, holds up
+// to 8 of its rows in shared memory, and a warp computes four columns at a time, its lanes side by side along the dense
+// inner axis: 16-byte loads, four in flight a lane, each row's values fetched from shared memory once for the four
+// columns; 32-bit multiply-adds and a sum across the warp.  4 rows x 2 of 16 experts, 2048 to 4096 in fp32: 49 us (4.1
+// TB/s); 16 rows x 2 of 64, 1001 to 1000 in bf16: 34 us, 87 us by a copy of the weights.
 constexpr int kFewRows = 32, kFewCols = 64;
 
 template <typename T>
