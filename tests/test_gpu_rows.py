@@ -656,6 +656,54 @@ def test_two_streams_at_once():
         assert all(torch.equal(g, want[i]) for g in got[i])
 
 
+def test_no_rows_at_all():
+    from featgraph.module import combine_rows, group_rows, grouped_matmul, quantize_rows, rms_norm, route
+    for t in sorted(TYPES):
+        dt = TYPES[t]
+        x = torch.empty((0, 24), device="cuda", dtype=dt).requires_grad_(True)
+        w = normal((3, 8, 24), 1, dt).requires_grad_(True)
+        r = route(torch.empty((0, 3), device="cuda", dtype=dt).requires_grad_(True), 2)
+        assert r.weights.shape == (0, 2) and r.groups.offsets.tolist() == [0, 0, 0, 0]
+        for groups in (r.groups, group_rows(torch.empty((0, 2), dtype=torch.int64, device="cuda"), 3)):
+            y = grouped_matmul(x, w, groups, gather=True)
+            out = combine_rows(y, groups, r.weights)
+            dx, dw = torch.autograd.grad(out.sum() + rms_norm(x).sum(), (x, w))
+            assert y.shape == (0, 8) and out.shape == (0, 8) and dx.shape == (0, 24) and not bool(dw.any())
+        assert quantize_rows(x.detach()).scales.shape == (0,)
+    # rows, but none of them in a group
+    groups = group_rows(torch.full((5, 2), -1, dtype=torch.int32, device="cuda"), 3)
+    x, w = normal((5, 24), 1).requires_grad_(True), normal((3, 8, 24), 2).requires_grad_(True)
+    weights = normal((5, 2), 3).requires_grad_(True)
+    out = combine_rows(grouped_matmul(x, w, groups, gather=True), groups, weights)
+    assert not bool(out.any())
+    assert not any(bool(g.any()) for g in torch.autograd.grad(out.sum(), (x, w, weights)))
+
+
+def test_arrays_of_more_than_2_to_the_31_values():
+    from featgraph.module import combine_rows, group_rows, grouped_matmul, rms_norm
+    n, d, t = 140001, 16384, torch.bfloat16
+    x = torch.empty((n, d), device="cuda", dtype=t)
+    x[:2], x[-2:] = normal((2, d), 1, t), normal((2, d), 2, t)
+    x[2:-2] = 1
+    y = rms_norm(x)
+    for rows in (slice(0, 2), slice(n - 2, n)):
+        want, _ = norm_reference(x[rows], None)
+        close(y[rows], want, want.abs() * (half_step(t) + STAT), "norm")
+    del x, y
+    n, inner, outer = 530001, 64, 4096
+    groups = group_rows(torch.arange(n, device="cuda", dtype=torch.int32) % 3, 3)
+    x, w = normal((n, inner), 3, t), normal((3, outer, inner), 4, t, inner ** -0.5)
+    z = grouped_matmul(x, w, groups, gather=True)
+    assert z.numel() > 2 ** 31
+    out = combine_rows(z, groups)
+    for row in (0, 1, n - 2, n - 1):
+        xd, wd = x[row].double(), w[row % 3].double()
+        want, size = wd @ xd, wd.abs() @ xd.abs()
+        close(out[row], want, want.abs() * half_step(t) + steps(inner) * size, "row %d" % row)
+    dx = torch.autograd.grad(combine_rows(z.requires_grad_(True), groups), z, out)[0]
+    assert torch.equal(dx[-1], out[groups.order[-1].long()])
+
+
 def test_refusals_that_need_a_device():
     from featgraph.module import grouped_matmul, quantize_rows, rms_norm
     x = normal((4, 8), 1).requires_grad_(True)
