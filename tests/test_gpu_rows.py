@@ -53,7 +53,7 @@ def norm_reference(h, w, eps=1e-6):
 
 
 @pytest.mark.parametrize("t", sorted(TYPES))
-@pytest.mark.parametrize("n,d", [(1, 1), (3, 7), (5, 32), (1, 255), (9, 256), (17, 300), (6, 512), (4, 513), (5, 1024), (3, 1500), (2, 2048),
+@pytest.mark.parametrize("n,d", [(1, 1), (3, 7), (5, 32), (60001, 32), (333, 64), (1000, 128), (77, 129), (9001, 99), (1, 255), (9, 256), (17, 300), (6, 512), (4, 513), (5, 1024), (3, 1500), (2, 2048),
                                  (3, 2050), (2, 4096), (3, 5001), (2, 8192), (2, 16384), (1, 16383)])
 def test_norm_forward(t, n, d):
     from featgraph.module import rms_norm
@@ -69,7 +69,7 @@ def test_norm_forward(t, n, d):
 
 
 @pytest.mark.parametrize("t", sorted(TYPES))
-@pytest.mark.parametrize("n,d", [(1, 1), (7, 40), (300, 331), (33, 512), (5, 1024), (1000, 96), (70, 2048), (9, 4096), (3, 8192), (2, 16384), (700, 130)])
+@pytest.mark.parametrize("n,d", [(1, 1), (7, 40), (5001, 32), (70003, 64), (2600, 100), (9, 128), (40001, 31), (300, 331), (33, 512), (5, 1024), (1000, 96), (70, 2048), (9, 4096), (3, 8192), (2, 16384), (700, 130)])
 @pytest.mark.parametrize("with_residual", [False, True])
 def test_norm_gradients(t, n, d, with_residual):
     from featgraph.module import rms_norm
@@ -114,7 +114,7 @@ def test_norm_gradient_against_differences():
 
 
 @pytest.mark.parametrize("t", sorted(TYPES))
-@pytest.mark.parametrize("n,d", [(1, 1), (16, 2048), (5, 77), (40, 512), (3, 8192), (2, 16384), (9, 1000)])
+@pytest.mark.parametrize("n,d", [(1, 1), (16, 2048), (5, 77), (4001, 32), (63, 128), (40, 512), (3, 8192), (2, 16384), (9, 1000)])
 def test_norm_in_8_bits(t, n, d):
     from featgraph.module import quantize_rows, rms_norm
     dt = TYPES[t]
