@@ -23,11 +23,11 @@
 // chunk of 64 - the five small ones first, then four steps at full size - and the output warps add the chunks in
 // registers, rounding to nearest.
 //
-// Rows that are gathered (slot p reads row order[p] / choices) are first copied into slot order: every column tile reads
-// them again, and row-gather TMA loads (tile::gather4, four rows an instruction) move a 128-row tile at a fraction of the
-// tile loads' rate.  Measured at 65536 x 2048 x 4096 in bf16: 2767 us with gather loads in the ring, 922 us for rows in
-// slot order, the copy about 70 us; dW 8512 against 1241 us.  The same kernel copies an operand that TMA cannot read (a
-// row pitch or a start off the 16-byte grid, two strides above 1) and cuts fp32 into parts.
+// Rows that are gathered (slot p reads row order[p] / choices) are first copied into slot order, unless there is one column
+// tile only: every column tile reads them again, and row-gather TMA loads (tile::gather4, four rows an instruction) move a
+// 128-row tile at a fraction of the tile loads' rate.  Measured at 65536 x 2048 x 4096 in bf16: 2767 us with gather loads in
+// the ring, 922 us for rows in slot order, the copy about 70 us; dW 8512 against 1241 us.  The same kernel copies an
+// operand that TMA cannot read (a row pitch or a start off the 16-byte grid, two strides above 1) and cuts fp32 into parts.
 #include <atomic>
 #include <climits>
 #include <mutex>
@@ -62,6 +62,7 @@ struct MmaArgs {
     int64_t ldx;
     int32_t stages, held;  // stages of weights; bytes of the rows
     bool vector_rows;      // rows on the 16-byte grid
+    bool gather;           // rows fetched from where they lie
 };
 
 // 16-bit values, e4m3, fp32 in three bf16 parts; kCut: the weight in parts, the rows as they are, cut on their way
@@ -270,11 +271,28 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
     return __all_sync(0xffffffffu, fg::barrier_wait(bar, parity, stop));
 }
 
-template <Kind KIND, bool WGRAD>
-constexpr int kThreads = KIND == kCut ? 608 : WGRAD ? 352 : 320;
+template <Kind KIND, bool WGRAD, bool GATHER>
+constexpr int kThreads = KIND == kCut ? 608 : GATHER ? 576 : WGRAD ? 352 : 320;
 
-template <int BN, Kind KIND, bool WGRAD, bool FEW, int BLOCKS>
-__global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
+// GATHER: a warp fetches the 128 bytes of each of a tile's rows that a chunk holds, each row from where it lies, and lays
+// them as a TMA load would: 16-byte cells, XOR-swizzled, zeros beyond the inner axis and for a slot without a row.
+__device__ __forceinline__ void gather_chunk(const MmaArgs& a, uint32_t to, const int* sources, int chunk, int row_bytes, int64_t pitch_bytes) {
+    const int lane = threadIdx.x & 31, q = lane & 7, at = chunk * kChunkBytes + q * 16, bytes = max(min(16, row_bytes - at), 0);
+#pragma unroll 8
+    for (int i = 0; i < 32; ++i) {
+        const int r = i * 4 + (lane >> 3), source = sources[r];
+        const char* from = static_cast<const char*>(a.x) + (source < 0 || bytes == 0 ? 0 : source * pitch_bytes + at);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + r * kChunkBytes + ((q ^ (r & 7)) << 4)), "l"(from),
+                     "r"(source < 0 ? 0 : bytes)
+                     : "memory");
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncwarp();
+}
+
+template <int BN, Kind KIND, bool WGRAD, bool FEW, int BLOCKS, bool GATHER>
+__global__ void __launch_bounds__(kThreads<KIND, WGRAD, GATHER>, 1)
     product_kernel(const MmaArgs a, const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b) {
     using S = Shape<BN, KIND, FEW, BLOCKS>;
     constexpr bool EIGHT = KIND == kEight;
@@ -282,6 +300,7 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
     constexpr int kRows = kTileRows * BLOCKS;
     extern __shared__ uint8_t dynamic[];
     __shared__ Tables t;
+    __shared__ int row_sources[GATHER ? 8 * kTileRows : 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int rank = BLOCKS == 2 ? (int)fg::cluster_rank() : 0;
     const uint32_t held = (fg::smem_address(dynamic) + 1023u) & ~1023u;  // few rows: they come first
@@ -291,7 +310,7 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
-            fg::barrier_init(fg::smem_address(&t.full[s]), KIND == kCut ? 8 : BLOCKS);
+            fg::barrier_init(fg::smem_address(&t.full[s]), KIND == kCut ? 8 : GATHER ? 2 : BLOCKS);
             fg::barrier_init(fg::smem_address(&t.tail[s]), 1);
             fg::barrier_init(fg::smem_address(&t.empty[s]), 1);
         }
@@ -307,7 +326,7 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
         fg::barrier_init(fg::smem_address(&t.last), 1);
         fg::barrier_init_fence();
         t.stop = 0;
-        if (!FEW) fg::prefetch_map(&map_a);
+        if (!FEW && !GATHER) fg::prefetch_map(&map_a);
         fg::prefetch_map(&map_b);
     }
     if (warp == 1) fg::tmem_alloc<BLOCKS>(fg::smem_address(&t.tmem), S::kColumns);
@@ -323,7 +342,7 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
 
     // groups' first slots and tile counts, scanned: thread i takes groups [i * each, (i + 1) * each)
     {
-        constexpr int kAll = kThreads<KIND, WGRAD>;
+        constexpr int kAll = kThreads<KIND, WGRAD, GATHER>;
         const int each = (a.groups + kAll - 1) / kAll, from = min((int)threadIdx.x * each, a.groups), to = min(from + each, a.groups);
         const int64_t unit = WGRAD ? (a.split ? a.split : (int64_t)INT_MAX) : kRows;
         int own = 0;
@@ -418,7 +437,7 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
                     return WGRAD || a.b_mn ? max(min(S::kOwnCols / 64, ((WGRAD ? a.inner : a.outer) - at + 63) / 64), 0) : S::kOwnCols / 64;
                 };
                 const int a_blocks = blocks_a(w.row), b_blocks = blocks_b(col);
-                const uint32_t own = ((WGRAD ? a_blocks * 8192 : KIND == kCut ? 0 : S::kA) + b_blocks * 8192) * S::kParts * S::kDeep;
+                const uint32_t own = ((WGRAD ? a_blocks * 8192 : KIND == kCut || GATHER ? 0 : S::kA) + b_blocks * 8192) * S::kParts * S::kDeep;
                 uint32_t bytes = own;
                 if (BLOCKS == 2)  // the first block's barrier counts the second one's loads too
                     bytes += ((WGRAD ? blocks_a(w.row + kTileRows) * 8192 : S::kA) + blocks_b(col + S::kOwnCols) * 8192) * S::kParts;
@@ -460,7 +479,7 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
                             for (int q = 0; q < b_blocks; ++q) fg::tma_load_2d<BLOCKS>(bt + q * 8192, &map_b, col + q * 64, slot, full);
                         } else {
                             const int g = a.shared_weight ? p : w.group + p * a.groups;
-                            if (!FEW && KIND != kCut) fg::tma_load_2d<BLOCKS>(at, &map_a, k, w.begin + p * (int)a.m, full);
+                            if (!FEW && KIND != kCut && !GATHER) fg::tma_load_2d<BLOCKS>(at, &map_a, k, w.begin + p * (int)a.m, full);
 #pragma unroll
                             for (int h = 0; h < S::kDeep; ++h) {
                                 const int kh = k + h * (kChunk / S::kDeep);
@@ -577,6 +596,35 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD>, 1)
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) fg::barrier_arrive(fg::smem_address(&t.full[s]));
+                if (++s == stages) s = 0, parity ^= 1;
+            }
+        }
+    } else if (GATHER && warp >= 10) {
+        // Warps take the chunks in turn, so that as many are on their way as the ring holds - and no more: a warp that is
+        // further ahead could take the emptying before the last for the one that it waits for.
+        constexpr int kTurns = S::kStages < 8 ? S::kStages : 8;
+        const int mine = warp - 10, size = EIGHT ? 1 : 2, row_bytes = a.inner * size;
+        const int64_t pitch = a.ldx * size;
+        int* sources = row_sources + mine * kTileRows;
+        int s = 0, parity = 1, turn = 0;
+        bool live = true;
+        for (int64_t i = start; mine < kTurns && live && i < total; i += stride) {
+            const Tile w = locate(i);
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int slot = w.begin + u * 32 + lane, e = slot < w.end ? a.order[slot] : -1, r = e >= 0 ? e / a.choices : -1;
+                sources[u * 32 + lane] = r < a.x_rows ? r : -1;
+            }
+            __syncwarp();
+            for (int c = 0; c < w.chunks; ++c) {
+                if (turn == mine) {
+                    live = warp_wait(fg::smem_address(&t.empty[s]), parity, stop);
+                    if (!live) break;
+                    gather_chunk(a, ring + s * S::kStageBytes, sources, c, row_bytes, pitch);
+                    if (lane == 0) fg::barrier_arrive(fg::smem_address(&t.full[s]));
+                }
+                if (++turn == kTurns) turn = 0;
                 if (++s == stages) s = 0, parity ^= 1;
             }
         }
@@ -1063,6 +1111,14 @@ int launch_few(const FewArgs& a, cudaStream_t s) {
     return FG_OK;
 }
 
+// Rows that the product gathers itself: 16- or 8-bit ones on the 16-byte grid, many of them for one column tile, where the
+// copy in slot order would be most of the work.  16-byte copies by a few warps fill a stage more slowly than TMA does:
+// 55960 slots, 2160 to 64 in bf16 50 us, by a copy first 134; 32854, 1776 to 208 48 and 79; 65536, 256 to 256 26 and 31; but
+// 65536, 2048 to 4096 1230 and 912, and 2000, 1024 to 512 20 and 16.
+bool rows_gathered(const void* p, int64_t ld, const int32_t* order, int64_t m, int32_t outer, int32_t type) {
+    return order && outer <= 256 && m >= 8192 && loadable(p, ld, 0, type);
+}
+
 // The weight is read as it is stored where its inner or its outer axis is dense (8-bit products want the inner one), or
 // copied with that axis dense; a group stride of 0 is one weight for all groups.
 struct WeightLayout {
@@ -1079,12 +1135,12 @@ struct WeightLayout {
     }
 };
 
-template <int BN, Kind KIND, bool WGRAD, bool FEW, int BLOCKS>
+template <int BN, Kind KIND, bool WGRAD, bool FEW, int BLOCKS, bool GATHER = false>
 int launch_shape(const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap& map_b, int64_t most_tiles, cudaStream_t s) {
     constexpr int kSmem = Shape<BN, KIND, FEW, BLOCKS>::kSmem;
-    const auto kernel = product_kernel<BN, KIND, WGRAD, FEW, BLOCKS>;
+    const auto kernel = product_kernel<BN, KIND, WGRAD, FEW, BLOCKS, GATHER>;
     cudaLaunchConfig_t config = {};
-    config.blockDim = dim3(kThreads<KIND, WGRAD>);
+    config.blockDim = dim3(kThreads<KIND, WGRAD, GATHER>);
     config.dynamicSmemBytes = kSmem;
     config.stream = s;
     cudaLaunchAttribute cluster;
@@ -1117,6 +1173,11 @@ int launch(int bn, const MmaArgs& a, const CUtensorMap& map_a, const CUtensorMap
     if constexpr (KIND != kParts && KIND != kCut) {
         if constexpr (!WGRAD)
             if (a.held) return launch_shape<64, KIND, false, true, 1>(a, map_a, map_b, most_tiles, s);
+        if constexpr (!WGRAD)
+            if (a.gather)
+                return bn == 256   ? launch_shape<256, KIND, false, false, 1, true>(a, map_a, map_b, most_tiles, s)
+                       : bn == 128 ? launch_shape<128, KIND, false, false, 1, true>(a, map_a, map_b, most_tiles, s)
+                                   : launch_shape<64, KIND, false, false, 1, true>(a, map_a, map_b, most_tiles, s);
         if (bn == 512) return launch_shape<256, KIND, WGRAD, false, 2>(a, map_a, map_b, most_tiles, s);
         if (bn == 256) return launch_shape<256, KIND, WGRAD, false, 1>(a, map_a, map_b, most_tiles, s);
     }
@@ -1197,10 +1258,11 @@ int run_product(const Problem& p, const Matrix& x, const void* d_x, int64_t ldx,
     // half a tile of each group is empty on average
     const int64_t expected = p.m / kTileRows + p.groups / 2, expected_pairs = p.m / (2 * kTileRows) + p.groups / 2;
     const bool cut = p.type == FG_F32 && x.type == FG_F32;  // rows as they are
-    const bool paired = !held && pairs_pay(expected, expected_pairs, p.outer, p.type);
+    const bool gather = !held && rows_gathered(d_x, ldx, p.order, p.m, p.outer, p.type);
+    const bool paired = !held && !gather && pairs_pay(expected, expected_pairs, p.outer, p.type);
     const int bn = held || cut ? 64 : paired ? 512 : tile_width(units, p.outer, p.type), chunk = p.type == FG_E4M3 ? 128 : 64;
     CUtensorMap map_x = {}, map_w;
-    if (!held)
+    if (!held && !gather)
         if (int rc = make_map(&map_x, x, cut ? 32 : chunk, kTileRows)) return rc;
     if (int rc = make_map(&map_w, w, chunk, b_mn ? 64 : paired ? 128 : bn)) return rc;
     MmaArgs a{};
@@ -1209,7 +1271,7 @@ int run_product(const Problem& p, const Matrix& x, const void* d_x, int64_t ldx,
     a.out_type = out_type, a.format = w.type == FG_BF16 ? 1 : 0;
     a.b_mn = b_mn, a.shared_weight = w_group == 0;
     a.x = d_x, a.ldx = ldx, a.held = (int32_t)held, a.vector_rows = fg::aligned16(d_x) && ldx * fg::type_size(p.type) % 16 == 0;
-    a.stages = (int32_t)((196608 - held) / 16384);
+    a.stages = (int32_t)((196608 - held) / 16384), a.gather = gather;
     const int64_t tiles = units * ((p.outer + (paired ? 256 : bn) - 1) / (paired ? 256 : bn));
     return p.type == FG_E4M3  ? launch<kEight, false>(bn, a, map_x, map_w, tiles, s)
            : cut              ? launch<kCut, false>(bn, a, map_x, map_w, tiles, s)
@@ -1270,7 +1332,8 @@ int64_t fg_grouped_matmul_workspace(const void* d_x, int64_t ldx, const void* d_
                                     const int32_t* d_order, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
     if (num_rows <= 0 || groups < 1 || inner < 1 || outer < 1 || few_rows(num_rows, d_w, w_group, w_out, w_in, inner, type)) return 0;
     const WeightLayout w(d_w, w_group, w_out, w_in, groups, inner, outer, type);
-    const bool as_is = held_bytes(num_rows, inner, type) || rows_cut_on_the_way(d_x, ldx ? ldx : inner, d_order, outer, type);
+    const bool as_is = held_bytes(num_rows, inner, type) || rows_cut_on_the_way(d_x, ldx ? ldx : inner, d_order, outer, type) ||
+                       rows_gathered(d_x, ldx ? ldx : inner, d_order, num_rows, outer, type);
     return (!as_is && rows_need_copy(d_x, ldx ? ldx : inner, d_order, type) ? packed_bytes(num_rows, inner, type) : 0) +
            (w.copy ? packed_bytes(w.count * w.rows, w.cols, type) : 0);
 }
@@ -1310,7 +1373,7 @@ int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, con
     Matrix x{};
     const int64_t held = held_bytes(num_rows, inner, type);
     if (rows_cut_on_the_way(d_x, ldx, d_order, outer, type)) x = Matrix{d_x, inner, num_rows, 0, ldx, 0, type};
-    else if (!held)
+    else if (!held && !rows_gathered(d_x, ldx, d_order, num_rows, outer, type))
         if (int rc = rows_matrix(&x, d_x, ldx, x_rows, d_order, choices, num_rows, inner, type, &work, s)) return rc;
     return run_product(p, x, d_x, ldx, d_x_scales, d_w, w_group, w_out, w_in, d_w_scales, held, d_y, out_type, &work, s);
 }

@@ -338,7 +338,8 @@ def per_slot_size(groups, w, dy):
 @pytest.mark.parametrize("n,k,count,inner,outer", [
     (1, 1, 1, 1, 1), (3, 2, 4, 16, 8), (5, 1, 3, 17, 33), (130, 1, 2, 64, 64), (257, 2, 5, 128, 96), (64, 4, 40, 200, 264), (1000, 3, 7, 72, 520),
     (300, 1, 1, 96, 24), (2000, 2, 3, 331, 127), (40, 8, 300, 64, 40), (129, 2, 2, 512, 1024), (777, 1, 4, 1000, 160),
-    (10000, 1, 4, 1304, 1000), (5001, 2, 2, 520, 1301), (30, 1, 9, 520, 264), (8, 4, 5, 72, 1000), (33, 1, 3, 264, 520)])
+    (10000, 1, 4, 1304, 1000), (5001, 2, 2, 520, 1301), (30, 1, 9, 520, 264), (8, 4, 5, 72, 1000), (33, 1, 3, 264, 520),
+    (4100, 2, 5, 520, 96), (9001, 1, 3, 72, 250)])
 def test_product_and_gradients(t, gather, n, k, count, inner, outer):
     dt = TYPES[t]
     groups = make_groups(n, k, count, 5)
@@ -408,7 +409,7 @@ def test_product_strides(t):
     close(got, want, 4 * half_step(dt) * size + steps(2 * n) * size, "broadcast weight")
 
 
-@pytest.mark.parametrize("n,k,count,inner,outer", [(1, 1, 1, 16, 8), (5, 2, 3, 32, 24), (300, 2, 4, 128, 136), (129, 1, 2, 1040, 520), (64, 4, 33, 77, 45), (2000, 1, 5, 256, 128), (10000, 1, 4, 272, 1000), (16, 2, 9, 272, 264)])
+@pytest.mark.parametrize("n,k,count,inner,outer", [(1, 1, 1, 16, 8), (5, 2, 3, 32, 24), (300, 2, 4, 128, 136), (129, 1, 2, 1040, 520), (64, 4, 33, 77, 45), (2000, 1, 5, 256, 128), (10000, 1, 4, 272, 1000), (16, 2, 9, 272, 264), (3000, 3, 7, 400, 130)])
 @pytest.mark.parametrize("out", sorted(TYPES))
 def test_product_of_8_bit_rows(n, k, count, inner, outer, out):
     from featgraph.module import QuantizedRows, grouped_matmul, quantize_rows
