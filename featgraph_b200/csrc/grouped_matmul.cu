@@ -494,6 +494,11 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD, GATHER>, 1)
                     }
                 }
             }
+            if (BLOCKS == 2)  // the first block's products arrive at both blocks' stages: none may arrive when this one has ended
+                for (int q = 0; live && q < stages; ++q) {
+                    live = fg::barrier_wait(fg::smem_address(&t.empty[s]), parity, stop);
+                    if (++s == stages) s = 0, parity ^= 1;
+                }
             if (*stop) {  // no copy may be in flight when the block (or its pair) ends
                 for (int64_t q = max(step - stages, (int64_t)0); q < step; ++q) {
                     const int at = (int)(q % stages);
