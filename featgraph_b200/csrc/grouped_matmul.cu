@@ -1233,6 +1233,9 @@ int check_product(int64_t m, int64_t x_rows, int32_t choices, int32_t groups, in
     return FG_OK;
 }
 
+// Bytes of the slots' 32-bit parts of a gathered row's gradient.
+int64_t slot_parts_bytes(int64_t m, int32_t inner) { return round_up(m * (int64_t)inner * 4, 256); }
+
 // A launch's sizes and lists, as the entry points get them.
 struct Problem {
     const int32_t *offsets, *order;
@@ -1390,7 +1393,7 @@ int64_t fg_grouped_matmul_backward_workspace(const void* d_x, int64_t ldx, const
     const Problem p{nullptr, d_order, num_rows, 0, 1, groups, inner, outer, type};
     return (rows_need_copy(d_dy, lddy ? lddy : outer, nullptr, type) ? packed_bytes(num_rows, outer, type) : 0) +
            (want_dx ? weight_bytes(other_way(p), d_w, w_group, w_in, w_out) : 0) +
-           (want_dx && d_order ? round_up(num_rows * (int64_t)inner * fg::type_size(type), 256) : 0) +
+           (want_dx && d_order ? slot_parts_bytes(num_rows, inner) : 0) +
            (want_dw ? partial_bytes(num_rows, groups, inner, outer) : 0) +
            (want_dw && rows_need_copy(d_x, ldx ? ldx : inner, d_order, type) ? packed_bytes(num_rows, inner, type) : 0);
 }
@@ -1426,16 +1429,22 @@ int fg_grouped_matmul_backward(const void* d_x, int64_t ldx, const void* d_w, in
     if (!d_dw && rows_cut_on_the_way(d_dy, lddy, nullptr, inner, type)) dy = Matrix{d_dy, outer, num_rows, 0, lddy, 0, type};
     else if (int rc = rows_matrix(&dy, d_dy, lddy, num_rows, nullptr, 1, num_rows, outer, type, &work, s)) return rc;
     if (d_dx) {
-        // A gathered row's gradient is the sum over its slots: each slot's part in x's type (one more rounding than the sum
-        // itself has, half the bytes of 32-bit parts), their sum in 32 bits.
+        // A gathered row's gradient is the sum over its slots.  The slots' parts stay in 32 bits and the sum is rounded once: parts
+        // in x's type would add a rounding each, and in fp16 overflow where their sum does not.  One slot a row has nothing
+        // to add, so its part is rounded as the product leaves it.
+        const int32_t parts_type = choices > 1 ? FG_F32 : type;
         void* parts = d_dx;
         if (d_order) {
             parts = work;
-            work += round_up(num_rows * (int64_t)inner * fg::type_size(type), 256);
+            work += slot_parts_bytes(num_rows, inner);
         }
-        if (int rc = run_product(other_way(p), dy, nullptr, 0, nullptr, d_w, w_group, w_in, w_out, nullptr, 0, parts, type, &work, s)) return rc;
-        if (d_order)
+        if (int rc = run_product(other_way(p), dy, nullptr, 0, nullptr, d_w, w_group, w_in, w_out, nullptr, 0, parts, d_order ? parts_type : type, &work, s))
+            return rc;
+        if (d_order && parts_type == FG_F32) {
+            if (int rc = fg::sum_slots(static_cast<const float*>(parts), d_position, d_dx, x_rows, choices, inner, type, s)) return rc;
+        } else if (d_order) {
             if (int rc = fg_combine_rows(parts, 0, nullptr, d_position, d_dx, x_rows, choices, inner, type, stream)) return rc;
+        }
     }
     if (!d_dw) return FG_OK;
     float* sums = reinterpret_cast<float*>(work);

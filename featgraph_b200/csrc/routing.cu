@@ -411,8 +411,8 @@ struct CombineArgs {
 
 // out[t] = sum over j of weights[t, j] y[position[t, j]], in ascending j, in 32 bits.  A thread owns VEC columns of a
 // row; the k slices of a row are independent loads.  Bound: device memory (M rows read, n written): 32768 rows of 2048 bf16,
-// k = 4, in 119 us (5.6 TB/s).  Four slices held at a time cost a third of the warps and 148 us.
-template <typename T, int VEC>
+// k = 4, in 119 us (5.6 TB/s).  Four slices held at a time cost a third of the warps and 148 us.  O: the output's type.
+template <typename T, int VEC, typename O = T>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
     const int per_row = (a.d + VEC - 1) / VEC;
     const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -431,10 +431,10 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineArgs a) {
 #pragma unroll
         for (int v = 0; v < VEC; ++v) acc[v] = __fmaf_rn(w, to_f32<T>(r.v[v]), acc[v]);
     }
-    Pack<T, VEC> o;
+    Pack<O, VEC> o;
 #pragma unroll
-    for (int v = 0; v < VEC; ++v) o.v[v] = from_f32<T>(acc[v]);
-    store_pack<T, VEC>(static_cast<T*>(a.out) + t * a.d + c, o);
+    for (int v = 0; v < VEC; ++v) o.v[v] = from_f32<O>(acc[v]);
+    store_pack<O, VEC>(static_cast<O*>(a.out) + t * a.d + c, o);
 }
 
 // dy[position[t, j]] = weights[t, j] dout[t];   dweights[t, j] = dot(dout[t], y[position[t, j]]).
@@ -481,13 +481,13 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(const CombineArgs a) 
     }
 }
 
-template <typename T>
+template <typename T, typename O = T>
 int launch_combine(const CombineArgs& a, bool vec, cudaStream_t s) {
     constexpr int kVec = 16 / sizeof(T);
     const int64_t units = a.n * ((a.d + (vec ? kVec : 1) - 1) / (vec ? kVec : 1)), blocks = (units + 255) / 256;
     if (blocks > INT_MAX) return fg::fail(FG_ERR_INVALID_ARGUMENT, "grid too large");
-    if (vec) combine_kernel<T, kVec><<<(unsigned)blocks, 256, 0, s>>>(a);
-    else combine_kernel<T, 1><<<(unsigned)blocks, 256, 0, s>>>(a);
+    if (vec) combine_kernel<T, kVec, O><<<(unsigned)blocks, 256, 0, s>>>(a);
+    else combine_kernel<T, 1, O><<<(unsigned)blocks, 256, 0, s>>>(a);
     FG_CUDA_TRY(cudaGetLastError());
     fg::count_launches(1);
     return FG_OK;
@@ -531,6 +531,20 @@ int64_t chunk_size(int64_t m) {
 }
 
 }  // namespace
+
+namespace fg {
+int sum_slots(const float* parts, const int32_t* position, void* out, int64_t n, int32_t k, int32_t d, int32_t type, cudaStream_t s) {
+    if (int rc = check_combine(n, k, d, type)) return rc;
+    if (n == 0) return FG_OK;
+    CombineArgs a{};
+    a.y = parts, a.position = position, a.out = out;
+    a.n = n, a.m = n * k, a.ldy = d, a.k = k, a.d = d;
+    const bool vec = d % 4 == 0 && aligned16(parts) && aligned16(out);
+    return type == FG_F32   ? launch_combine<float, float>(a, vec, s)
+           : type == FG_F16 ? launch_combine<float, __half>(a, vec, s)
+                            : launch_combine<float, __nv_bfloat16>(a, vec, s);
+}
+}  // namespace fg
 
 extern "C" {
 

@@ -59,6 +59,9 @@ __device__ __forceinline__ float warp_max(float v) {
 // Whether a wait of the norm's gradient ever ran out on the current device (row_norm.cu), copied to *out on `s`.
 int norm_stuck(cudaStream_t s, int* out);
 
+// out[t] = sum over j of parts[position[t * k + j]], rounded once to `type` (routing.cu).
+int sum_slots(const float* parts, const int32_t* position, void* out, int64_t n, int32_t k, int32_t d, int32_t type, cudaStream_t s);
+
 inline int type_size(int32_t t) { return t == FG_F32 ? 4 : t == FG_E4M3 ? 1 : 2; }
 inline bool float_type(int32_t t) { return t == FG_F32 || t == FG_F16 || t == FG_BF16; }
 

@@ -1,0 +1,79 @@
+"""Row operators (``featgraph_b200.module.rows``) at the ends of their range: sums that cancel or leave a 16-bit type's range
+on the way, the smallest and largest 32-bit values, infinities, lists that change under a backward pass, limits that two
+host threads need at once.  Tolerances count roundings: half a step of the type for a rounding to it, u = 2^-24 for one to 32 bits,
+twice that where the tensor cores cut a sum off."""
+import threading
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def tiny(t):
+    """Half the spacing of t's subnormal numbers."""
+    return torch.finfo(t).tiny * torch.finfo(t).eps / 2
+
+
+def within(got, want, tol, what=""):
+    got, want = got.double(), want.double()
+    assert got.shape == want.shape
+    assert bool(torch.isfinite(got).all()), "%s: not finite" % what
+    over = float(((got - want).abs() - tol).max())
+    assert over <= 0.0, "%s: over its tolerance by %.3g (largest value %.3g)" % (what, over, float(want.abs().max()))
+
+
+def normal(shape, seed, t=torch.float32, scale=1.0):
+    return (torch.randn(shape, device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed)) * scale).to(t)
+
+
+def choose(n, k, count, seed):
+    """k different groups for each row."""
+    from featgraph.module import group_rows
+    score = torch.rand((n, count), device="cuda", generator=torch.Generator(device="cuda").manual_seed(seed))
+    return group_rows(torch.topk(score, k, dim=1).indices.int(), count)
+
+
+# ---- the gradient of gathered rows: a sum over a row's slots ----
+
+@pytest.mark.parametrize("t", sorted(TYPES))
+@pytest.mark.parametrize("n,k,count,inner,outer", [(3, 2, 4, 16, 8), (130, 4, 9, 72, 48), (700, 8, 16, 128, 264), (33, 32, 40, 31, 17), (900, 1, 3, 64, 40),
+                                                   (5000, 3, 5, 264, 96)])
+def test_gradient_of_gathered_rows_is_rounded_once(t, n, k, count, inner, outer):
+    """dx[t] = sum over j of W[g(t, j)]^T dy[slot(t, j)]: 32-bit sums throughout, and one rounding to the type."""
+    from featgraph.module import grouped_matmul
+    dt = TYPES[t]
+    groups = choose(n, k, count, 1)
+    x, w, dy = normal((n, inner), 2, dt).requires_grad_(True), normal((count, outer, inner), 3, dt), normal((n * k, outer), 4, dt)
+    dx, = torch.autograd.grad(grouped_matmul(x, w, groups, gather=True), x, dy)
+    want, size = (torch.zeros((n, inner), dtype=torch.float64, device="cuda") for _ in range(2))
+    at, source = groups.offsets.tolist(), groups.order.long() // k
+    for g in range(count):
+        rows = slice(at[g], at[g + 1])
+        want.index_add_(0, source[rows], dy[rows].double() @ w[g].double())
+        size.index_add_(0, source[rows], dy[rows].double().abs() @ w[g].double().abs())
+    # a term passes outer / 16 cut-off additions and the inside of one, in fp32 six parts' sums, then k slots
+    within(dx, want, want.abs() * half_step(dt) + (2 * (outer / 16 + 24) + k) * U * size + tiny(dt), "dx")
+
+
+@pytest.mark.parametrize("parts", [(70000.0, -20000.0), (70000.0, -70000.0), (-60000.0, 30000.0), (65504.0, 0.0)])
+def test_gradient_of_gathered_rows_whose_slots_leave_the_range_of_fp16(parts):
+    """The parts of two slots may be larger than fp16 holds where their sum is not."""
+    from featgraph.module import group_rows, grouped_matmul
+    n, inner, outer = 40, 24, 16
+    groups = group_rows(torch.tensor([[0, 1]] * n, dtype=torch.int32, device="cuda"), 2)
+    x = normal((n, inner), 1, torch.float16).requires_grad_(True)
+    w = torch.zeros((2, outer, inner), device="cuda", dtype=torch.float16)
+    dy = torch.zeros((2 * n, outer), device="cuda", dtype=torch.float16)
+    dy[:, 3] = 1024.0
+    w[0, 3], w[1, 3] = parts[0] / 1024, parts[1] / 1024
+    dx, = torch.autograd.grad(grouped_matmul(x, w, groups, gather=True), x, dy)
+    want = (1024 * (w[0, 3].double() + w[1, 3].double())).expand(n, inner)
+    within(dx, want, want.abs() * half_step(torch.float16), "dx")
