@@ -1,7 +1,7 @@
 // Root-mean-square norm of rows with the residual's addition, its 8-bit form, and its gradient.
 //
 //   h = round(x + residual)      y = h * r * w,   r = 1 / sqrt(mean(h^2) + eps)
-//   8 bits: s = max|h r w| / 448 (1 for a row of zeros),  q = e4m3(h r w / s)
+//   8 bits: s = max|h r w| / 448 (1 where that is 0 in 32 bits),  q = e4m3(h r w / s)
 //   dx = dresidual = dh + r g - h r^3 / d * sum(g h),  g = dy w;      dw = sum over rows of dy h r
 //
 // Bound: device memory - each array is touched once.  TPR threads own a row and hold its E values each in
@@ -83,6 +83,15 @@ __device__ __forceinline__ float row_reduce(float v, float* buffer, int sub) {
         else v = __fadd_rn(v, w);
     }
     return v;
+}
+
+// The scale of an 8-bit row whose largest value is `most`.  The quotient is 0 for a row of zeros, and for one of up to 224 steps
+// of 2^-149: 1 then, since a scale of 0 would make NaN of its zeros.  A quotient of few steps is rounded up: to nearest it
+// could lose a thirtieth and more, and the largest values would lie beyond 464, the last number that rounds to 448; from 16
+// steps on they cannot (448 x 16.5 / 16 = 462).  Infinities and NaN stay what they are.
+__device__ __forceinline__ float row_scale(float most) {
+    const float s = __fdiv_rn(most, (float)kE4M3Max);
+    return s == 0.0f ? 1.0f : s < 0x1p-145f ? __fdiv_ru(most, (float)kE4M3Max) : s;
 }
 
 // The ring of a row's TPR threads: `stages` rows of ARRAYS arrays ahead of them in shared memory, filled by bulk copies, so
@@ -228,7 +237,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR <= 256 ? 2 : 1) nor
             most = (u > most || u != u) ? u : most;
         }
         most = row_reduce<TPR, kThreads, true>(most, buffer[2 + turn], sub);
-        const float scale = most == 0.0f ? 1.0f : __fdiv_rn(most, (float)kE4M3Max);
+        const float scale = row_scale(most);
         uint8_t* q = static_cast<uint8_t*>(a.y) + row * a.d;
         if (t == 0) a.scales[row] = scale;
 #pragma unroll
@@ -458,7 +467,7 @@ __global__ void __launch_bounds__(256) norm_narrow_kernel(const NormArgs a) {
                 const float u = __shfl_xor_sync(0xffffffffu, most, o);
                 most = (u > most || u != u) ? u : most;
             }
-            scale = most == 0.0f ? 1.0f : __fdiv_rn(most, (float)kE4M3Max);
+            scale = row_scale(most);
             if (live && t == 0) a.scales[row] = scale;
         }
 #pragma unroll

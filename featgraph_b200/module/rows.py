@@ -213,9 +213,9 @@ def rms_norm(x, weight=None, residual=None, eps=1e-6, quantize=False):
         h = x + residual (in x's type; h = x without one)      y = h / sqrt(mean(h^2) + eps) * weight
 
     Returns ``y``, or ``(y, h)`` with a residual: h is the stream that the next layer adds to.  ``weight`` [d] is of
-    x's type or float32 (None: ones).  ``quantize``: y as ``QuantizedRows`` (scale = max|y| / 448 a row, 1 for a
-    row of zeros; a row with an infinity or NaN has a scale that says so) - the form for serving, which has no gradient
-    and refuses inputs that want one."""
+    x's type or float32 (None: ones).  ``quantize``: y as ``QuantizedRows`` (scale = max|y| / 448 a row, 1 where
+    that quotient is 0 in 32 bits, as for a row of zeros; a row with an infinity or NaN has a scale that says so) - the
+    form for serving, which has no gradient and refuses inputs that want one."""
     _tensor(x, "x", _FLOATS)
     if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_WIDTH:
         raise ValueError("x must have rows of 1 to %d values, has shape %s" % (MAX_WIDTH, tuple(x.shape)))

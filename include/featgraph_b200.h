@@ -351,7 +351,8 @@ int fg_wait_status(void* stream);
 
 /* Root-mean-square norm: h = x + residual (rounded to `type`; h = x and d_h unused where d_residual is NULL),
  * y = h * r * weight with r = 1 / sqrt(mean(h^2) + eps).  d_weight may be NULL (ones), else of `type` or fp32.
- * out_type FG_E4M3: d_scales[row] = max|y| / 448 (1 for a row of zeros) and the 8-bit values y / scale.
+ * out_type FG_E4M3: d_scales[row] = max|y| / 448 (1 where that quotient is 0 in fp32: a row of zeros, or one below
+ * 3.2e-43, which becomes zeros) and the 8-bit values y / scale.
  * 1 <= d <= 16384; h, y dense.  fg_quantize_rows: the 8-bit form of x itself. */
 int fg_rms_norm(const void* d_x, int64_t ldx, const void* d_residual, int64_t ldr, const void* d_weight, void* d_h, void* d_y,
                 float* d_scales, int64_t n, int32_t d, float eps, int32_t type, int32_t weight_type, int32_t out_type,

@@ -77,3 +77,31 @@ def test_gradient_of_gathered_rows_whose_slots_leave_the_range_of_fp16(parts):
     dx, = torch.autograd.grad(grouped_matmul(x, w, groups, gather=True), x, dy)
     want = (1024 * (w[0, 3].double() + w[1, 3].double())).expand(n, inner)
     within(dx, want, want.abs() * half_step(torch.float16), "dx")
+
+
+# ---- 8-bit rows of very small values ----
+
+@pytest.mark.parametrize("d", [2, 31, 128, 129, 1000, 4096])
+@pytest.mark.parametrize("most", [1.4e-45, 1e-44, 3.1e-43, 3.2e-43, 6.2e-43, 9e-43, 1e-42, 3e-42, 1e-41, 1e-40, 1e-38])
+def test_8_bit_rows_of_the_smallest_values(d, most):
+    """A finite row stays finite: no scale of 0, nothing beyond the largest 8-bit value."""
+    from featgraph.module import quantize_rows, rms_norm
+    x = torch.zeros((3, d), device="cuda")
+    x[0, 0] = most
+    x[1] = normal((d,), 1).clamp(-1, 1) * most
+    x[1, d // 2] = -most
+    unit = 2.0 ** -149
+    for q in (quantize_rows(x), rms_norm(x * 2 ** 60, eps=1.0, weight=torch.full((d,), 2.0 ** -60, device="cuda"), quantize=True)):
+        values, scales = q.values.double(), q.scales.double()
+        assert bool(torch.isfinite(values).all()) and bool((scales > 0).all())
+        # half a step of 2^-3 of the value (and of the next 8-bit number down, near 0), and the smallest 32-bit steps; a row that
+        # is too small for a scale of its own becomes zeros
+        back = values * scales.unsqueeze(1)
+        want = x.double()
+        lost = torch.where(scales == 1.0, 224.5 * unit, 0.0).unsqueeze(1)
+        held = torch.where(scales == 1.0, 0.0, scales).unsqueeze(1)
+        within(back, want, want.abs() * (2.0 ** -4 + 2.0 ** -10) + held * 2.0 ** -10 * 1.001 + lost + 2 * unit, "values")
+        quotient = x[:2].double().abs().amax(1) / 448
+        given = scales[:2]
+        assert bool(torch.where(given == 1.0, quotient <= 0.51 * unit, (given - quotient).abs() <= 1.01 * unit + quotient * 4 * U).all())
+        assert float(scales[2]) == 1.0 and not bool(values[2].any())
