@@ -15,9 +15,11 @@
 // operands - a zero times their infinities or NaN would still be NaN - by a warp of its own as the group's last chunk
 // lands (by the warp that issues the products it took them 3000 cycles a tile).
 //
-// fp32: no tensor-core type holds it, so x and w are each cut into three bf16 parts of 8 bits (x = a + b + c exactly) and six
-// products of parts are summed, smallest first: a c', b b', c a', a b', b a', a a'; the parts left out, b c', c b' and
-// c c', are below 2^-23 of a term.  Six bf16 products against one fp32 product on the scalar units.  The tensor cores cut the
+// fp32: no tensor-core type holds it, so x and w are each cut into three bf16 parts (x = a + b + c exactly, but for bits below
+// 2^-133, bf16's smallest step) and six products of parts are summed, smallest first: a c', b b', c a', a b', b a', a a'.
+// a and b are rounded to nearest, so |b| <= 2^-8 |x| and |c| <= 2^-17 |x|, and what is left out, b c', c b' and c c', is below
+// 2^-23.9 of a term and of either sign; parts that were cut off instead all had x's sign and left out up to 2^-21, always
+// towards zero.  Six bf16 products against one fp32 product on the scalar units.  The tensor cores cut the
 // sum off at 24 bits at each step, always towards zero, which adds up: summed through a whole inner axis, 704 x 6
 // / 16 steps left dW 5e-6 off, against 1e-6 for a library's fp32 product.  So an accumulator holds the products of one
 // chunk of 64 - the five small ones first, then four steps at full size - and the output warps add the chunks in
@@ -224,15 +226,21 @@ __device__ __forceinline__ void hold_rows(const MmaArgs& a, uint32_t held, int c
     }
 }
 
-// Eight fp32 values in three bf16 parts each, by cutting 16 bits off: x = a + b + c exactly (8 bits of its 24 each), and no
-// conversion, which rounding to bf16 would take (at a fraction of the multiply-adds' rate).
+// Eight fp32 values in three bf16 parts each: x = a + b + c.  a and b are rounded to nearest by adding half a step of theirs to
+// the bits (a carry into the exponent is a rounding up to the next power of two), where conversions to bf16 would run at a
+// fraction of the adds' rate; c has 8 bits at most and is exact.  Where one of the eight would round up to an infinity, a is cut
+// off instead: b is then up to 2^-7 of x, and the sum still exact.  An infinity's parts have a NaN among them, a NaN's too.
 __device__ __forceinline__ void cut_values(const float (&v)[8], Pack<__nv_bfloat16, 8> (&p)[3]) {
     uint32_t part[3][8];
+    float most = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = fmaxf(most, fabsf(v[j]));
+    const uint32_t half = most < 0x1.ffp127f ? 0x8000u : 0u;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-        part[0][j] = __float_as_uint(v[j]);
+        part[0][j] = __float_as_uint(v[j]) + half;
         const float rest = __fsub_rn(v[j], __uint_as_float(part[0][j] & 0xffff0000u));
-        part[1][j] = __float_as_uint(rest);
+        part[1][j] = __float_as_uint(rest) + 0x8000u;
         part[2][j] = __float_as_uint(__fsub_rn(rest, __uint_as_float(part[1][j] & 0xffff0000u)));
     }
 #pragma unroll
@@ -1076,8 +1084,8 @@ int pack(const void* src, int64_t s0, int64_t s1, int64_t s2, int64_t groups, in
 // The slots' rows [m, cols] as a loadable matrix: where they lie, or copied.
 bool rows_need_copy(const void* p, int64_t ld, const int32_t* order, int32_t type) { return order || !loadable(p, ld, 0, type); }
 // fp32 rows that a product takes as they are (kCut): on the 16-byte grid, in slot order, and at most two column tiles, each of
-// which cuts them again.  100003 rows, 7 groups: 256 to 128 columns 72 us, in parts beforehand 90; 64 to 64: 20 and 26; but 128
-// to 256 79 and 72.
+// which cuts them again.  100003 rows, 7 groups: 256 to 128 columns 74 us (72 with the parts cut off instead of rounded), in
+// parts beforehand 90; 64 to 64: 20 and 26; but 128 to 256 79 and 74.
 bool rows_cut_on_the_way(const void* p, int64_t ld, const int32_t* order, int32_t outer, int32_t type) {
     return type == FG_F32 && !order && outer <= 128 && fg::aligned16(p) && ld % 4 == 0 && ld < (1ll << 38);
 }

@@ -105,3 +105,61 @@ def test_8_bit_rows_of_the_smallest_values(d, most):
         given = scales[:2]
         assert bool(torch.where(given == 1.0, quotient <= 0.51 * unit, (given - quotient).abs() <= 1.01 * unit + quotient * 4 * U).all())
         assert float(scales[2]) == 1.0 and not bool(values[2].any())
+
+
+# ---- fp32 products: parts of the operands ----
+
+def patterns():
+    """Significands whose bits after the eighth are all ones, all zeros but the last, halfway, and random ones; both signs."""
+    base = [1 + 2.0 ** -7 - 2.0 ** -23, 2 - 2.0 ** -23, 1 + 2.0 ** -8, 1 + 2.0 ** -8 - 2.0 ** -23, 1 + 2.0 ** -16, 1 + 2.0 ** -16 - 2.0 ** -23,
+            1 + 2.0 ** -8 + 2.0 ** -16, 1.5 + 2.0 ** -7 - 2.0 ** -15, 1 + 2.0 ** -23, 1.0]
+    some = (1 + torch.rand(54, generator=torch.Generator().manual_seed(3), dtype=torch.float64)).tolist()
+    v = torch.tensor(base + some, dtype=torch.float32, device="cuda")
+    return torch.cat([v, -v])
+
+
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("inner", [1, 4, 40])
+@pytest.mark.parametrize("outer", [128, 200])
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** 40, 2.0 ** -60])
+def test_a_single_fp32_product_is_within_its_bound(gather, inner, outer, scale):
+    """One nonzero term a sum: what the parts leave out is below 2^-24 (1 + 2^-9) of it, the last of the six sums is cut
+    off at 24 bits (2 u), the five before it are below 2^-6 of the term (2^-6 x 5 x 2 u)."""
+    from featgraph.module import group_rows, grouped_matmul
+    v = patterns()
+    n = v.numel()
+    x, w = torch.zeros((n, inner), device="cuda"), torch.zeros((2, outer, inner), device="cuda")
+    x[:, 0] = v * scale
+    column = v.repeat(outer // n + 1)[:outer]
+    w[0, :, 0], w[1, :, 0] = column, -column.flip(0)
+    keys = (torch.arange(n, device="cuda", dtype=torch.int32) % 2)
+    groups = group_rows(keys, 2)
+    order = groups.order.long()
+    leaf, weight = (x if gather else x[order].contiguous()).requires_grad_(True), w.clone().requires_grad_(True)
+    y = grouped_matmul(leaf, weight, groups, gather=gather)
+    want = x.detach().double()[order][:, :1] * w.double()[keys[order].long()][:, :, 0]
+    bound = (1 + 2.0 ** -9 + 2 + 10 * 2.0 ** -6) * U
+    within(y.detach(), want, bound * want.abs(), "y")
+    # the gradient of x reads the weight the other way: one nonzero output a row
+    dy = torch.zeros_like(y)
+    dy[torch.arange(n, device="cuda"), torch.arange(n, device="cuda") % outer] = v * scale
+    dx, = torch.autograd.grad(y, leaf, dy)
+    dx = dx[order] if gather else dx
+    want = (v.double() * scale) * w.double()[keys[order].long(), torch.arange(n, device="cuda") % outer, 0]
+    within(dx[:, 0], want, (bound + U) * want.abs(), "dx")
+
+
+def test_largest_and_smallest_fp32_values():
+    from featgraph.module import group_rows, grouped_matmul
+    n = 64
+    groups = group_rows(torch.zeros(n, dtype=torch.int32, device="cuda"), 1)
+    top = torch.finfo(torch.float32).max
+    x = torch.zeros((n, 8), device="cuda")
+    x[:, 0] = torch.tensor([top, -top, top * (1 - 2.0 ** -9), top / 2, 2.0 ** 127, 1.0, (1 + 2.0 ** -23) * 2.0 ** -112,
+                            (1 + 2.0 ** -7 - 2.0 ** -23) * 2.0 ** -105], device="cuda").repeat(8)
+    w = torch.zeros((1, 16, 8), device="cuda")
+    w[0, :, 0] = torch.tensor([1.0, -1.0, 0.5, 0.75] * 4, device="cuda")
+    y = grouped_matmul(x, w, groups)
+    want = x.double()[:, :1] * w[0].double()[:, 0]
+    # below 2^-110 a value's bits under 2^-133 are cut off
+    within(y, want, (1 + 2.0 ** -9 + 2 + 10 * 2.0 ** -6) * U * want.abs() + 2.0 ** -133, "y")
