@@ -408,6 +408,10 @@ def grouped_matmul(x, weight, groups, gather=False, out_dtype=None):
     ``gather``, [n, in] the rows in their own order, of which slot p reads row order[p] // k.  The groups' sizes stay on
     the device.  Differentiable in x and weight.
 
+    An infinity or NaN stays in the rows (of ``weight``: the groups and outputs) that it belongs to.  In float32 an
+    infinity gives NaN there, as operands are cut into parts; up to 32 slots of a weight with a dense inner axis of at most
+    6144 values, and the other types, give what the sum gives.
+
     ``x`` and ``weight`` may both be ``QuantizedRows`` (scales [rows] and [groups, out]): products of the 8-bit values
     in 32-bit sums, scaled at the end, in ``out_dtype`` (bfloat16 unless stated); no gradient."""
     if not isinstance(groups, RowGroups):

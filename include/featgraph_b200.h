@@ -394,8 +394,10 @@ int fg_group_rows(const int32_t* d_keys, int64_t num_entries, int32_t num_groups
  * fg_grouped_matmul_backward, either output NULL where it is not wanted: d_dx[t, i] = sum over the slots p of row t of
  * sum over o of w[g, o, i] * dy[p, o] (rows without a slot are 0), d_dw[g, o, i] = sum over the rows p of g of
  * dy[p, o] * x[row(p), i]; both dense.  d_position: the inverse of d_order, where that is given.
- * fp32 products: sums of six bf16 products of three parts of each operand, which leave out less than 2^-23 of a term (and
- * bits of an operand below 2^-133); an infinity among the operands gives NaN. */
+ * fp32 products: sums of six bf16 products of three parts of each operand, which leave out less than 2^-23 of a term (2^-22
+ * beside values above 3.38e38) and bits of an operand below 2^-133; an infinity's parts cannot be summed, so it gives NaN.  Up
+ * to 32 slots of a weight whose inner axis is dense and at most 6144 values are plain fp32 multiply-adds in the forward call:
+ * there it gives what the sum gives. */
 int64_t fg_grouped_matmul_workspace(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,
                                     const int32_t* d_order, int64_t num_rows, int32_t groups, int32_t inner, int32_t outer, int32_t type);
 int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, const void* d_w, int64_t w_group, int64_t w_out,

@@ -163,3 +163,24 @@ def test_largest_and_smallest_fp32_values():
     want = x.double()[:, :1] * w[0].double()[:, 0]
     # below 2^-110 a value's bits under 2^-133 are cut off
     within(y, want, (1 + 2.0 ** -9 + 2 + 10 * 2.0 ** -6) * U * want.abs() + 2.0 ** -133, "y")
+
+
+# ---- infinities ----
+
+@pytest.mark.parametrize("n", [1, 8, 32, 33, 200])
+@pytest.mark.parametrize("t", sorted(TYPES))
+def test_an_infinity_stays_in_its_row(t, n):
+    """16 bits: what the sum gives.  fp32: the sum's infinity for up to 32 slots of a weight with a dense inner axis, NaN for more."""
+    from featgraph.module import group_rows, grouped_matmul
+    dt = TYPES[t]
+    groups = group_rows(torch.zeros(n, dtype=torch.int32, device="cuda"), 1)
+    x, w = normal((n, 40), 1, dt), normal((1, 24, 40), 2, dt)
+    row = n // 2
+    x[row, 5] = float("-inf")
+    y = grouped_matmul(x, w, groups)
+    others = torch.arange(n, device="cuda") != row
+    assert bool(torch.isfinite(y[others]).all())
+    if dt == torch.float32 and n > 32:
+        assert bool(torch.isnan(y[row]).all())
+    else:
+        assert torch.equal(y[row], torch.where(w[0, :, 5] > 0, float("-inf"), float("inf")).to(dt))
