@@ -43,7 +43,8 @@ class RowGroups:
     """The lists of ``group_rows``: slots ``offsets[g] .. offsets[g + 1]`` belong to group g, ``order[slot]`` is the
     entry (row * k + choice) that a slot holds, ``position`` [n, k] the slot of each entry.  Entries in no group have
     position -1; the slots from ``offsets[-1]`` on hold -1.  All int32, on one device.  The lists are trusted to
-    be such a pair of permutations; values out of range are treated as -1."""
+    be such a pair of permutations; values out of range are treated as -1.  A backward pass needs them as they were in the
+    forward pass: lists that were written to in between raise, as other saved tensors do."""
     __slots__ = ("offsets", "order", "position")
 
     def __init__(self, offsets, order, position):
@@ -377,27 +378,26 @@ class _Product(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, groups, gather):
         xr, ldx = _as_rows(x)
-        ctx.groups, ctx.gather = groups, gather
-        ctx.save_for_backward(x, w)
+        ctx.gather = gather
+        ctx.save_for_backward(x, w, groups.offsets, groups.order, groups.position)  # the lists too: refilled in place, they raise
         return _product(xr, ldx, None, w, w.stride(), None, groups, gather, x.shape[0], w.shape[2], w.shape[1], x.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, w = ctx.saved_tensors
-        groups, gather = ctx.groups, ctx.gather
+        x, w, offsets, slots, places = ctx.saved_tensors
         outer, inner = w.shape[1], w.shape[2]
         want_dx, want_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         dyr, ldy = _as_rows(dy)
         xr, ldx = _as_rows(x)
-        device, kind, m, g = x.device, _TYPES[x.dtype], groups.order.numel(), groups.offsets.numel() - 1
+        device, kind, m, g = x.device, _TYPES[x.dtype], slots.numel(), offsets.numel() - 1
         dx = torch.empty(x.shape, dtype=x.dtype, device=device) if want_dx else None
         dw = torch.empty(w.shape, dtype=w.dtype, device=device) if want_dw else None
-        order, position = (groups.order.data_ptr(), groups.position.data_ptr()) if gather else (None, None)
+        order, position = (slots.data_ptr(), places.data_ptr()) if ctx.gather else (None, None)
         operands = (xr.data_ptr(), ldx, w.data_ptr(), *w.stride())
         size = _size("fg_grouped_matmul_backward_workspace", *operands, order, dyr.data_ptr(), ldy, want_dx, want_dw, m, g, inner, outer, kind)
         work = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-        _call("fg_grouped_matmul_backward", x.get_device(), *operands, groups.offsets.data_ptr(), order, position, groups.position.shape[1],
+        _call("fg_grouped_matmul_backward", x.get_device(), *operands, offsets.data_ptr(), order, position, places.shape[1],
               x.shape[0], dyr.data_ptr(), ldy, _ptr(dx), _ptr(dw), m, g, inner, outer, kind, _ptr(work), size)
         return dx, dw, None, None
 
@@ -469,22 +469,20 @@ def _combine(y, groups, weights):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, groups, weights):
-        ctx.groups = groups
-        ctx.save_for_backward(y, weights)
+        ctx.save_for_backward(y, weights, groups.offsets, groups.position, groups.order)  # the lists too: refilled in place, they raise
         return _combine(y, groups, weights)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        y, weights = ctx.saved_tensors
-        groups = ctx.groups
+        y, weights, offsets, position, _ = ctx.saved_tensors
         yr, ldy = _as_rows(y)
         gr, ldd = _as_rows(dout)
-        n, k, d = groups.num_rows, groups.choices, y.shape[1]
+        (n, k), d = position.shape, y.shape[1]
         dy = torch.empty(n * k, d, dtype=y.dtype, device=y.device) if ctx.needs_input_grad[0] else None
         dw = torch.empty(n, k, dtype=torch.float32, device=y.device) if weights is not None and ctx.needs_input_grad[2] else None
-        _call("fg_combine_rows_backward", y.get_device(), yr.data_ptr(), ldy, _ptr(weights), groups.position.data_ptr(), groups.offsets.data_ptr(),
-              groups.num_groups, gr.data_ptr(), ldd, _ptr(dy), _ptr(dw), n, k, d, _TYPES[y.dtype])
+        _call("fg_combine_rows_backward", y.get_device(), yr.data_ptr(), ldy, _ptr(weights), position.data_ptr(), offsets.data_ptr(),
+              offsets.numel() - 1, gr.data_ptr(), ldd, _ptr(dy), _ptr(dw), n, k, d, _TYPES[y.dtype])
         return dy, None, dw
 
 

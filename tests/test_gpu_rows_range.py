@@ -184,3 +184,21 @@ def test_an_infinity_stays_in_its_row(t, n):
         assert bool(torch.isnan(y[row]).all())
     else:
         assert torch.equal(y[row], torch.where(w[0, :, 5] > 0, float("-inf"), float("inf")).to(dt))
+
+
+# ---- lists that change under a backward pass ----
+
+@pytest.mark.parametrize("which", ["offsets", "order", "position"])
+def test_lists_refilled_before_the_backward_pass_are_noticed(which):
+    from featgraph.module import RowGroups, combine_rows, grouped_matmul
+    made = choose(50, 2, 4, 1)
+    x, w = normal((50, 16), 2).requires_grad_(True), normal((4, 24, 16), 3).requires_grad_(True)
+    rows, weights = normal((100, 24), 4).requires_grad_(True), normal((50, 2), 5).requires_grad_(True)
+    for call in (lambda g: grouped_matmul(x, w, g, gather=True), lambda g: combine_rows(rows, g, weights)):
+        groups = RowGroups(made.offsets.clone(), made.order.clone(), made.position.clone())
+        out = call(groups)
+        getattr(groups, which).copy_(getattr(choose(50, 2, 4, 9), which))
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            out.sum().backward()
+        out = call(made)
+        out.sum().backward()  # untouched lists are fine
