@@ -363,6 +363,18 @@ def route(logits, k, scoring="softmax", normalize=True):
 
 # ---- products ----
 
+def _save(ctx, groups, *tensors):
+    """Keeps ``tensors`` and the lists for the backward pass.  The lists count as saved tensors, so that ones that are refilled
+    before it raise - but for lists made in inference mode, which autograd does not save (nor sees written to)."""
+    lists = (groups.offsets, groups.order, groups.position)
+    ctx.lists = lists if any(t.is_inference() for t in lists) else ()
+    ctx.save_for_backward(*tensors, *(() if ctx.lists else lists))
+
+
+def _saved(ctx):
+    return (*ctx.saved_tensors, *ctx.lists)
+
+
 def _product(x, ldx, x_scales, w, strides, w_scales, groups, gather, x_rows, inner, outer, out_dtype):
     device, kind, m, g = x.device, _TYPES[x.dtype], groups.order.numel(), groups.offsets.numel() - 1
     y = torch.empty(m, outer, dtype=out_dtype, device=device)
@@ -379,13 +391,13 @@ class _Product(torch.autograd.Function):
     def forward(ctx, x, w, groups, gather):
         xr, ldx = _as_rows(x)
         ctx.gather = gather
-        ctx.save_for_backward(x, w, groups.offsets, groups.order, groups.position)  # the lists too: refilled in place, they raise
+        _save(ctx, groups, x, w)
         return _product(xr, ldx, None, w, w.stride(), None, groups, gather, x.shape[0], w.shape[2], w.shape[1], x.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, w, offsets, slots, places = ctx.saved_tensors
+        x, w, offsets, slots, places = _saved(ctx)
         outer, inner = w.shape[1], w.shape[2]
         want_dx, want_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         dyr, ldy = _as_rows(dy)
@@ -469,13 +481,13 @@ def _combine(y, groups, weights):
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, groups, weights):
-        ctx.save_for_backward(y, weights, groups.offsets, groups.position, groups.order)  # the lists too: refilled in place, they raise
+        _save(ctx, groups, y, weights)
         return _combine(y, groups, weights)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        y, weights, offsets, position, _ = ctx.saved_tensors
+        y, weights, offsets, _, position = _saved(ctx)
         yr, ldy = _as_rows(y)
         gr, ldd = _as_rows(dout)
         (n, k), d = position.shape, y.shape[1]

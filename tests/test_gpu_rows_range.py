@@ -202,3 +202,15 @@ def test_lists_refilled_before_the_backward_pass_are_noticed(which):
             out.sum().backward()
         out = call(made)
         out.sum().backward()  # untouched lists are fine
+
+
+def test_lists_made_in_inference_mode_serve_a_training_step():
+    from featgraph.module import combine_rows, group_rows, grouped_matmul
+    keys = torch.arange(100, device="cuda", dtype=torch.int32).view(50, 2) % 4
+    with torch.inference_mode():
+        fixed = group_rows(keys, 4)
+    x, w = normal((50, 16), 2).requires_grad_(True), normal((4, 24, 16), 3).requires_grad_(True)
+    weights, dout = normal((50, 2), 5).requires_grad_(True), normal((50, 24), 6)
+    got, want = (torch.autograd.grad(combine_rows(grouped_matmul(x, w, groups, gather=True), groups, weights), (x, w, weights), dout)
+                 for groups in (fixed, group_rows(keys, 4)))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
