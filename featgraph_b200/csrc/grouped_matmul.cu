@@ -1341,7 +1341,7 @@ int fg_wait_status(void* stream) {
     FG_CUDA_TRY(cudaMemcpyFromSymbolAsync(&product, g_stuck, sizeof(int), 0, cudaMemcpyDeviceToHost, s));
     if (int rc = fg::norm_stuck(s, &norm)) return rc;
     FG_CUDA_TRY(cudaStreamSynchronize(s));
-    return product || norm ? fg::fail(FG_ERR_CUDA, "%s gave up waiting for its own copies", product ? "a grouped product" : "a norm's gradient") : FG_OK;
+    return product || norm ? fg::fail(FG_ERR_CUDA, "%s gave up waiting for its own copies", product ? "a grouped product" : "a norm of rows, its gradient or 8-bit form") : FG_OK;
 }
 
 int64_t fg_grouped_matmul_workspace(const void* d_x, int64_t ldx, const void* d_w, int64_t w_group, int64_t w_out, int64_t w_in,

@@ -56,7 +56,8 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-// Whether a wait of the norm's gradient ever ran out on the current device (row_norm.cu), copied to *out on `s`.
+// Whether a wait of the norm, its 8-bit form or its gradient ever ran out on the current device (row_norm.cu), copied to *out on
+// `s`.
 int norm_stuck(cudaStream_t s, int* out);
 
 // out[t] = sum over j of parts[position[t * k + j]], rounded once to `type` (routing.cu).

@@ -10,5 +10,5 @@ VanillaSDDMM = VanillaSDDMMcuda
 from .fused import AggregateThenScore
 
 # what a layer with several experts, node types or relations computes densely around them (module/rows.py)
-from .rows import (QuantizedRows, Routing, RowGroups, combine_rows, group_rows, grouped_matmul, quantize_rows,
+from .rows import (QuantizedRows, Routing, RowGroups, check_waits, combine_rows, group_rows, grouped_matmul, quantize_rows,
                    rms_norm, route)

@@ -108,6 +108,16 @@ def _size(name, *args):
     return fn(*args)
 
 
+def check_waits(device=None):
+    """Waits for the current stream of ``device`` (the current one unless stated) and raises ``FeatGraphError`` if a row
+    operator on that device ever gave up waiting for its own copies, which it does after some four seconds instead of
+    hanging.  What that call returned is undefined.  For points where a program synchronises anyway; not for capture."""
+    device = dev.resolve_device(device)
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("check_waits() synchronises: it cannot be captured")
+    _call("fg_wait_status", device.index)
+
+
 def _ptr(t):
     return None if t is None else t.data_ptr()
 

@@ -346,7 +346,7 @@ int fg_coo_validate(const int32_t* d_row, const int32_t* d_col, int64_t n_rows, 
 #define FG_E4M3 3
 
 /* Kernels wait for their own copies with a limit (seconds).  Synchronises `stream` and returns FG_ERR_CUDA if such a
- * wait ever ran out on the current device; the output of that call was wrong. */
+ * wait ever ran out on the current device in this process; what that call returned is undefined. */
 int fg_wait_status(void* stream);
 
 /* Root-mean-square norm: h = x + residual (rounded to `type`; h = x and d_h unused where d_residual is NULL),

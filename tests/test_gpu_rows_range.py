@@ -214,3 +214,36 @@ def test_lists_made_in_inference_mode_serve_a_training_step():
     got, want = (torch.autograd.grad(combine_rows(grouped_matmul(x, w, groups, gather=True), groups, weights), (x, w, weights), dout)
                  for groups in (fixed, group_rows(keys, 4)))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---- waits ----
+
+def test_waits_are_reported():
+    from featgraph.module import check_waits
+    x = normal((100, 300), 1)
+    from featgraph.module import quantize_rows
+    quantize_rows(x)
+    assert check_waits() is None and check_waits("cuda:0") is None and check_waits(x.device) is None
+
+
+def test_a_wait_that_ran_out_is_raised(monkeypatch):
+    """The answer of the library is a fake here: no wait is made to run out."""
+    from featgraph.module import check_waits
+    from featgraph_b200 import _native
+    from featgraph_b200.module import rows
+    monkeypatch.setitem(rows._entries, "fg_wait_status", lambda stream: 2)
+    with pytest.raises(_native.FeatGraphError):
+        check_waits()
+
+
+def test_waits_are_not_asked_for_in_a_capture():
+    from featgraph.module import check_waits
+    graph = torch.cuda.CUDAGraph()
+    x = torch.zeros(8, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        with pytest.raises(RuntimeError, match="cannot be captured"):
+            check_waits()
+    graph.replay()
+    assert check_waits() is None and float(x[0]) == 1.0
