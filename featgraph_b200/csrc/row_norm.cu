@@ -620,6 +620,9 @@ int64_t grid_blocks(int64_t n, int32_t d) {
     return want < most ? want : most;
 }
 
+// Three arrays of the widest fp32 rows, the most that a launch asks for.
+constexpr int kWidestRows = 3 * (kMaxWidth * 4 + 16);
+
 // Sets the ring: some 180 KB of rows ahead an SM, no more than a block has rows; a very wide row takes what it takes.
 template <typename Args, typename K>
 void launch_rows(Args& a, int arrays, int size, int threads, int64_t blocks, K kernel, cudaStream_t s) {
@@ -629,7 +632,9 @@ void launch_rows(Args& a, int arrays, int size, int threads, int64_t blocks, K k
     a.stages = most < 1 ? 1 : most < kMaxStages ? most : kMaxStages;
     if (a.stages > walks) a.stages = (int32_t)walks;
     const int smem = a.stages * row;
-    if (smem > 30 * 1024) (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem < room ? room : smem);
+    // one limit for all widths of a kernel: a smaller one, set by another thread before this launch, would have it refused
+    static_assert(kWidestRows + 17 * 1024 <= 227 * 1024, "the widest rows and a kernel's own shared memory fit a block");
+    if (smem > 30 * 1024) (void)cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kWidestRows);
     kernel<<<(unsigned)blocks, threads, smem, s>>>(a);
 }
 template <typename T, int VEC, int LANES>

@@ -247,3 +247,31 @@ def test_waits_are_not_asked_for_in_a_capture():
             check_waits()
     graph.replay()
     assert check_waits() is None and float(x[0]) == 1.0
+
+
+# ---- two host threads ----
+
+def test_gradients_of_different_widths_from_two_threads():
+    """The widest fp32 rows with a residual's gradient take more shared memory than others of the same kernel: a limit that one
+    thread sets is never below what another one's launch needs."""
+    from featgraph_b200 import _native
+    call, refused = _native.lib().fg_rms_norm_backward, []
+
+    def work(d, n=2):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            h, dy, dh, dx = (torch.ones((n, d), device="cuda") for _ in range(4))
+            args = (h.data_ptr(), d, None, dy.data_ptr(), d, dh.data_ptr(), d, dx.data_ptr(), None, None, n, n, d, 1e-6, 0, 0, stream.cuda_stream)
+            for i in range(20000):
+                if call(*args):
+                    refused.append((d, i))
+                if i % 256 == 0:
+                    stream.synchronize()
+            stream.synchronize()
+
+    threads = [threading.Thread(target=work, args=(d,)) for d in (16384, 9000)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not refused, "%d launches were refused, the first %s" % (len(refused), refused[0])
