@@ -2,7 +2,8 @@
 //
 //   h = round(x + residual)      y = h * r * w,   r = 1 / sqrt(mean(h^2) + eps)
 //   8 bits: s = max|h r w| / 448 (1 where that is 0 in 32 bits),  q = e4m3(h r w / s)
-//   dx = dresidual = dh + r g - h r^3 / d * sum(g h),  g = dy w;      dw = sum over rows of dy h r
+//   dx = dresidual = dh + r (g - (h r) (r / d * sum(g h))),  g = dy w;      dw = sum over rows of dy h r
+//   (r^3 would leave the 32-bit range before dx does: without eps at rows of 1e-18)
 //
 // Bound: device memory - each array is touched once.  TPR threads own a row and hold its E values each in
 // registers between the reductions and the output, so a row is read once whatever is computed from it (its sum of
@@ -336,7 +337,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR <= 256 ? 2 : 1) nor
         if (t == 0 && row + a.stages * step < a.n) ring.request(ring.s, row + a.stages * step);
         ring.next();
         const float r = __frsqrt_rn(__fmaf_rn(ss, over_d, a.eps));
-        const float along = __fmul_rn(__fmul_rn(r, r), __fmul_rn(r, __fmul_rn(sg, over_d)));
+        const float along = __fmul_rn(r, __fmul_rn(sg, over_d));
         T* dx = static_cast<T*>(a.dx) + row * a.d;
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
@@ -346,11 +347,11 @@ __global__ void __launch_bounds__(TPR < 256 ? 256 : TPR, TPR <= 256 ? 2 : 1) nor
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     const float u = to_f32<T>(h[c].v[j]), dyj = to_f32<T>(g[c].v[j]);
-                    const float v = __fmul_rn(dyj, weight[c * VEC + j]);
-                    float w = __fmaf_rn(-u, along, __fmul_rn(r, v));
+                    const float v = __fmul_rn(dyj, weight[c * VEC + j]), unit = __fmul_rn(u, r);
+                    float w = __fmul_rn(r, __fmaf_rn(-unit, along, v));
                     if (DH) w = __fadd_rn(w, to_f32<T>(d[c].v[j]));
                     o.v[j] = from_f32<T>(w);
-                    acc[c * VEC + j] = __fmaf_rn(dyj, __fmul_rn(u, r), acc[c * VEC + j]);
+                    acc[c * VEC + j] = __fmaf_rn(dyj, unit, acc[c * VEC + j]);
                 }
                 store_pack<T, VEC>(dx + i, o);
             }
@@ -533,7 +534,7 @@ __global__ void __launch_bounds__(256) norm_narrow_grad_kernel(const NormGradArg
                     sg = __fmaf_rn(u, __fmul_rn(to_f32<T>(g.v[c].v[j]), weight[c * VEC + j]), sg);
                 }
         const float r = __frsqrt_rn(__fmaf_rn(lanes_sum<LANES>(ss), over_d, a.eps));
-        const float along = __fmul_rn(__fmul_rn(r, r), __fmul_rn(r, __fmul_rn(lanes_sum<LANES>(sg), over_d)));
+        const float along = __fmul_rn(r, __fmul_rn(lanes_sum<LANES>(sg), over_d));
 #pragma unroll
         for (int c = 0; c < NV; ++c) {
             const int i = (c * LANES + t) * VEC;
@@ -542,10 +543,11 @@ __global__ void __launch_bounds__(256) norm_narrow_grad_kernel(const NormGradArg
 #pragma unroll
                 for (int j = 0; j < VEC; ++j) {
                     const float u = to_f32<T>(h.v[c].v[j]), dyj = to_f32<T>(g.v[c].v[j]);
-                    float w = __fmaf_rn(-u, along, __fmul_rn(r, __fmul_rn(dyj, weight[c * VEC + j])));
+                    const float unit = __fmul_rn(u, r);
+                    float w = __fmul_rn(r, __fmaf_rn(-unit, along, __fmul_rn(dyj, weight[c * VEC + j])));
                     if (DH) w = __fadd_rn(w, to_f32<T>(d.v[c].v[j]));
                     o.v[j] = from_f32<T>(w);
-                    acc[c * VEC + j] = __fmaf_rn(dyj, __fmul_rn(u, r), acc[c * VEC + j]);
+                    acc[c * VEC + j] = __fmaf_rn(dyj, unit, acc[c * VEC + j]);
                 }
                 store_pack<T, VEC>(static_cast<T*>(a.dx) + row * a.d + i, o);
             }

@@ -275,3 +275,19 @@ def test_gradients_of_different_widths_from_two_threads():
     for t in threads:
         t.join()
     assert not refused, "%d launches were refused, the first %s" % (len(refused), refused[0])
+
+
+# ---- norm without eps ----
+
+@pytest.mark.parametrize("d", [24, 128, 300, 2048])
+@pytest.mark.parametrize("size", [2.0 ** -60, 2.0 ** -50, 2.0 ** 40])
+def test_norm_gradient_of_small_and_large_rows_without_eps(d, size):
+    """r = 1 / |h| reaches 1e18 and its square leaves the 32-bit range where the gradient, r times g, does not."""
+    from featgraph.module import rms_norm
+    x, dy = normal((20, d), 1, scale=size).requires_grad_(True), normal((20, d), 2, scale=1e4)
+    dx, = torch.autograd.grad(rms_norm(x, eps=0.0), x, dy)
+    h, g = x.detach().double(), dy.double()
+    r = 1 / torch.sqrt(h.pow(2).mean(1, keepdim=True))
+    first, second = r * g, h * r ** 3 * (g * h).sum(1, keepdim=True) / d
+    parts = first.abs() + h.abs() * r ** 3 * (g * h).abs().sum(1, keepdim=True) / d
+    within(dx, first - second, (first - second).abs() * U + 240 * U * parts, "dx")  # 240 u: the statistics' additions, as for rows near 1
