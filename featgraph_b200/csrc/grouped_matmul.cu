@@ -1384,6 +1384,7 @@ int fg_grouped_matmul(const void* d_x, int64_t ldx, const float* d_x_scales, con
     }
     const int64_t need = fg_grouped_matmul_workspace(d_x, ldx, d_w, w_group, w_out, w_in, d_order, num_rows, groups, inner, outer, type);
     if (workspace_bytes < need || (need && !d_workspace)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_grouped_matmul_workspace()");
+    if (need && !fg::aligned16(d_workspace)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "the workspace must start on a 16-byte boundary");
     uint8_t* work = static_cast<uint8_t*>(d_workspace);
     const Problem p{d_offsets, d_order, num_rows, x_rows, choices, groups, inner, outer, type};
     Matrix x{};
@@ -1430,6 +1431,7 @@ int fg_grouped_matmul_backward(const void* d_x, int64_t ldx, const void* d_w, in
                                                               num_rows, groups, inner, outer, type);
     if (workspace_bytes < need || (need && !d_workspace))
         return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_grouped_matmul_backward_workspace()");
+    if (need && !fg::aligned16(d_workspace)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "the workspace must start on a 16-byte boundary");
     uint8_t* work = static_cast<uint8_t*>(d_workspace);
     const Problem p{d_offsets, d_order, num_rows, x_rows, choices, groups, inner, outer, type};
     // dW needs dy in parts; alone, dx may take it as it is

@@ -576,6 +576,8 @@ int fg_group_rows(const int32_t* d_keys, int64_t num_entries, int32_t num_groups
     if (!d_offsets || (num_entries && (!d_keys || !d_order || !d_position))) return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
     if (workspace_bytes < fg_group_rows_workspace(num_entries, num_groups) || (fg_group_rows_workspace(num_entries, num_groups) && !d_workspace))
         return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_group_rows_workspace()");
+    if (fg_group_rows_workspace(num_entries, num_groups) && !fg::aligned16(d_workspace))
+        return fg::fail(FG_ERR_INVALID_ARGUMENT, "the workspace must start on a 16-byte boundary");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (num_entries == 0) {
         FG_CUDA_TRY(cudaMemsetAsync(d_offsets, 0, ((size_t)num_groups + 1) * 4, s));
@@ -615,6 +617,8 @@ int fg_route(const void* d_logits, int64_t ld, float* d_weights, int32_t* d_expe
     if (!d_logits || !d_weights || !d_experts || (d_offsets && (!d_order || !d_position))) return fg::fail(FG_ERR_INVALID_ARGUMENT, "NULL array argument");
     if (d_offsets && workspace_bytes < fg_group_rows_workspace(n * k, experts))
         return fg::fail(FG_ERR_INVALID_ARGUMENT, "workspace smaller than fg_group_rows_workspace()");
+    if (d_offsets && fg_group_rows_workspace(n * k, experts) && !fg::aligned16(d_workspace))
+        return fg::fail(FG_ERR_INVALID_ARGUMENT, "the workspace must start on a 16-byte boundary");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const RouteArgs a{d_logits, ld, n, experts, k, scoring == FG_SCORE_SIGMOID, normalize != 0, d_weights, d_experts};
     if (d_offsets && n <= kOneBlockRows) {

@@ -338,7 +338,8 @@ int fg_coo_validate(const int32_t* d_row, const int32_t* d_col, int64_t n_rows, 
  * types or relations computes densely before and after it aggregates.  Value types are FG_F32, FG_F16, FG_BF16 and,
  * for rows held in 8 bits with a scale each, FG_E4M3.  Sums, statistics and accumulators are fp32; each output is
  * rounded once to its type unless stated.  No atomics on values: the same bits on every run.  Strides in values
- * (0 = dense).  Lists are bounds-checked in the kernels: a wrong entry gives wrong rows, not a wrong address.
+ * (0 = dense); workspaces start on a 16-byte boundary, other arrays on one of their type.  Lists are bounds-checked in the
+ * kernels: a wrong entry gives wrong rows, not a wrong address.
  * -------------------------------------------------------------------------------------- */
 #define FG_F32 0
 #define FG_F16 1
@@ -387,7 +388,7 @@ int64_t fg_group_rows_workspace(int64_t num_entries, int32_t num_groups);
 int fg_group_rows(const int32_t* d_keys, int64_t num_entries, int32_t num_groups, int32_t* d_offsets, int32_t* d_order,
                   int32_t* d_position, void* d_workspace, int64_t workspace_bytes, void* stream);
 
-/* Workspaces: as large as the *_workspace call says for the same arguments.
+/* Workspaces: as large as the *_workspace call says for the same arguments, on a 16-byte boundary.
  * y[p, o] = sum over i of x[row(p), i] * w[g, o, i] for the rows p of each group g; rows in no group are 0.
  * row(p) = p where d_order is NULL, else d_order[p] / choices.  w[g, o, i] is d_w[g w_group + o w_out + i w_in].
  * FG_E4M3: times d_x_scales[row(p)] * d_w_scales[g * outer + o], output of out_type.  y dense, [num_rows, outer].
