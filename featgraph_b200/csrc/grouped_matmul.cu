@@ -1235,6 +1235,7 @@ int64_t partial_bytes(int64_t m, int32_t groups, int32_t inner, int32_t outer) {
 
 int check_product(int64_t m, int64_t x_rows, int32_t choices, int32_t groups, int32_t inner, int32_t outer, int32_t type) {
     if (m < 0 || m > INT_MAX - 1024 || x_rows < 0 || x_rows > INT_MAX || choices < 1 || groups < 1 || groups > kMaxGroups || inner < 1 || outer < 1 ||
+        inner > INT_MAX - 1024 || outer > INT_MAX - 1024 ||
         (type == FG_F32 && (m > INT_MAX / 4 || x_rows > INT_MAX / 4)))
         return fg::fail(FG_ERR_INVALID_ARGUMENT, "bad sizes rows=%lld of %lld choices=%d groups=%d inner=%d outer=%d (groups <= %d)",
                         (long long)m, (long long)x_rows, choices, groups, inner, outer, kMaxGroups);

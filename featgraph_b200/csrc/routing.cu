@@ -503,7 +503,7 @@ int launch_combine_grad(const CombineArgs& a, bool vec, cudaStream_t s) {
 }
 
 int check_combine(int64_t n, int32_t k, int32_t d, int32_t type) {
-    if (n < 0 || k < 1 || k > kMaxChoices || d < 1 || n > INT_MAX / k)
+    if (n < 0 || k < 1 || k > kMaxChoices || d < 1 || d > INT_MAX - 1024 || n > INT_MAX / k)
         return fg::fail(FG_ERR_INVALID_ARGUMENT, "bad sizes n=%lld k=%d d=%d (1 <= k <= %d, n k < 2^31)", (long long)n, k, d, kMaxChoices);
     if (!fg::float_type(type)) return fg::fail(FG_ERR_INVALID_ARGUMENT, "unknown value type %d", type);
     return FG_OK;

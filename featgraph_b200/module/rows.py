@@ -31,6 +31,7 @@ _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.float8_e4
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 _SCORING = {"softmax": 0, "sigmoid": 1}
 MAX_WIDTH, MAX_GROUPS, MAX_CHOICES = 16384, 1024, 32
+MAX_COLUMNS = 2 ** 31 - 1025  # of products and sums: counted in 32 bits, up to the end of the last tile
 
 
 class QuantizedRows(NamedTuple):
@@ -463,7 +464,7 @@ def grouped_matmul(x, weight, groups, gather=False, out_dtype=None):
         raise ValueError("weight has %d groups, the rows %d" % (weight.shape[0], groups.num_groups))
     if weight.shape[2] != x.shape[1]:
         raise ValueError("weight takes %d values, the rows have %d" % (weight.shape[2], x.shape[1]))
-    if weight.shape[1] < 1 or weight.shape[2] < 1:
+    if not 1 <= weight.shape[1] <= MAX_COLUMNS or not 1 <= weight.shape[2] <= MAX_COLUMNS:
         raise ValueError("weight has shape %s" % (tuple(weight.shape),))
     want = groups.num_rows if gather else groups.num_entries
     if x.shape[0] != want:
@@ -515,7 +516,7 @@ def combine_rows(y, groups, weights=None):
     if not isinstance(groups, RowGroups):
         raise TypeError("groups: expected RowGroups (group_rows, route), got %r" % (type(groups),))
     _tensor(y, "y", _FLOATS, 2)
-    if y.shape[0] != groups.num_entries or y.shape[1] < 1:
+    if y.shape[0] != groups.num_entries or not 1 <= y.shape[1] <= MAX_COLUMNS:
         raise ValueError("y must have a row for each of %d slots, has shape %s" % (groups.num_entries, tuple(y.shape)))
     if weights is not None:
         _tensor(weights, "weights", (torch.float32,), 2)

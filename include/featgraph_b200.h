@@ -339,7 +339,7 @@ int fg_coo_validate(const int32_t* d_row, const int32_t* d_col, int64_t n_rows, 
  * for rows held in 8 bits with a scale each, FG_E4M3.  Sums, statistics and accumulators are fp32; each output is
  * rounded once to its type unless stated.  No atomics on values: the same bits on every run.  Strides in values
  * (0 = dense); workspaces start on a 16-byte boundary, other arrays on one of their type.  Lists are bounds-checked in the
- * kernels: a wrong entry gives wrong rows, not a wrong address.
+ * kernels: a wrong entry gives wrong rows, not a wrong address.  Widths are below 2^31 - 1024.
  * -------------------------------------------------------------------------------------- */
 #define FG_F32 0
 #define FG_F16 1
