@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD, GATHER>, 1)
             w.row = tile % rows_tiles * kRows + rank * kTileRows;
             w.col = tile / rows_tiles * BN;
             w.begin = a.split ? first + part * a.split : first;
-            w.end = a.split ? min(w.begin + a.split, stop_at) : stop_at;
+            w.end = a.split ? (int)min((int64_t)w.begin + a.split, (int64_t)stop_at) : stop_at;
             w.chunks = max(w.end - w.begin + kChunk - 1, 0) / kChunk;
         } else {
             // up to 16 row tiles share a column tile's weights while they are in L2, then the next column tile

@@ -291,3 +291,21 @@ def test_norm_gradient_of_small_and_large_rows_without_eps(d, size):
     first, second = r * g, h * r ** 3 * (g * h).sum(1, keepdim=True) / d
     parts = first.abs() + h.abs() * r ** 3 * (g * h).abs().sum(1, keepdim=True) / d
     within(dx, first - second, (first - second).abs() * U + 240 * U * parts, "dx")  # 240 u: the statistics' additions, as for rows near 1
+
+
+# ---- row numbers near 2^31 ----
+
+def test_weight_gradient_of_almost_2_to_the_31_rows():
+    """A group's last part ends with the group, also where row numbers and part sizes add up to more than 32 bits hold."""
+    from featgraph.module import RowGroups, grouped_matmul
+    m, width = 2 ** 31 - 2048, 8
+    x = torch.zeros((m, width), device="cuda", dtype=torch.bfloat16)
+    x[-5:] = 1
+    x[:3] = 2
+    lists = torch.empty(m, device="cuda", dtype=torch.int32)  # not read: the rows are in slot order
+    groups = RowGroups(torch.tensor([0, m - 3000, m], dtype=torch.int32, device="cuda"), lists, lists.view(m, 1))
+    w = torch.ones((2, width, width), device="cuda", dtype=torch.bfloat16).requires_grad_(True)
+    y = grouped_matmul(x, w, groups)
+    assert bool((y.detach()[-5:] == 8).all()) and bool((y.detach()[:3] == 16).all()) and not bool(y.detach()[-6].any())
+    dw, = torch.autograd.grad(y, w, y.detach())
+    assert bool((dw[0] == 3 * 16 * 2).all()) and bool((dw[1] == 5 * 8).all()), dw[:, 0, 0]  # whole numbers below 2^8: exact
