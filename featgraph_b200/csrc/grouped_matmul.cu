@@ -348,11 +348,13 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD, GATHER>, 1)
         t.sources[threadIdx.x] = r < a.x_rows ? r : -1;
     }
 
-    // groups' first slots and tile counts, scanned: thread i takes groups [i * each, (i + 1) * each)
+    // groups' first slots and tile counts, scanned: thread i takes groups [i * each, (i + 1) * each).  Lists whose groups overlap
+    // can add up to more tiles than 32 bits count: the sums end at INT_MAX, so that the table never falls.
     {
         constexpr int kAll = kThreads<KIND, WGRAD, GATHER>;
         const int each = (a.groups + kAll - 1) / kAll, from = min((int)threadIdx.x * each, a.groups), to = min(from + each, a.groups);
         const int64_t unit = WGRAD ? (a.split ? a.split : (int64_t)INT_MAX) : kRows;
+        auto plus = [](int x, int y) { return (int)min((uint32_t)x + (uint32_t)y, (uint32_t)INT_MAX); };
         int own = 0;
         for (int g = from; g < to; ++g) {
             const int64_t b = min((int64_t)max(a.offsets[g], 0), a.m), e = min((int64_t)max(a.offsets[g + 1], 0), a.m);
@@ -364,17 +366,17 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD, GATHER>, 1)
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
+            if (lane >= o) sum = plus(sum, v);
         }
         if (lane == 31) t.warp_sums[warp] = sum;
         __syncthreads();
-        int before = sum - own;
-        for (int w = 0; w < warp; ++w) before += t.warp_sums[w];
+        int before = sum < INT_MAX ? sum - own : sum;
+        for (int w = 0; w < warp; ++w) before = plus(before, t.warp_sums[w]);
         for (int g = from; g < to; ++g) {
             const int64_t b = t.start[g], e = min((int64_t)max(a.offsets[g + 1], 0), a.m);
             const int64_t n = max(e - b, (int64_t)0);
             t.tiles[g] = before;
-            before += (int)(WGRAD ? max((n + unit - 1) / unit, (int64_t)1) : (n + unit - 1) / unit);
+            before = plus(before, (int)(WGRAD ? max((n + unit - 1) / unit, (int64_t)1) : (n + unit - 1) / unit));
         }
         if (threadIdx.x == kAll - 1) {
             t.tiles[a.groups] = before;
@@ -410,7 +412,7 @@ __global__ void __launch_bounds__(kThreads<KIND, WGRAD, GATHER>, 1)
         w.group = cursor;
         if (WGRAD) {
             const int part = (int)(local / per_unit), tile = (int)(local - (int64_t)part * per_unit);
-            w.unit = min(t.tiles[cursor] + part, a.units - 1);  // lists that overlap: wrong sums, no wrong address
+            w.unit = (int)min((int64_t)t.tiles[cursor] + part, (int64_t)a.units - 1);  // lists that overlap: wrong sums, no wrong address
             w.row = tile % rows_tiles * kRows + rank * kTileRows;
             w.col = tile / rows_tiles * BN;
             w.begin = a.split ? first + part * a.split : first;
@@ -920,14 +922,14 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
     __shared__ int first, count;
     const int g = blockIdx.y;  // `units`: partial sums that there are
     if (threadIdx.x == 0) {
-        int before = 0, n = 0;
+        int64_t before = 0, n = 0;
         for (int q = 0; q <= g; ++q) {
             const int64_t b = min((int64_t)max(offsets[q], 0), m), e = min((int64_t)max(offsets[q + 1], 0), m);
-            n = (int)max((max(e - b, (int64_t)0) + split - 1) / split, (int64_t)1);
+            n = max((max(e - b, (int64_t)0) + split - 1) / split, (int64_t)1);
             if (q < g) before += n;
         }
-        first = min(before, units - 1);
-        count = min(n, units - first);
+        first = (int)min(before, (int64_t)units - 1);
+        count = (int)min(n, (int64_t)units - first);
     }
     __syncthreads();
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < cells; i += (int64_t)gridDim.x * 256) {
