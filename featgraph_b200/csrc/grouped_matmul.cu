@@ -25,8 +25,8 @@
 // chunk of 64 - the five small ones first, then four steps at full size - and the output warps add the chunks in
 // registers, rounding to nearest.
 //
-// Rows that are gathered (slot p reads row order[p] / choices) are first copied into slot order, unless there is one column
-// tile only: every column tile reads them again, and row-gather TMA loads (tile::gather4, four rows an instruction) move a
+// Rows that are gathered (slot p reads row order[p] / choices) are first copied into slot order, unless there are few columns
+// (rows_gathered): every column tile reads them again, and row-gather TMA loads (tile::gather4, four rows an instruction) move a
 // 128-row tile at a fraction of the tile loads' rate.  Measured at 65536 x 2048 x 4096 in bf16: 2767 us with gather loads in
 // the ring, 922 us for rows in slot order, the copy about 70 us; dW 8512 against 1241 us.  The same kernel copies an
 // operand that TMA cannot read (a row pitch or a start off the 16-byte grid, two strides above 1) and cuts fp32 into parts.
@@ -949,7 +949,8 @@ __global__ void __launch_bounds__(256) join_kernel(const float* __restrict__ par
 
 // dst[g][r][c], c < pitch, from src at g s0 + r s1 + c s2: the same type, or the three bf16 parts of an fp32 value in
 // three consecutive copies.  With an order (one group), row r comes from row order[r] / choices; a slot that names no row
-// gets zeros.  16 bytes of output (of each part) a thread and step; 2^shift threads share a row.  Bound: device memory.
+// gets zeros.  16 bytes of output (of each part) a thread and step; 2^shift threads share a row.  Bound: device memory in 16 and
+// 32 bits; 8-bit rows are bound by instructions (16384 rows of 4096: 33 us, ALU pipe 67 % busy, DRAM 20 %).
 struct PackArgs {
     const void* src;
     void* dst;
@@ -1126,10 +1127,12 @@ int launch_few(const FewArgs& a, cudaStream_t s) {
     return FG_OK;
 }
 
-// Rows that the product gathers itself: 16- or 8-bit ones on the 16-byte grid, many of them for one column tile, where the
-// copy in slot order would be most of the work.  16-byte copies by a few warps fill a stage more slowly than TMA does:
-// 55960 slots, 2160 to 64 in bf16 50 us, by a copy first 134; 32854, 1776 to 208 48 and 79; 65536, 256 to 256 26 and 31; but
-// 65536, 2048 to 4096 1230 and 912, and 2000, 1024 to 512 20 and 16.
+// Rows that the product gathers itself: 16- or 8-bit ones on the 16-byte grid, many of them for at most 256 columns, where the
+// copy in slot order would be much of the work.  16-byte copies by a few warps fill a stage more slowly than TMA does, and
+// every column tile (one from some 18000 slots on, up to four below) fetches its rows again.  Gathered / copied first, in bf16:
+// 55960 slots, 2160 to 64 50 / 134 us; 32854, 1776 to 208 48 / 79; 65536, 256 to 256 26 / 31; but 65536, 2048 to 4096
+// 1230 / 912, and 2000, 1024 to 512 20 / 16.  Several tiles, 4096 to 256: 16384 68 / 86, 12000 64 / 69, 8192 in two groups
+// 55 / 50, in sixteen 34 / 46; 1024 to 256: 16384 22 / 23, 12000 22 / 20, 8192 19.5 / 17.4 and 14.4 / 15.5.
 bool rows_gathered(const void* p, int64_t ld, const int32_t* order, int64_t m, int32_t outer, int32_t type) {
     return order && outer <= 256 && m >= 8192 && loadable(p, ld, 0, type);
 }
